@@ -29,7 +29,12 @@ EXPORTED = ("mle_q8_0_abi_version", "mle_q8_0_linear", "mle_q8_0_linear_ex",
             "mle_q8_0_linear_multi_tiled", "mle_q8_0_workspace_size", "mle_workspace_reserve",
             "mle_workspace_info", "mle_workspace_plan_growth", "mle_q8_0_linear_noalloc",
             "mle_q8_0_dequantize", "mle_q8_0_linear_bias_bf16",
-            "mle_q8_0_linear_tiled_bias_bf16", "mle_probe_stream_read")
+            "mle_q8_0_linear_tiled_bias_bf16", "mle_probe_stream_read",
+            "mle_paged_plan", "mle_rope_table", "mle_paged_kv_write", "mle_paged_attention",
+            "mle_paged_attention_workspace_size")
+
+KV_TYPES = {"f16": 0, "bf16": 1, "int8": 2}
+ROPE_MODES = {"pairs": 0, "halves": 1, "none": 0}
 
 OP_LINEAR, OP_LINEAR_SWIGLU, OP_LINEAR_MULTI, OP_MATMUL = 0, 1, 2, 3
 
@@ -116,6 +121,19 @@ def load() -> ctypes.CDLL:
     lib.mle_workspace_info.argtypes = [_vp, _vp, _vp, _vp]
     lib.mle_workspace_plan_growth.restype = _i
     lib.mle_workspace_plan_growth.argtypes = [_sz, _sz, _sz, _sz, _vp, _vp]
+    lib.mle_paged_plan.restype = _i
+    lib.mle_paged_plan.argtypes = [_vp, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp,
+                                   _vp, _vp, _vp, _vp]
+    lib.mle_rope_table.restype = _i
+    lib.mle_rope_table.argtypes = [_vp, _i, _i, ctypes.c_double, _vp, _vp]
+    lib.mle_paged_kv_write.restype = _i
+    lib.mle_paged_kv_write.argtypes = [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i,
+                                       _i, _vp, _vp, _i, _vp]
+    lib.mle_paged_attention.restype = _i
+    lib.mle_paged_attention.argtypes = [_vp, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _i,
+                                        _vp, _vp, _i, _i, _vp]
+    lib.mle_paged_attention_workspace_size.restype = _i
+    lib.mle_paged_attention_workspace_size.argtypes = [_vp, _i, _i, _i, _vp, _vp]
     _lib = lib
     return lib
 
@@ -419,3 +437,133 @@ def workspace_plan_growth(cap_bytes, cap_counters, need_bytes, need_counters):
     rc = load().mle_workspace_plan_growth(cap_bytes, cap_counters, need_bytes, need_counters,
                                           ctypes.byref(nb), ctypes.byref(nc))
     return bool(rc), nb.value, nc.value
+
+
+# The paged KV cache (include/mle_paged.h).
+
+class _CacheStruct(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+                ("type", ctypes.c_int32), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+class PagedCache:
+    """One layer's paged KV cache: the buffers (kept alive here) and their shape.
+
+    kv_type: "f16", "bf16" or "int8" (or the header's number); k and v hold num_pages *
+    kv_heads * page_size * head_dim elements, the int8 scales num_pages * kv_heads *
+    page_size.  :meth:`allocate` makes zeroed ones."""
+
+    def __init__(self, kv_type, num_pages, page_size, kv_heads, head_dim, k, v, k_scale=None,
+                 v_scale=None):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.struct = _CacheStruct(_addr(k), _addr(v), _addr(k_scale), _addr(v_scale),
+                                   KV_TYPES.get(kv_type, kv_type), num_pages, page_size,
+                                   kv_heads, head_dim)
+        self._as_parameter_ = ctypes.addressof(self.struct)
+
+    @classmethod
+    def allocate(cls, kv_type, num_pages, page_size, kv_heads, head_dim, device="cuda"):
+        import torch
+        dtype = {"f16": torch.float16, "bf16": torch.bfloat16, "int8": torch.int8}[kv_type]
+        cells = num_pages * kv_heads * page_size
+        bufs = [torch.zeros(cells * head_dim, dtype=dtype, device=device) for _ in range(2)]
+        if kv_type == "int8":
+            bufs += [torch.zeros(cells, dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(kv_type, num_pages, page_size, kv_heads, head_dim, *bufs)
+
+
+def _row_stride(t, stride, row):
+    """A row stride in floats: the given one, the tensor's, or (an address) the row's size."""
+    if stride is not None:
+        return stride
+    if t is None or isinstance(t, int) or t.dim() < 2:
+        return row
+    return t.stride(0)
+
+
+def paged_plan_status(cached_lens, new_lens, sequences, block_table, max_pages, page_size,
+                      num_pages, free_pages, free_count, free_count_out, tokens, kv_lens,
+                      cu_tokens, positions, slots, granted, stream=None):
+    rc = load().mle_paged_plan(_addr(cached_lens), _addr(new_lens), sequences,
+                               _addr(block_table), max_pages, page_size, num_pages,
+                               _addr(free_pages), _addr(free_count), _addr(free_count_out),
+                               tokens, _addr(kv_lens), _addr(cu_tokens), _addr(positions),
+                               _addr(slots), _addr(granted), _stream(stream))
+    return _status(rc)
+
+
+def paged_plan(cached_lens, new_lens, sequences, block_table, max_pages, page_size, num_pages,
+               free_pages, free_count, free_count_out, tokens, kv_lens, cu_tokens, positions,
+               slots, granted, stream=None) -> None:
+    """Pages for a step's new tokens: block_table, the free stack, kv_lens, cu_tokens and each
+    row's position and slot, all int32 on the device."""
+    _raise(paged_plan_status(cached_lens, new_lens, sequences, block_table, max_pages,
+                             page_size, num_pages, free_pages, free_count, free_count_out,
+                             tokens, kv_lens, cu_tokens, positions, slots, granted, stream)[0])
+
+
+def rope_table_status(table, positions, rope_dim, theta=10000.0, freq_factors=None,
+                      stream=None):
+    rc = load().mle_rope_table(_addr(table), positions, rope_dim, theta, _addr(freq_factors),
+                               _stream(stream))
+    return _status(rc)
+
+
+def rope_table(table, positions, rope_dim, theta=10000.0, freq_factors=None,
+               stream=None) -> None:
+    """table [positions, rope_dim/2, 2] fp32: (cos, sin) of every position's angles."""
+    _raise(rope_table_status(table, positions, rope_dim, theta, freq_factors, stream)[0])
+
+
+def paged_kv_write_status(cache, q, q_out, heads, k, v, rope, rope_positions, rope_dim,
+                          rope_mode, positions, slots, tokens, q_stride=None,
+                          q_out_stride=None, k_stride=None, v_stride=None, stream=None):
+    dim = cache.struct.head_dim
+    row, kv_row = heads * dim, cache.struct.kv_heads * dim
+    rc = load().mle_paged_kv_write(
+        cache, _addr(q), _row_stride(q, q_stride, row), _addr(q_out),
+        _row_stride(q_out, q_out_stride, row), heads, _addr(k),
+        _row_stride(k, k_stride, kv_row), _addr(v), _row_stride(v, v_stride, kv_row),
+        _addr(rope), rope_positions, rope_dim, ROPE_MODES.get(rope_mode, rope_mode),
+        _addr(positions), _addr(slots), tokens, _stream(stream))
+    return _status(rc)
+
+
+def paged_kv_write(cache, q, q_out, heads, k, v, rope, rope_positions, rope_dim, rope_mode,
+                   positions, slots, tokens, q_stride=None, q_out_stride=None, k_stride=None,
+                   v_stride=None, stream=None) -> None:
+    """q_out = rotated q; rotated k, and v, into their slots of the cache.  rope_mode "pairs"
+    or "halves" (ignored where rope is None); row strides default to the tensors'."""
+    _raise(paged_kv_write_status(cache, q, q_out, heads, k, v, rope, rope_positions, rope_dim,
+                                 rope_mode, positions, slots, tokens, q_stride, q_out_stride,
+                                 k_stride, v_stride, stream)[0])
+
+
+def paged_attention_status(cache, q, out, heads, scale, window, block_table, max_pages, kv_lens,
+                           cu_tokens, sequences, tokens, q_stride=None, out_stride=None,
+                           stream=None):
+    row = heads * cache.struct.head_dim
+    rc = load().mle_paged_attention(
+        cache, _addr(q), _row_stride(q, q_stride, row), _addr(out),
+        _row_stride(out, out_stride, row), heads, scale, window, _addr(block_table), max_pages,
+        _addr(kv_lens), _addr(cu_tokens), sequences, tokens, _stream(stream))
+    return _status(rc)
+
+
+def paged_attention(cache, q, out, heads, scale, window, block_table, max_pages, kv_lens,
+                    cu_tokens, sequences, tokens, q_stride=None, out_stride=None,
+                    stream=None) -> None:
+    """out[row] = attention of the step's rows over the cache (causal; window 0: no limit)."""
+    _raise(paged_attention_status(cache, q, out, heads, scale, window, block_table, max_pages,
+                                  kv_lens, cu_tokens, sequences, tokens, q_stride, out_stride,
+                                  stream)[0])
+
+
+def paged_attention_workspace_size(cache, heads, sequences, tokens):
+    """(bytes, counters) that hold any attention call of up to these sizes."""
+    b, c = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _raise(load().mle_paged_attention_workspace_size(cache, heads, sequences, tokens,
+                                                     ctypes.byref(b), ctypes.byref(c)))
+    return b.value, c.value

@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <map>
 #include <vector>
@@ -18,8 +19,10 @@
 #include <tuple>
 #include <utility>
 
+#include "../../include/mle_paged.h"
 #include "../../include/mle_q8_0.h"
 #include "launch.hpp"
+#include "paged.hpp"
 
 namespace {
 
@@ -68,11 +71,89 @@ int check_align(const char* ctx, const void* p, uintptr_t a, const char* name) {
   return MLE_OK;
 }
 
+int check_ptr(const char* ctx, const void* p, const char* name) {
+  return check_ptrs(ctx, p, name, p, name, p, name);
+}
+
 #define MLE_TRY(expr)          \
   do {                         \
     const int _rc = (expr);    \
     if (_rc != MLE_OK) return _rc; \
   } while (0)
+
+// Checks of the paged KV cache's calls (include/mle_paged.h).
+constexpr int kPagedMax = 1 << 30;
+
+int check_tokens(const char* ctx, int tokens) {
+  if (tokens < 0)
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": tokens must not be negative");
+  if (tokens >= kPagedMax)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": tokens must fit 30 bits");
+  return MLE_OK;
+}
+
+int check_rows(const char* ctx, const float* p, int stride, int64_t row, const char* name) {
+  MLE_TRY(check_align(ctx, p, 16, name));
+  if (stride < row || stride % 4 != 0)
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": " + name +
+                                          " stride must be a multiple of 4 and at least " +
+                                          std::to_string(row));
+  return MLE_OK;
+}
+
+int check_cache_sizes(const char* ctx, const mle_paged_cache& c) {
+  MLE_TRY(check_positive(ctx, c.num_pages, "num_pages"));
+  MLE_TRY(check_positive(ctx, c.page_size, "page_size"));
+  MLE_TRY(check_positive(ctx, c.kv_heads, "kv_heads"));
+  if (c.type != MLE_KV_F16 && c.type != MLE_KV_BF16 && c.type != MLE_KV_INT8)
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": unknown cache type " + std::to_string(c.type));
+  if (c.head_dim != 64 && c.head_dim != 96 && c.head_dim != 128 && c.head_dim != 256)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": head_dim must be 64, 96, 128 or 256, got " +
+                                     std::to_string(c.head_dim));
+  if (c.page_size % mle::kKvTile != 0 || c.page_size > 1024)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": page_size must be a multiple of 16 up to 1024, got " +
+                                     std::to_string(c.page_size));
+  if ((int64_t)c.num_pages * c.page_size > INT32_MAX || c.kv_heads > 65535)
+    return fail(MLE_UNSUPPORTED,
+                std::string("hip ") + ctx +
+                    ": num_pages * page_size must fit 31 bits, kv_heads be at most 65535");
+  return MLE_OK;
+}
+
+int check_cache(const char* ctx, const mle_paged_cache* c, mle::PagedCache* out) {
+  MLE_TRY(check_ptr(ctx, c, "cache"));
+  MLE_TRY(check_cache_sizes(ctx, *c));
+  MLE_TRY(check_ptrs(ctx, c->k, "cache k", c->v, "cache v", c->v, "cache v"));
+  MLE_TRY(check_align(ctx, c->k, 16, "cache k"));
+  MLE_TRY(check_align(ctx, c->v, 16, "cache v"));
+  if (c->type == MLE_KV_INT8) {
+    MLE_TRY(check_ptr(ctx, c->k_scale, "cache k_scale"));
+    MLE_TRY(check_ptr(ctx, c->v_scale, "cache v_scale"));
+    MLE_TRY(check_align(ctx, c->k_scale, 16, "cache k_scale"));
+    MLE_TRY(check_align(ctx, c->v_scale, 16, "cache v_scale"));
+  }
+  *out = mle::PagedCache{c->k,         c->v,         c->k_scale,  c->v_scale, (mle::KvType)c->type,
+                         c->num_pages, c->page_size, c->kv_heads, c->head_dim};
+  return MLE_OK;
+}
+
+int check_attention_sizes(const char* ctx, const mle_paged_cache* c, int heads, int sequences,
+                          int tokens) {
+  MLE_TRY(check_cache_sizes(ctx, *c));
+  MLE_TRY(check_positive(ctx, heads, "heads"));
+  MLE_TRY(check_positive(ctx, sequences, "sequences"));
+  MLE_TRY(check_tokens(ctx, tokens));
+  if (heads % c->kv_heads != 0)
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": heads must be a multiple of kv_heads");
+  if (heads / c->kv_heads > 64)
+    return fail(MLE_UNSUPPORTED,
+                std::string("hip ") + ctx + ": heads / kv_heads must be at most 64");
+  return MLE_OK;
+}
 
 int validate_linear(const float* x, const uint8_t* w, const void* bias, float* y,
                     int M, int N, int K, uintptr_t bias_align = 4) {
@@ -1128,6 +1209,167 @@ int mle_q8_0_f16_decode(const uint16_t* bits, float* out, int64_t n, hipStream_t
   if (n < 0) return fail(MLE_INVALID_ARGUMENT, "hip f16_decode: n must not be negative");
   return check_launch(mle::launch_f16_decode(bits, out, n, stream),
                       "hip f16_decode launch failed");
+}
+
+// ---- paged KV cache (include/mle_paged.h) ----
+
+int mle_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int sequences,
+                   int32_t* block_table, int max_pages, int page_size, int num_pages,
+                   int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
+                   int tokens, int32_t* kv_lens, int32_t* cu_tokens, int32_t* positions,
+                   int32_t* slots, int32_t* granted, hipStream_t stream) {
+  const char* ctx = "paged_plan";
+  const struct { const void* p; const char* name; bool need; } bufs[] = {
+      {cached_lens, "cached_lens", true}, {new_lens, "new_lens", true},
+      {block_table, "block_table", true}, {free_pages, "free_pages", true},
+      {free_count, "free_count", true},   {free_count_out, "free_count_out", true},
+      {kv_lens, "kv_lens", true},         {cu_tokens, "cu_tokens", true},
+      {granted, "granted", true},         {positions, "positions", tokens > 0},
+      {slots, "slots", tokens > 0}};
+  for (const auto& b : bufs) {
+    if (b.need) MLE_TRY(check_ptr(ctx, b.p, b.name));
+    MLE_TRY(check_align(ctx, b.p, 4, b.name));
+  }
+  MLE_TRY(check_positive(ctx, sequences, "sequences"));
+  MLE_TRY(check_positive(ctx, max_pages, "max_pages"));
+  MLE_TRY(check_positive(ctx, page_size, "page_size"));
+  MLE_TRY(check_positive(ctx, num_pages, "num_pages"));
+  MLE_TRY(check_tokens(ctx, tokens));
+  if ((int64_t)sequences * max_pages > INT32_MAX || (int64_t)num_pages * page_size > INT32_MAX ||
+      num_pages >= kPagedMax || max_pages >= kPagedMax)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": sequences * max_pages and num_pages * page_size must "
+                                     "fit 31 bits, num_pages and max_pages 30");
+  const mle::PlanArgs a{cached_lens, new_lens,   sequences,  block_table,    max_pages,
+                        page_size,   num_pages,  free_pages, free_count,     free_count_out,
+                        tokens,      kv_lens,    cu_tokens,  positions,      slots,
+                        granted};
+  return check_launch(mle::launch_paged_plan(a, stream), "hip paged_plan launch failed");
+}
+
+int mle_rope_table(float* table, int positions, int rope_dim, double theta,
+                   const float* freq_factors, hipStream_t stream) {
+  const char* ctx = "rope_table";
+  MLE_TRY(check_ptr(ctx, table, "table"));
+  MLE_TRY(check_positive(ctx, positions, "positions"));
+  MLE_TRY(check_positive(ctx, rope_dim, "rope_dim"));
+  if (rope_dim % 2 != 0)
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": rope_dim must be even");
+  if (!(theta > 0.0) || !std::isfinite(theta))
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": theta must be positive and finite");
+  MLE_TRY(check_align(ctx, table, 16, "table"));
+  MLE_TRY(check_align(ctx, freq_factors, 4, "freq_factors"));
+  return check_launch(
+      mle::launch_rope_table(table, positions, rope_dim, theta, freq_factors, stream),
+      "hip rope_table launch failed");
+}
+
+int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_stride,
+                       float* q_out, int q_out_stride, int heads, const float* k, int k_stride,
+                       const float* v, int v_stride, const float* rope, int rope_positions,
+                       int rope_dim, int rope_mode, const int32_t* positions,
+                       const int32_t* slots, int tokens, hipStream_t stream) {
+  const char* ctx = "paged_kv_write";
+  mle::KvWriteArgs a{};
+  MLE_TRY(check_cache(ctx, cache, &a.cache));
+  MLE_TRY(check_positive(ctx, heads, "heads"));
+  MLE_TRY(check_tokens(ctx, tokens));
+  MLE_TRY(check_ptrs(ctx, q, "q", q_out, "q_out", k, "k"));
+  MLE_TRY(check_ptrs(ctx, v, "v", slots, "slots", slots, "slots"));
+  const int64_t row = (int64_t)heads * cache->head_dim;
+  const int64_t kv_row = (int64_t)cache->kv_heads * cache->head_dim;
+  MLE_TRY(check_rows(ctx, q, q_stride, row, "q"));
+  MLE_TRY(check_rows(ctx, q_out, q_out_stride, row, "q_out"));
+  MLE_TRY(check_rows(ctx, k, k_stride, kv_row, "k"));
+  MLE_TRY(check_rows(ctx, v, v_stride, kv_row, "v"));
+  MLE_TRY(check_align(ctx, slots, 4, "slots"));
+  if (rope != nullptr) {
+    MLE_TRY(check_ptr(ctx, positions, "positions"));
+    MLE_TRY(check_align(ctx, positions, 4, "positions"));
+    MLE_TRY(check_align(ctx, rope, 16, "rope"));
+    MLE_TRY(check_positive(ctx, rope_positions, "rope_positions"));
+    MLE_TRY(check_positive(ctx, rope_dim, "rope_dim"));
+    if (rope_dim % 8 != 0 || rope_dim > cache->head_dim)
+      return fail(MLE_INVALID_ARGUMENT,
+                  std::string("hip ") + ctx +
+                      ": rope_dim must be a multiple of 8 and at most head_dim");
+    if (rope_mode != MLE_ROPE_PAIRS && rope_mode != MLE_ROPE_HALVES)
+      return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": unknown rope_mode " +
+                                            std::to_string(rope_mode));
+  }
+  if (tokens == 0) return ok();
+  a.q = q;
+  a.q_out = q_out;
+  a.k = k;
+  a.v = v;
+  a.rope = rope;
+  a.positions = positions;
+  a.slots = slots;
+  a.q_stride = q_stride;
+  a.q_out_stride = q_out_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.heads = heads;
+  a.rope_positions = rope_positions;
+  a.rope_dim = rope != nullptr ? rope_dim : 0;
+  a.rope_halves = rope_mode == MLE_ROPE_HALVES;
+  a.tokens = tokens;
+  return check_launch(mle::launch_paged_kv_write(a, stream), "hip paged_kv_write launch failed");
+}
+
+int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stride, float* out,
+                        int out_stride, int heads, float scale, int window,
+                        const int32_t* block_table, int max_pages, const int32_t* kv_lens,
+                        const int32_t* cu_tokens, int sequences, int tokens,
+                        hipStream_t stream) {
+  const char* ctx = "paged_attention";
+  mle::AttentionArgs a{};
+  MLE_TRY(check_cache(ctx, cache, &a.cache));
+  MLE_TRY(check_attention_sizes(ctx, cache, heads, sequences, tokens));
+  MLE_TRY(check_ptrs(ctx, q, "q", out, "out", block_table, "block_table"));
+  MLE_TRY(check_ptrs(ctx, kv_lens, "kv_lens", cu_tokens, "cu_tokens", cu_tokens, "cu_tokens"));
+  const int64_t row = (int64_t)heads * cache->head_dim;
+  MLE_TRY(check_rows(ctx, q, q_stride, row, "q"));
+  MLE_TRY(check_rows(ctx, out, out_stride, row, "out"));
+  MLE_TRY(check_align(ctx, block_table, 4, "block_table"));
+  MLE_TRY(check_align(ctx, kv_lens, 4, "kv_lens"));
+  MLE_TRY(check_align(ctx, cu_tokens, 4, "cu_tokens"));
+  MLE_TRY(check_positive(ctx, max_pages, "max_pages"));
+  if (!std::isfinite(scale))
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": scale must be finite");
+  if (window < 0)
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": window must not be negative");
+  if ((int64_t)max_pages * cache->page_size > INT32_MAX)
+    return fail(MLE_UNSUPPORTED,
+                std::string("hip ") + ctx + ": max_pages * page_size must fit 31 bits");
+  if (tokens == 0) return ok();
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.heads = heads;
+  a.scale = scale;
+  a.window = window;
+  a.table = block_table;
+  a.max_pages = max_pages;
+  a.kv_lens = kv_lens;
+  a.cu = cu_tokens;
+  a.sequences = sequences;
+  a.tokens = tokens;
+  return check_launch(mle::launch_paged_attention(a, stream),
+                      "hip paged_attention launch failed");
+}
+
+int mle_paged_attention_workspace_size(const mle_paged_cache* cache, int heads, int sequences,
+                                       int tokens, size_t* bytes, size_t* counters) {
+  const char* ctx = "paged_attention_workspace_size";
+  MLE_TRY(check_ptrs(ctx, bytes, "bytes", counters, "counters", counters, "counters"));
+  MLE_TRY(check_ptr(ctx, cache, "cache"));
+  MLE_TRY(check_attention_sizes(ctx, cache, heads, sequences, tokens));
+  *bytes = 0;
+  *counters = 0;
+  return ok();
 }
 
 }  // extern "C"

@@ -1,0 +1,83 @@
+// paged.hpp -- internal launchers of the paged KV cache behind the C ABI (not exported),
+// and its layout.  Every launcher assumes that the caller (capi.hip) has validated
+// pointers and shapes; each only enqueues work on `stream` and returns the launch status.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mle {
+
+constexpr int kKvTile = 16;  // tokens of a cache tile
+enum class KvType { kF16 = 0, kBF16 = 1, kInt8 = 2 };
+struct PagedCache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  KvType type;
+  int num_pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+};
+
+struct PlanArgs {
+  const int32_t* cached;
+  const int32_t* fresh;  // new tokens, or negative: finished
+  int sequences;
+  int32_t* table;
+  int max_pages;
+  int page_size;
+  int num_pages;
+  int32_t* stack;
+  const int32_t* count;
+  int32_t* count_out;
+  int tokens;
+  int32_t* kv_lens;
+  int32_t* cu;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* granted;
+};
+hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream);
+
+hipError_t launch_rope_table(float* table, int positions, int rope_dim, double theta,
+                             const float* freq_factors, hipStream_t stream);
+
+struct KvWriteArgs {
+  PagedCache cache;
+  const float* q;
+  float* q_out;
+  const float* k;
+  const float* v;
+  const float* rope;  // null: no rotation
+  const int32_t* positions;
+  const int32_t* slots;
+  int64_t q_stride, q_out_stride, k_stride, v_stride;
+  int heads;
+  int rope_positions;
+  int rope_dim;
+  int rope_halves;
+  int tokens;
+};
+hipError_t launch_paged_kv_write(const KvWriteArgs& a, hipStream_t stream);
+
+struct AttentionArgs {
+  PagedCache cache;
+  const float* q;
+  float* out;
+  int64_t q_stride, out_stride;
+  int heads;
+  float scale;
+  int window;
+  const int32_t* table;
+  int max_pages;
+  const int32_t* kv_lens;
+  const int32_t* cu;
+  int sequences;
+  int tokens;
+};
+hipError_t launch_paged_attention(const AttentionArgs& a, hipStream_t stream);
+
+}  // namespace mle
