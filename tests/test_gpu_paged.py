@@ -1,0 +1,683 @@
+"""GPU numerics of the paged KV cache (include/mle_paged.h) against plain implementations.
+
+The plan is compared entry by entry with a host loop over the requests, the write bit by bit
+with the rotation and the cell formats in 64 bits, and the attention with softmax in 64 bits
+over the values that the cache holds.
+
+Tolerance of the attention: the kernel's q differs from the fp32 one by less than 2^-22 of a
+row's largest element, products are exact, and sums of D terms in fp32 are off by less than
+(D + 8) 2^-24 of the sum of magnitudes; a logit is so off by less than
+ds = (D + 16) 2^-22 scale max_j sum_d |q_d k_jd|.  Weights e^s are off by ds + 2^-20 relative
+(exp2 of a rounded product, the 8-bit scales' logarithms), sums over the keys by their number
+n of partial sums (at most keys / 8 + 64) times 2^-24, and both numerator and denominator are
+off so: |error| <= 2 max|v| (ds + 2^-20 + (keys / 8 + 64) 2^-24).
+"""
+import math
+
+import numpy as np
+import pytest
+
+from helpers import empty_f32, note, to_dev
+from llmengine_amd import capi
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ("f16", "bf16", "int8")
+
+
+def i32(values, dev):
+    return to_dev(np.asarray(values, np.int32), dev)
+
+
+def prefix(values):
+    return np.concatenate([[0], np.cumsum(values)]).astype(np.int64)
+
+
+# ---- the plan ----
+
+def plan_host(cached, new, table, page, num_pages, stack, count, tokens):
+    """The header's rules, request by request."""
+    B, max_pages = table.shape
+    table, stack = table.copy(), stack.copy()
+    top = min(max(count, 0), num_pages)
+    for b in range(B):
+        if new[b] < 0:
+            for j in range(min(-(-max(cached[b], 0) // page), max_pages)):
+                if top < num_pages:
+                    stack[top] = table[b, j]
+                    top += 1
+    whole, asked, rows = top, 0, 0
+    kv, granted, cu = [], [], [0]
+    pos, slots = np.zeros(tokens, np.int32), np.full(tokens, -1, np.int32)
+    for b in range(B):
+        want, first = max(int(new[b]), 0), rows
+        rows += want
+        cu.append(min(rows, tokens))
+        if new[b] < 0:
+            kv.append(0)
+            granted.append(1)
+            continue
+        have, need = -(-int(cached[b]) // page), -(-(int(cached[b]) + want) // page)
+        ok = rows <= tokens and need <= max_pages
+        if ok:
+            asked += need - have
+            ok = need == have or asked <= whole
+        if ok:
+            for j in range(have, need):
+                table[b, j] = stack[whole - 1 - (asked - need + j)]
+                top = whole - asked
+            for i in range(want):
+                p = int(cached[b]) + i
+                pos[first + i] = p
+                pg = table[b, p // page]
+                slots[first + i] = pg * page + p % page if 0 <= pg < num_pages else -1
+        kv.append(int(cached[b]) + want if ok else 0)
+        granted.append(int(ok))
+    return table, stack, top, kv, cu, pos, slots, granted
+
+
+def plan_case(rng, B, page, lens, news, free, max_pages, extra=0):
+    have = [-(-c // page) for c in lens]
+    num_pages = sum(have) + free + extra
+    order = rng.permutation(num_pages).astype(np.int32)
+    table = np.full((B, max_pages), -1, np.int32)
+    at = free
+    for b, h in enumerate(have):
+        table[b, :h] = order[at:at + h]
+        at += h
+    stack = np.full(num_pages, -1, np.int32)
+    stack[:free] = order[:free]
+    return table, stack, num_pages
+
+
+def run_plan(dev, cached, new, table, page, num_pages, stack, count, tokens):
+    import torch
+    B, max_pages = table.shape
+    d = dict(cached=i32(cached, dev), new=i32(new, dev), table=i32(table, dev),
+             stack=i32(stack, dev), count=i32([count], dev))
+    out = {n: torch.full((max(k, 1),), -7, dtype=torch.int32, device=dev)
+           for n, k in (("count", 1), ("kv", B), ("cu", B + 1), ("pos", tokens),
+                        ("slots", tokens), ("granted", B))}
+    for _ in range(2):  # a repeated call gives the same
+        capi.paged_plan(d["cached"], d["new"], B, d["table"], max_pages, page, num_pages,
+                        d["stack"], d["count"], out["count"], tokens, out["kv"], out["cu"],
+                        out["pos"], out["slots"], out["granted"])
+    torch.cuda.synchronize()
+    o = {n: x.cpu().numpy() for n, x in out.items()}
+    return (d["table"].cpu().numpy(), d["stack"].cpu().numpy(), int(o["count"][0]), o["kv"],
+            o["cu"], o["pos"][:tokens], o["slots"][:tokens], o["granted"])
+
+
+@pytest.mark.parametrize("B,page,longest,most_new,short,finished,slack", [
+    (1, 16, 1, 1, False, 0, 0), (1, 16, 40, 0, False, 0, 3), (5, 16, 100, 40, True, 1, 0),
+    (64, 32, 900, 1, False, 3, 0), (65, 48, 300, 1, True, 9, 5), (300, 16, 200, 60, True, 30, 0),
+    (1025, 16, 90, 3, True, 70, 0), (2500, 32, 50, 2, False, 100, 11),
+    (40, 128, 2000, 600, True, 4, 0), (3, 1024, 5000, 9000, False, 0, 1)])
+def test_plan_matches_host_loop(dev, B, page, longest, most_new, short, finished, slack):
+    note(f"plan B={B} page={page} longest={longest} new={most_new} short={short}")
+    rng = np.random.default_rng(B * 7 + page)
+    cached = rng.integers(0, longest + 1, B)
+    new = rng.integers(0, most_new + 1, B)
+    new[rng.choice(B, finished, replace=False)] = -1
+    asked = sum(-(-(c + n) // page) - -(-c // page) for c, n in zip(cached, new) if n > 0)
+    free = asked * 2 // 3 if short else asked + 3
+    max_pages = max(-(-(c + max(n, 0)) // page) for c, n in zip(cached, new)) + 1
+    table, stack, num_pages = plan_case(rng, B, page, cached, new, free, max_pages)
+    tokens = int(np.maximum(new, 0).sum()) + slack
+    args = (cached, new, table, page, num_pages, stack, free, tokens)
+    for got, want in zip(run_plan(dev, *args), plan_host(*args)):
+        np.testing.assert_array_equal(got, want)
+
+
+def test_plan_refuses_what_does_not_fit(dev):
+    """Requests past max_pages, rows past `tokens`, negative lengths and bad page numbers."""
+    rng = np.random.default_rng(5)
+    cached, new = np.array([20, 10, 33, 0, 7]), np.array([5, 100, 3, 16, 2])
+    table, stack, num_pages = plan_case(rng, 5, 16, cached, new, 6, 4)
+    table[2, 2] = num_pages + 5          # row 2 lies in a page outside the cache
+    for tokens in (126, 124, 60, 5, 0):  # all rows, then fewer and fewer of them
+        note(f"plan refusals tokens={tokens}")
+        args = (cached, new, table, 16, num_pages, stack, 6, tokens)
+        for got, want in zip(run_plan(dev, *args), plan_host(*args)):
+            np.testing.assert_array_equal(got, want)
+
+
+# ---- rotations and the write ----
+
+@pytest.mark.parametrize("rope_dim,theta,factors", [(64, 10000.0, False), (128, 5e5, True),
+                                                    (8, 1e6, False)])
+def test_rope_table(dev, rope_dim, theta, factors):
+    import torch
+    half, n = rope_dim // 2, 9001
+    f = np.linspace(1, 8, half).astype(np.float32) if factors else None
+    table = empty_f32((n, half, 2), dev)
+    capi.rope_table(table, n, rope_dim, theta, to_dev(f, dev) if factors else None)
+    torch.cuda.synchronize()
+    a = np.arange(n)[:, None] * theta ** (-np.arange(half) / half)
+    if factors:
+        a = a / f.astype(np.float64)
+    want = np.stack([np.cos(a), np.sin(a)], -1)
+    # Angles up to 9001 are off by a few ulps of 64 bits (2^-38); then one rounding.
+    np.testing.assert_allclose(table.cpu().numpy(), want, rtol=2.0 ** -24, atol=2.0 ** -36)
+
+
+def rotate_host(x, rope, pos, rope_dim, mode):
+    """x [T, heads, D] fp32; exact products and sums (53 bits hold them), one rounding."""
+    if mode == "none":
+        return x
+    out = x.copy()
+    t = rope[pos].astype(np.longdouble)[:, None]
+    c, s = t[..., 0], t[..., 1]
+    h = rope_dim // 2
+    ia = np.arange(h) if mode == "halves" else 2 * np.arange(h)
+    ib = ia + h if mode == "halves" else ia + 1
+    a, b = x[..., ia].astype(np.longdouble), x[..., ib].astype(np.longdouble)
+    out[..., ia] = (a * c - b * s).astype(np.float64).astype(np.float32)
+    out[..., ib] = (a * s + b * c).astype(np.float64).astype(np.float32)
+    return out
+
+
+def cells_of(cache, pages, page, G, D):
+    """(K, V) of a cache as [slot, G, D] tensors in the cache's type, by the header's layout,
+    and the scales as [slot, G] (or None)."""
+    k = cache.k.view(pages, G, page // 16, D // 8, 16, 8).permute(0, 2, 4, 1, 3, 5)
+    v = cache.v.view(pages, G, page // 16, 2, D, 2, 4).permute(0, 2, 5, 3, 6, 1, 4)
+    scales = [None if s is None else s.view(pages, G, page).permute(0, 2, 1).reshape(-1, G)
+              for s in (cache.k_scale, cache.v_scale)]
+    return k.reshape(-1, G, D), v.reshape(-1, G, D), *scales
+
+
+def stored_host(x, kv_type):
+    """[T, G, D] fp32 -> (cells, scales) as the header says."""
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x))
+    if kv_type != "int8":
+        return t.to({"f16": torch.float16, "bf16": torch.bfloat16}[kv_type]), None
+    amax = t.abs().amax(-1)
+    s = amax * torch.tensor(1.0 / 127.0, dtype=torch.float32)
+    q = torch.where(s[..., None] > 0, (t / s[..., None]).round(), 0.0).clamp(-127, 127)
+    return q.to(torch.int8), s
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("H,G,D,rope_dim,mode,page,T,fused", [
+    (14, 2, 64, 64, "halves", 16, 1, False), (4, 4, 128, 128, "pairs", 32, 37, True),
+    (6, 3, 96, 64, "halves", 16, 130, True), (8, 1, 256, 256, "pairs", 64, 67, False),
+    (5, 5, 64, 64, "none", 48, 29, False), (2, 1, 128, 8, "halves", 16, 300, True),
+    (3, 1, 96, 96, "pairs", 16, 18, False)])
+def test_write_bits(dev, kv_type, H, G, D, rope_dim, mode, page, T, fused):
+    import torch
+    note(f"write {kv_type} H={H} G={G} D={D} rope={rope_dim}/{mode} page={page} T={T}")
+    rng = np.random.default_rng(T + D)
+    n = H + 2 * G
+    qkv = rng.standard_normal((T, n, D)).astype(np.float32)
+    qkv[T // 2, H:] *= 1e-3
+    qkv[T - 1, n - 1] = 0            # a V row of zeros
+    limit = 500
+    rope = rng.uniform(-1, 1, (limit, rope_dim // 2, 2)).astype(np.float32)
+    # Runs of consecutive slots from any offset, some rows nowhere, one past the rope's end.
+    pages = T // page * 2 + 8 * (T // 40 + 1)
+    free = rng.permutation(pages)
+    pos, slots, at, p = [], [], 0, int(rng.integers(0, 9))
+    for t in range(T):
+        if t % 41 == 40:
+            p, at = int(rng.integers(0, 60)), at + p // page + 1
+        pos.append(p)
+        slots.append(free[(at + p // page) % pages] * page + p % page)
+        p += 1
+    pos, slots = np.array(pos, np.int64) % limit, np.array(slots, np.int64)
+    if T > 10:
+        slots[5], slots[9] = -1, pages * page
+        pos[7] = limit if mode != "none" else pos[7]
+    dq = to_dev(qkv.reshape(T, -1), dev)
+    parts = [dq[:, :H * D], dq[:, H * D:(H + G) * D], dq[:, (H + G) * D:]]
+    if not fused:
+        parts = [x.contiguous() for x in parts]
+    cache = capi.PagedCache.allocate(kv_type, pages, page, G, D, dev)
+    q_out = empty_f32((T, H * D), dev)
+    capi.paged_kv_write(cache, parts[0], q_out, H, parts[1], parts[2],
+                        None if mode == "none" else to_dev(rope, dev), limit, rope_dim, mode,
+                        i32(pos, dev), i32(slots, dev), T)
+    torch.cuda.synchronize()
+    placed = pos < limit
+    safe = np.where(placed, pos, 0)
+    want_q = rotate_host(qkv[:, :H], rope, safe, rope_dim, mode)
+    want_q[~placed] = 0
+    np.testing.assert_array_equal(q_out.cpu().numpy().reshape(T, H, D), want_q)
+    k = rotate_host(qkv[:, H:H + G], rope, safe, rope_dim, mode)
+    got = [None if x is None else x.cpu() for x in cells_of(cache, pages, page, G, D)]
+    want = [torch.zeros_like(x) if x is not None else None for x in got]
+    kept = placed & (slots >= 0) & (slots < pages * page)
+    last = {int(s): t for t, s in enumerate(slots) if kept[t]}
+    rows, ts = list(last), list(last.values())
+    if len(set(slots[kept])) != kept.sum():
+        pytest.fail("the test's slots repeat")
+    for i, x in ((0, k), (1, qkv[:, H + G:])):
+        c, s = stored_host(x, kv_type)
+        want[i][rows] = c[ts]
+        if s is not None:
+            want[2 + i][rows] = s[ts]
+    for g, w in zip(got, want):
+        if w is not None:
+            assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_write_in_place_and_non_finite(dev, kv_type):
+    """q rotated in place; rows with NaN or infinity read back as such, never as numbers."""
+    import torch
+    H, G, D, T, page = 3, 2, 64, 9, 16
+    rng = np.random.default_rng(3)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    k, v = (rng.standard_normal((T, G, D)).astype(np.float32) for _ in range(2))
+    k[2, 1, 5], v[3, 0, 63], v[8, 1, 0], k[4, 0, 0] = np.nan, np.inf, np.nan, -np.inf
+    rope = rng.uniform(-1, 1, (T, D // 2, 2)).astype(np.float32)
+    cache = capi.PagedCache.allocate(kv_type, 2, page, G, D, dev)
+    dq = to_dev(q.reshape(T, -1), dev)
+    capi.paged_kv_write(cache, dq, dq, H, to_dev(k.reshape(T, -1), dev),
+                        to_dev(v.reshape(T, -1), dev), to_dev(rope, dev), T, D, "halves",
+                        i32(np.arange(T), dev), i32(np.arange(T) + 3, dev), T)
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(dq.cpu().numpy().reshape(T, H, D),
+                                  rotate_host(q, rope, np.arange(T), D, "halves"))
+    ck, cv, ks, vs = cells_of(cache, 2, page, G, D)
+    values = [x.float() if s is None else x.float() * s[..., None] for x, s in ((ck, ks),
+                                                                               (cv, vs))]
+    want_bad = [np.zeros((T, G), bool) for _ in range(2)]
+    for i, x in ((0, k), (1, v)):
+        want_bad[i] = ~np.isfinite(x).all(-1)
+    for x, bad in zip(values, want_bad):
+        finite = torch.isfinite(x).all(-1).cpu().numpy()[3:3 + T]
+        np.testing.assert_array_equal(~finite, bad)
+
+
+# ---- the attention ----
+
+def make_cache(rng, dev, kv_type, pages, page, G, D, poison=True):
+    """A cache that holds NaN wherever fill_pages does not put values."""
+    import torch
+    cache = capi.PagedCache.allocate(kv_type, pages, page, G, D, dev)
+    if poison:
+        if kv_type == "int8":
+            cache.k.fill_(-128), cache.v.fill_(127)
+            cache.k_scale.fill_(float("nan")), cache.v_scale.fill_(float("nan"))
+        else:
+            cache.k.fill_(float("nan")), cache.v.fill_(float("nan"))
+    return cache
+
+
+def put(cache, kv_type, page, slots, k, v):
+    """k, v [n, G, D] fp32 into `slots`; returns what the cache holds of them, 64 bits."""
+    import torch
+    G, D = k.shape[1:]
+    slots = torch.as_tensor(slots, device=cache.k.device)
+    p, t = slots // page, slots % page
+    kc = cache.k.view(-1, G, page // 16, D // 8, 16, 8)
+    vc = cache.v.view(-1, G, page // 16, 2, D, 2, 4)
+    r, tile = t % 16, t // 16
+    out = []
+    for x, is_k in ((k, True), (v, False)):
+        c, s = stored_host(x, kv_type)
+        c = c.to(cache.k.device)
+        if is_k:
+            kc[p, :, tile, :, r] = c.view(-1, G, D // 8, 8)
+        else:
+            vc[p, :, tile, r // 4 % 2, :, r // 8, r % 4] = c
+        if s is not None:
+            (cache.k_scale if is_k else cache.v_scale).view(-1, G, page)[p, :, t] = \
+                s.to(cache.k.device)
+            out.append(c.cpu().double().numpy() * s.double().numpy()[..., None])
+        else:
+            out.append(c.cpu().double().numpy())
+    return out
+
+
+def attention_host(q, k, v, pos, window, scale, ok=None):
+    """q [n, H, D], k/v [keys, G, D] in 64 bits; returns (out, tolerance)."""
+    n, H, D = q.shape
+    R = H // k.shape[1]
+    j = np.arange(k.shape[0])
+    seen = j[None] <= pos[:, None]
+    if window:
+        seen &= j[None] > pos[:, None] - window
+    if ok is not None:
+        seen &= ok[None]
+    out, tol = np.zeros((n, H, D)), 0.0
+    for h in range(H):
+        kk, vv = k[:, h // R], v[:, h // R]
+        s = scale * (q[:, h].astype(np.float64) @ kk.T)
+        s = np.where(seen, s, -np.inf)
+        top = s.max(-1, keepdims=True) if s.shape[1] else np.full((n, 1), -np.inf)
+        e = np.where(seen, np.exp(s - np.where(np.isfinite(top), top, 0)), 0)
+        z = e.sum(-1, keepdims=True)
+        out[:, h] = (e @ vv) / np.where(z > 0, z, 1)
+        if not seen.any():
+            continue
+        use = seen.any(0)
+        ds = (D + 16) * 2.0 ** -22 * abs(scale) * (np.abs(q[:, h]) @ np.abs(kk[use]).T).max()
+        tol = max(tol, 2 * np.abs(vv[use]).max()
+                  * (ds + 2.0 ** -20 + (use.sum() / 8 + 64) * 2.0 ** -24))
+    return out, tol
+
+
+class Batch:
+    """A batch of sequences (new, total) in a poisoned cache, and its expected outputs."""
+
+    def __init__(self, dev, kv_type, H, G, D, page, lens, window=0, seed=1, q_scale=2.0,
+                 bad_pages=(), pages_extra=3, first_page=0, scale=None, v_spread=False):
+        import torch
+        rng = np.random.default_rng(seed)
+        self.dev, self.H, self.G, self.D, self.page, self.lens = dev, H, G, D, page, lens
+        self.window, self.scale = window, D ** -0.5 if scale is None else scale
+        need = [-(-t // page) for _, t in lens]
+        pages = first_page + sum(need) + pages_extra
+        self.cache = make_cache(rng, dev, kv_type, pages, page, G, D, poison=first_page == 0)
+        order = first_page + rng.permutation(pages - first_page)
+        self.max_pages = max(need + [1]) + 2
+        table = np.full((len(lens), self.max_pages), -1, np.int64)
+        T = sum(n for n, _ in lens)
+        self.T = T
+        q = (q_scale * rng.standard_normal((T, H, D))).astype(np.float32)
+        self.want, self.tol, at, row = np.zeros((T, H, D)), 0.0, 0, 0
+        for b, ((n, total), np_) in enumerate(zip(lens, need)):
+            table[b, :np_] = order[at:at + np_]
+            at += np_
+            k, v = (rng.standard_normal((total, G, D)).astype(np.float32) for _ in range(2))
+            if v_spread:  # rows of V of very different sizes
+                v *= 10.0 ** rng.uniform(-4, 3, (total, 1, 1)).astype(np.float32)
+            ok = np.ones(total, bool)
+            if total:
+                slots = table[b, np.arange(total) // page] * page + np.arange(total) % page
+                k, v = put(self.cache, kv_type, page, slots, k, v)
+            for bb, j in bad_pages:
+                if bb == b and j < np_:
+                    table[b, j] = -5 if j % 2 else pages + 3
+                    ok[j * page:(j + 1) * page] = False
+            pos = total - n + np.arange(n)
+            if n:
+                o, tol = attention_host(q[row:row + n], k, v, pos, window, self.scale, ok)
+                self.want[row:row + n] = o
+                self.tol = max(self.tol, tol)
+            row += n
+        self.q = to_dev(q.reshape(T, H * D), dev)
+        self.table = i32(table, dev)
+        self.kv_lens = i32([t for _, t in lens], dev)
+        self.cu = i32(prefix([n for n, _ in lens]), dev)
+
+    def run(self, out=None, q=None, stream=None):
+        out = empty_f32((self.T, self.H * self.D), self.dev) if out is None else out
+        capi.paged_attention(self.cache, self.q if q is None else q, out, self.H, self.scale,
+                             self.window, self.table, self.max_pages, self.kv_lens, self.cu,
+                             len(self.lens), self.T, stream=stream)
+        return out
+
+    def check(self, out):
+        import torch
+        torch.cuda.synchronize()
+        got = out.cpu().numpy().reshape(self.want.shape).astype(np.float64)
+        assert np.isfinite(got).all()
+        err = np.abs(got - self.want).max()
+        assert err <= self.tol, (err, self.tol)
+
+
+LAYOUTS = [(14, 2, 64), (4, 4, 128), (8, 2, 128), (8, 4, 96), (8, 1, 256), (6, 6, 64),
+           (7, 1, 128), (64, 1, 64), (3, 3, 96)]
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("H,G,D", LAYOUTS)
+@pytest.mark.parametrize("lens,page,window", [
+    ([(1, 1)], 16, 0), ([(1, 129), (1, 1), (1, 16), (1, 700)], 16, 0),
+    ([(1, 333), (70, 70), (0, 50), (1, 64), (17, 190)], 32, 0),
+    ([(130, 300), (1, 17), (1, 1000)], 48, 100)])
+def test_attention(dev, kv_type, H, G, D, lens, page, window):
+    note(f"attention {kv_type} H={H} G={G} D={D} lens={lens} page={page} window={window}")
+    b = Batch(dev, kv_type, H, G, D, page, lens, window, seed=D + H)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("lens,page,window", [
+    ([(1, 9000)], 64, 0), ([(1, 5000), (3, 2100), (2, 33)], 128, 0), ([(257, 1500)], 16, 1),
+    ([(40, 40)] * 5, 16, 7), ([(1, 4095), (300, 2049)], 1024, 1024), ([(64, 64)], 16, 0)])
+def test_attention_lengths(dev, kv_type, lens, page, window):
+    note(f"attention lengths {kv_type} lens={lens} page={page} window={window}")
+    b = Batch(dev, kv_type, 8, 2, 64, page, lens, window, seed=sum(t for _, t in lens))
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_many_sequences(dev, kv_type):
+    """More sequences than a workgroup has threads, most of them short, some without rows."""
+    rng = np.random.default_rng(9)
+    lens = [(int(rng.integers(0, 3)), int(rng.integers(2, 60))) for _ in range(700)]
+    lens[30], lens[650] = (50, 90), (1, 1500)
+    note(f"attention many sequences {kv_type}")
+    b = Batch(dev, kv_type, 4, 2, 64, 16, lens)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_bad_pages_hide_their_keys(dev, kv_type):
+    lens = [(1, 300), (40, 200), (1, 40), (5, 90)]
+    bad = [(0, 0), (0, 7), (1, 3), (1, 12), (2, 0), (2, 1), (2, 2), (3, 5)]
+    for window in (0, 30):
+        note(f"attention bad pages {kv_type} window={window}")
+        b = Batch(dev, kv_type, 8, 2, 128, 16, lens, window, bad_pages=bad)
+        b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_rows_without_keys(dev, kv_type):
+    """Rows before the first token (kv_lens below the new rows: refused requests) are zero,
+    rows outside every sequence are not written."""
+    import torch
+    b = Batch(dev, kv_type, 4, 2, 64, 16, [(1, 20), (30, 40), (2, 50), (20, 33)])
+    b.kv_lens = i32([20, 0, 50, 5], dev)
+    note(f"attention rows without keys {kv_type}")
+    out = empty_f32((b.T + 4, b.H * b.D), dev)
+    capi.paged_attention(b.cache, torch.cat([b.q, b.q[:4]]), out, 4, b.scale, 0, b.table,
+                         b.max_pages, b.kv_lens, b.cu, 4, b.T + 4)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(-1, 4, 64)
+    assert np.isnan(got[b.T:]).all()
+    assert (got[1:31] == 0).all() and (got[33:48] == 0).all()
+    for rows in (slice(0, 1), slice(31, 33)):
+        assert np.abs(got[rows] - b.want[rows]).max() <= b.tol
+    assert np.isfinite(got[48:53]).all() and (got[48:53] != 0).any()
+
+
+@pytest.mark.parametrize("kv_type", ("f16", "bf16"))
+@pytest.mark.parametrize("H,G,n", [(4, 2, 5), (4, 2, 60), (4, 1, 140)])
+def test_attention_non_finite_values(dev, kv_type, H, G, n):
+    """A later token's NaN or infinite K or V reaches the rows that see it and no other."""
+    import torch
+    D, page, total = 64, 16, n + 45
+    for what, value in (("k", float("nan")), ("v", float("nan")), ("v", float("inf")),
+                        ("v", float("-inf"))):
+        note(f"attention non-finite {kv_type} {what}={value} n={n}")
+        b = Batch(dev, kv_type, H, G, D, page, [(n, total)], seed=n)
+        at = total - n + n // 2           # seen by the second half of the rows
+        slot = int(b.table[0, at // page]) * page + at % page
+        p, r, tile = slot // page, slot % 16, slot % page // 16
+        if what == "k":
+            b.cache.k.view(-1, G, page // 16, D // 8, 16, 8)[p, 0, tile, 3, r, 5] = value
+        else:
+            b.cache.v.view(-1, G, page // 16, 2, D, 2, 4)[
+                p, 0, tile, r // 4 % 2, 29, r // 8, r % 4] = value
+        out = b.run()
+        torch.cuda.synchronize()
+        got = out.cpu().numpy().reshape(n, H, D)
+        first, mine = n // 2, slice(0, H // G)
+        assert np.abs(got[:first] - b.want[:first]).max() <= b.tol
+        if G > 1:
+            assert np.abs(got[:, H // G:] - b.want[:, H // G:]).max() <= b.tol
+        if what == "k":
+            assert np.isnan(got[first:, mine]).all()
+        else:
+            hit = got[first:, mine, 29]
+            assert (np.isnan(hit) if math.isnan(value) else hit == value).all()
+            other = np.arange(D) != 29
+            assert np.abs(got[first:, mine][..., other]
+                          - b.want[first:, mine][..., other]).max() <= b.tol
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("lens", [[(1, 300), (3, 70)], [(90, 300)]])
+def test_attention_scales_and_magnitudes(dev, kv_type, lens):
+    """Scales of zero, below zero and large; q of very small and very large values; V rows of
+    sizes from 1e-4 to 1e3."""
+    for scale, q_scale, spread in ((0.0, 1.0, False), (-0.2, 1.0, False), (4.0, 1.0, False),
+                                   (0.125, 1e-30, False), (1e-6, 3e5, True),
+                                   (0.125, 2.0, True)):
+        note(f"attention magnitudes {kv_type} scale={scale} q={q_scale} lens={lens}")
+        b = Batch(dev, kv_type, 4, 2, 64, 16, lens, scale=scale, q_scale=q_scale,
+                  v_spread=spread)
+        b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("lens", [[(1, 40), (2, 300)], [(50, 200)]])
+def test_attention_non_finite_q(dev, kv_type, lens):
+    """A row with NaN in q is NaN in that head and leaves the others as they are."""
+    import torch
+    b = Batch(dev, kv_type, 4, 2, 64, 16, lens)
+    note(f"attention NaN in q {kv_type}")
+    row, h = b.T - 2, 1
+    b.q.view(b.T, 4, 64)[row, h, 7] = float("nan")
+    out = b.run()
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(b.T, 4, 64)
+    assert np.isnan(got[row, h]).all()
+    got[row, h] = b.want[row, h]
+    assert np.abs(got - b.want).max() <= b.tol
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_strides_streams_and_repeats(dev, kv_type):
+    """Strided rows, out over q, another stream, and the same bits on every run."""
+    import torch
+    b = Batch(dev, kv_type, 8, 2, 64, 32, [(1, 3000), (40, 700), (2, 90)])
+    note(f"attention strides {kv_type}")
+    first = b.run()
+    b.check(first)
+    wide_q = torch.zeros(b.T, 8 * 64 + 20, device=dev)
+    wide_q[:, :512] = b.q
+    wide_out = empty_f32((b.T, 8 * 64 + 4), dev)
+    b.run(out=wide_out[:, :512], q=wide_q[:, :512])
+    torch.cuda.synchronize()
+    assert torch.equal(wide_out[:, :512], first) and torch.isnan(wide_out[:, 512:]).all()
+    same = b.q.clone()
+    b.run(out=same, q=same)
+    torch.cuda.synchronize()
+    assert torch.equal(same, first)
+    stream = torch.cuda.Stream()
+    for _ in range(5):
+        other = empty_f32(first.shape, dev)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            b.run(out=other)
+        stream.synchronize()
+        assert torch.equal(other, first)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_graph_replays(dev, kv_type):
+    """A captured call follows the lengths on the device; eager calls run between replays."""
+    import torch
+    b = Batch(dev, kv_type, 8, 2, 64, 32, [(1, 3000), (40, 700), (2, 90)])
+    c = Batch(dev, kv_type, 8, 2, 64, 32, [(1, 2000), (40, 300), (2, 70)], seed=2)
+    eager = [x.run() for x in (b, c)]
+    stream = torch.cuda.Stream()
+    capi.workspace_reserve(*capi.paged_attention_workspace_size(b.cache, 8, 3, b.T),
+                           stream=stream)
+    torch.cuda.synchronize()
+    note(f"attention captured {kv_type}")
+    names = ("q", "table", "kv_lens")
+    held = {n: getattr(b, n).clone() for n in names}
+    out = empty_f32(eager[0].shape, dev)
+    cache_c = [c.cache.k, c.cache.v, c.cache.k_scale, c.cache.v_scale]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        capi.paged_attention(b.cache, held["q"], out, 8, b.scale, 0, held["table"], b.max_pages,
+                             held["kv_lens"], b.cu, 3, b.T, stream=stream)
+    for rep in range(4):
+        if rep == 2:  # the same graph on other lengths and pages
+            table = torch.full_like(held["table"], -1)
+            table[:, :c.max_pages] = c.table
+            held["table"].copy_(table)
+            held["q"].copy_(c.q), held["kv_lens"].copy_(c.kv_lens)
+            for x, y in zip((b.cache.k, b.cache.v, b.cache.k_scale, b.cache.v_scale), cache_c):
+                if y is not None:
+                    x[:y.numel()].copy_(y)
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        extra = c.run()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[rep // 2]), rep
+        assert torch.equal(extra, eager[1])
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_far_pages(dev, kv_type):
+    """Pages whose elements lie past 2^31 of the cache's buffers."""
+    G, D, page = 2, 64, 256
+    first = 2 ** 31 // (G * page * D) + 5
+    note(f"attention far pages {kv_type}")
+    b = Batch(dev, kv_type, 4, G, D, page, [(1, 900), (30, 600)], first_page=first)
+    b.check(b.run())
+
+
+# ---- the step as a whole ----
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_steps_together(dev, kv_type):
+    """Plan, write and attention over several steps: prompts, a chunk, decoding, a finished
+    request whose pages the next one takes."""
+    import torch
+    H, G, D, page, pages, B = 4, 2, 64, 16, 24, 3
+    note(f"steps {kv_type}")
+    rng = np.random.default_rng(8)
+    cache = make_cache(rng, dev, kv_type, pages, page, G, D)
+    table = i32(np.full((B, 10), -1), dev)
+    stack, count = i32(rng.permutation(pages), dev), i32([pages], dev)
+    rope = empty_f32((200, D // 2, 2), dev)
+    capi.rope_table(rope, 200, D)
+    torch.cuda.synchronize()
+    host_rope = rope.cpu().numpy()
+    history = [[np.zeros((0, G, D))] * 2 for _ in range(B)]
+    lens = np.zeros(B, int)
+    for news in ([40, 17, 0], [1, 30, 60], [1, 1, 1], [-1, 1, 1], [90, 1, 1], [1, 1, 1]):
+        T = sum(max(n, 0) for n in news)
+        kv, cu, pos, slots, granted = (torch.zeros(n, dtype=torch.int32, device=dev)
+                                       for n in (B, B + 1, T, T, B))
+        capi.paged_plan(i32(lens, dev), i32(news, dev), B, table, 10, page, pages, stack,
+                        count, count, T, kv, cu, pos, slots, granted)
+        qkv = rng.standard_normal((T, H + 2 * G, D)).astype(np.float32)
+        d = to_dev(qkv.reshape(T, -1), dev)
+        q, k, v = d.split([H * D, G * D, G * D], dim=1)
+        q_out, out = empty_f32((T, H * D), dev), empty_f32((T, H * D), dev)
+        capi.paged_kv_write(cache, q, q_out, H, k, v, rope, 200, D, "halves", pos, slots, T)
+        capi.paged_attention(cache, q_out, out, H, D ** -0.5, 0, table, 10, kv, cu, B, T)
+        torch.cuda.synchronize()
+        assert granted.cpu().tolist() == [1] * B
+        got, row = out.cpu().numpy().reshape(T, H, D), 0
+        for b, n in enumerate(news):
+            if n < 0:
+                history[b], lens[b] = [np.zeros((0, G, D))] * 2, 0
+                continue
+            p = lens[b] + np.arange(n)
+            mine = qkv[row:row + n]
+            new = [rotate_host(mine[:, H:H + G], host_rope, p, D, "halves"), mine[:, H + G:]]
+            for i, x in enumerate(new):
+                c, s = stored_host(x, kv_type)
+                c = c.double().numpy() * (1.0 if s is None else s.double().numpy()[..., None])
+                history[b][i] = np.concatenate([history[b][i], c])
+            lens[b] += n
+            if n:
+                want, tol = attention_host(rotate_host(mine[:, :H], host_rope, p, D, "halves"),
+                                           *history[b], p, 0, D ** -0.5)
+                assert np.abs(got[row:row + n] - want).max() <= tol
+            row += n
+    assert count.item() == pages - sum(-(-int(n) // page) for n in lens)
