@@ -152,6 +152,9 @@ int check_attention_sizes(const char* ctx, const mle_paged_cache* c, int heads, 
   if (heads / c->kv_heads > 64)
     return fail(MLE_UNSUPPORTED,
                 std::string("hip ") + ctx + ": heads / kv_heads must be at most 64");
+  if ((int64_t)tokens * (heads / c->kv_heads) > INT32_MAX - 256)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": tokens * heads / kv_heads must fit 31 bits");
   return MLE_OK;
 }
 
@@ -1340,10 +1343,12 @@ int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stri
     return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": scale must be finite");
   if (window < 0)
     return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": window must not be negative");
-  if ((int64_t)max_pages * cache->page_size > INT32_MAX)
+  // The kernel's key numbers run a few steps past the last key.
+  if ((int64_t)max_pages * cache->page_size > INT32_MAX - 65536)
     return fail(MLE_UNSUPPORTED,
                 std::string("hip ") + ctx + ": max_pages * page_size must fit 31 bits");
   if (tokens == 0) return ok();
+  const int group = heads / cache->kv_heads;
   a.q = q;
   a.out = out;
   a.q_stride = q_stride;
@@ -1357,7 +1362,11 @@ int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stri
   a.cu = cu_tokens;
   a.sequences = sequences;
   a.tokens = tokens;
-  return check_launch(mle::launch_paged_attention(a, stream),
+  mle::SplitKWorkspace ws;
+  std::unique_lock<std::mutex> hold;
+  MLE_TRY(get_workspace(mle::paged_attention_workspace(cache->head_dim, (int64_t)tokens * group),
+                        stream, &ws, &hold));
+  return check_launch(mle::launch_paged_attention(a, ws, stream),
                       "hip paged_attention launch failed");
 }
 
@@ -1367,8 +1376,10 @@ int mle_paged_attention_workspace_size(const mle_paged_cache* cache, int heads, 
   MLE_TRY(check_ptrs(ctx, bytes, "bytes", counters, "counters", counters, "counters"));
   MLE_TRY(check_ptr(ctx, cache, "cache"));
   MLE_TRY(check_attention_sizes(ctx, cache, heads, sequences, tokens));
-  *bytes = 0;
-  *counters = 0;
+  const mle::SplitKNeed need = mle::paged_attention_workspace(
+      cache->head_dim, (int64_t)tokens * (heads / cache->kv_heads));
+  *bytes = tokens > 0 ? need_bytes(need) : 0;
+  *counters = tokens > 0 ? need.counters : 0;
   return ok();
 }
 

@@ -1,114 +1,1359 @@
 // paged_attention.hip -- attention of new tokens over the paged KV cache.
 //
-// One wave per row and query head: 64 keys at a time, a lane per key for the logits, a
-// lane per 4 dimensions for the sum over the keys, with the running maximum and sum of
-// the softmax between them.
+// out = sum_j softmax_j(scale q . k_j) v_j in one pass over the keys, with the running
+// maximum m and sum l of the softmax beside the output.  Both products are transposed,
+// S^T = K q^T and O^T = V^T P^T, so that a lane keeps one row of q throughout: row maxima
+// and sums are sums over its registers, and with the cache's layout (include/mle_paged.h)
+// the registers of S^T are those of the P operand, without a transpose of K, V or P.
+//
+// fp32 accuracy from 16-bit matrix instructions: q and P go in as sums of 16-bit parts, two
+// f16 (22 bits) against f16 and 8-bit caches, three bf16 (24 bits) against bf16, whose
+// range f16 does not have.  A row of q is first scaled by a power of two to [2^9, 2^10), P
+// carries a factor 2^6, so the f16 parts keep 22 bits down to 2^-13 of the largest.
+//
+// 8-bit caches: s_j = (q . k_j) ks_j; the V row's scale goes into the exponent, p_j vs_j =
+// 2^(s_j + log2 vs_j - m), with m the maximum of those sums, so that the parts have their
+// bits where the row's contributions are; l gets p_j vs_j * (1 / vs_j).
+//
+// A value of V that is not finite must reach the rows that see it and no others, and 0 times
+// it, or the parts of P times it, are NaN.  Where rows of a tile do not all see a key, such
+// values are taken out of the product and added to the rows that see them; where the
+// product of keys that all rows see comes out non-finite, the keys are gone through again
+// that way.
+//
+// The maximum moves only when a logit passes it by 2^8 (P and l stay far from their limits),
+// so that the rescaling of O is rare.
+//
+// Work is laid out on the device, from the lengths there: units of 64 keys of one (sequence,
+// KV head, row tile), cut into as many equal runs as there are workgroups, whatever the mix
+// of short and long sequences, decoding and prompts.  A tile cut by a run's end is joined,
+// in order, by the workgroup that finishes last.
+#include "../launch.hpp"
 #include "../paged.hpp"
 #include "../q8_0_device.hpp"
 
 namespace mle {
 namespace {
 
+constexpr int kThreads = 256;
+constexpr int kUnit = 64;         // keys of a unit of work, and of a stage in LDS
+constexpr int kFewRows = 16;      // up to this many rows the waves split the keys
+constexpr int kTileRows = 128;    // above: four waves of 32 rows share the keys in LDS
+constexpr float kSlack = 8.0f;    // log2 of what a logit may pass the kept maximum by
+constexpr float kTinyScale = 0x1p-100f;
+constexpr int kDeviceScope = 16;  // cache policy of loads and stores
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// ---- element types ----
+
+// 8-bit caches are computed in f16, which holds their whole numbers.
 template <KvType T>
-__device__ __forceinline__ float kv_at(const void* base, int64_t at) {
-  if constexpr (T == KvType::kF16) return (float)static_cast<const _Float16*>(base)[at];
-  else if constexpr (T == KvType::kBF16) return (float)static_cast<const __bf16*>(base)[at];
-  else return (float)static_cast<const int8_t*>(base)[at];
+constexpr int kParts = T == KvType::kBF16 ? 3 : 2;
+template <KvType T>
+constexpr bool kBytes = T == KvType::kInt8;
+// log2 of P's factor: f16 parts reach further down with it, bf16 parts need none.
+template <KvType T>
+constexpr float kHeadroom = T == KvType::kBF16 ? 0.0f : 6.0f;
+
+// Two fp32 values as pairs of 16-bit parts that add up to them.
+template <KvType T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t* part, int stride) {
+  if constexpr (T == KvType::kBF16) {
+    // Truncation leaves 8 bits a part: three hold all 24.
+    const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
+    part[0] = top_halves(ua, ub);
+    const float ra = a - __builtin_bit_cast(float, ua & 0xffff0000u);
+    const float rb = b - __builtin_bit_cast(float, ub & 0xffff0000u);
+    const uint32_t va = __builtin_bit_cast(uint32_t, ra), vb = __builtin_bit_cast(uint32_t, rb);
+    part[stride] = top_halves(va, vb);
+    const float sa = ra - __builtin_bit_cast(float, va & 0xffff0000u);
+    const float sb = rb - __builtin_bit_cast(float, vb & 0xffff0000u);
+    part[2 * stride] =
+        top_halves(__builtin_bit_cast(uint32_t, sa), __builtin_bit_cast(uint32_t, sb));
+  } else {
+    const f16x2 hi = __builtin_convertvector((f32x2{a, b}), f16x2);
+    const f32x2 rest = {a - (float)hi.x, b - (float)hi.y};
+    part[0] = __builtin_bit_cast(uint32_t, hi);
+    part[stride] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
+  }
 }
 
 template <KvType T>
-__global__ __launch_bounds__(64) void attention_rows_kernel(AttentionArgs a) {
-  __shared__ float s_q[256], s_p[64];
-  __shared__ int64_t s_cell[64];
-  const int lane = threadIdx.x, row = blockIdx.x, h = blockIdx.y;
-  const int D = a.cache.head_dim, P = a.cache.page_size, G = a.cache.kv_heads;
-  const int g = h / (a.heads / G);
-  int lo = 0, hi = a.sequences;  // the first b with cu[b + 1] > row
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid + 1] > row) hi = mid; else lo = mid + 1;
-  }
-  if (lo == a.sequences || a.cu[lo] > row) return;
-  const int64_t most = (int64_t)a.max_pages * P;
-  const int fresh = a.cu[lo + 1] - a.cu[lo];
-  const int pos = a.kv_lens[lo] - fresh + (row - a.cu[lo]);
-  const int end = (int)(pos + 1LL < most ? pos + 1LL : most);
-  const int begin = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-  for (int d = lane; d < D; d += 64)
-    s_q[d] = a.q[row * a.q_stride + (int64_t)h * D + d] * a.scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, acc[4] = {};
-  for (int j0 = begin; j0 < end; j0 += 64) {
-    const int j = j0 + lane;
-    float s = -INFINITY, v_scale = 1.0f;
-    int64_t cell = -1;
-    if (j < end) {
-      const int page = a.table[(int64_t)lo * a.max_pages + j / P];
-      if ((uint32_t)page < (uint32_t)a.cache.num_pages) {
-        cell = ((int64_t)page * G + g) * P + j % P;
-        const int64_t at = (cell - j % 16) * D + j % 16 * 8;
-        float dot = 0.0f;
-        for (int d = 0; d < D; ++d)
-          dot = fmaf(s_q[d], kv_at<T>(a.cache.k, at + d / 8 * 128 + d % 8), dot);
-        if (T == KvType::kInt8) {
-          dot *= a.cache.k_scale[cell];
-          v_scale = a.cache.v_scale[cell];
-        }
-        s = dot;
-      }
-    }
-    float top = s;
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-    // A NaN logit (no key with it may be lost in the maximum) makes the row NaN below.
-    const float m_new = fmaxf(m, top);
-    const bool any = __any(cell >= 0);
-    if (!any) continue;
-    const float ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float keep = expf(m - ref), p = cell >= 0 ? expf(s - ref) : 0.0f;
-    float sum = p;
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-    l = l * keep + sum;
-    m = m_new;
-    s_p[lane] = p * v_scale;
-    s_cell[lane] = cell;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d >= D) break;
-      float o = acc[i] * keep;
-      for (int x = 0; x < 64; ++x) {
-        const int64_t c = s_cell[x];
-        if (c < 0) continue;
-        const int r = (j0 + x) % 16;
-        o = fmaf(s_p[x],
-                 kv_at<T>(a.cache.v, (c - r) * D + r / 4 % 2 * D * 8 + d * 8 + r / 8 * 4 + r % 4),
-                 o);
-      }
-      acc[i] = o;
-    }
-    __syncthreads();
-  }
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (T == KvType::kBF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <KvType T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (T == KvType::kBF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Four 8-bit quants to f16 (exact): 0x6400 | u is 1024 + u.
+__device__ __forceinline__ u32x2 quants_to_f16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;  // q + 128
+  const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+  const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+  const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  return u32x2{__builtin_bit_cast(uint32_t, lo - off), __builtin_bit_cast(uint32_t, hi - off)};
+}
+__device__ __forceinline__ u32x4 quants_to_f16(u32x2 w) {
+  const u32x2 a = quants_to_f16(w.x), b = quants_to_f16(w.y);
+  return u32x4{a.x, a.y, b.x, b.y};
+}
+
+// Bit 15 of each 16-bit half whose value is an infinity or a NaN.
+template <KvType T>
+__device__ __forceinline__ uint32_t non_finite(uint32_t w) {
+  constexpr uint32_t e = T == KvType::kBF16 ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t one = T == KvType::kBF16 ? 0x00800080u : 0x04000400u;
+  return ((w & e) + one) & 0x80008000u;
+}
+
+template <KvType T>
+__device__ __forceinline__ float value_of(uint32_t half) {
+  if constexpr (T == KvType::kBF16) return __builtin_bit_cast(float, half << 16);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+}
+
+template <KvType T>
+__device__ __forceinline__ bool is_non_finite(uint32_t half) {
+  constexpr uint32_t e = T == KvType::kBF16 ? 0x7f80u : 0x7c00u;
+  return (half & e) == e;
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The scale of a V row as its logarithm and inverse; an all-zero row's scale of 0 counts as
+// a tiny one (its quants are 0).  NaN and infinity stay in the logarithm, which hidden keys
+// do not use; the inverse, times their weight of 0, is always finite.
+__device__ __forceinline__ void v_scale_parts(float v, float* log2v, float* inv) {
+  const float s = v <= kTinyScale ? kTinyScale : v;
+  *log2v = __builtin_amdgcn_logf(s);
+  *inv = s == s ? __builtin_amdgcn_rcpf(s) : 1.0f;
+}
+
+// Power of two that brings a row of q to [2^9, 2^10), and its inverse.
+__device__ __forceinline__ void row_scale(uint32_t amax_bits, float* up, float* down) {
+  const int ex = (int)(amax_bits >> 23);
+  int f = 0;  // non-finite rows: any
+  if (amax_bits != 0 && ex != 255) f = 136 - ex < 126 ? 136 - ex : 126;
+  *up = __builtin_bit_cast(float, (uint32_t)(127 + f) << 23);
+  *down = __builtin_bit_cast(float, (uint32_t)(127 - f) << 23);
+}
+
+__device__ __forceinline__ uint32_t magnitude(f32x4 v) {
+  uint32_t m = 0;
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < D) a.out[row * a.out_stride + (int64_t)h * D + d] = l != 0.0f ? acc[i] / l : 0.0f;
+    const uint32_t b = __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu;
+    m = b > m ? b : m;
   }
+  return m;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x);
+}
+// A value, made anew: what is computed from it is computed there, instead of before a loop
+// and kept in registers across it.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ int fresh_tid() { return fresh((int)threadIdx.x); }
+__device__ __forceinline__ int from_lane(int v, int lane) {
+  return __builtin_amdgcn_ds_bpermute(lane << 2, v);
+}
+__device__ __forceinline__ int64_t from_lane(int64_t v, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)from_lane((int)(v >> 32), lane) << 32 |
+                   (uint32_t)from_lane((int)v, lane));
+}
+
+// f of a value and that of the lane 32 (16) away, in both.
+template <class F>
+__device__ __forceinline__ uint32_t with_32(uint32_t v, F f) {
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f((uint32_t)r[0], (uint32_t)r[1]);
+}
+template <class F>
+__device__ __forceinline__ uint32_t with_16(uint32_t v, F f) {
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return f((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ uint32_t max_bits(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t max_float(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(
+      uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+}
+__device__ __forceinline__ uint32_t sum_float(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+}
+template <class F>
+__device__ __forceinline__ float with_32(float v, F f) {
+  return __builtin_bit_cast(float, with_32(__builtin_bit_cast(uint32_t, v), f));
+}
+template <class F>
+__device__ __forceinline__ float with_16(float v, F f) {
+  return __builtin_bit_cast(float, with_16(__builtin_bit_cast(uint32_t, v), f));
+}
+
+// The kernel's first argument, read anew for the same reason.
+__device__ __forceinline__ AttentionArgs fresh_args() {
+  typedef const __attribute__((address_space(4))) AttentionArgs* Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttentionArgs*)p;
+}
+__device__ __forceinline__ int64_t lane_of(int64_t x, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+                   (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
+}
+
+// ---- the work ----
+
+struct Seq {
+  int row0, n, pos0;  // first row, rows, position of the first row
+};
+
+__device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int b) {
+  // Offsets and lengths come from the caller's device memory: held to their range.
+  int c0 = a.cu[b], c1 = a.cu[b + 1], len = a.kv_lens[b];
+  c0 = c0 < 0 ? 0 : c0 < a.tokens ? c0 : a.tokens;
+  c1 = c1 < c0 ? c0 : c1 < a.tokens ? c1 : a.tokens;
+  return {c0, c1 - c0, (len < 0 ? 0 : len) - (c1 - c0)};
+}
+
+__device__ __forceinline__ int clamp_key(int64_t x, int most) {
+  return (int)(x < 0 ? 0 : x < most ? x : most);
+}
+
+// Keys of the rows [r0, r1) of a sequence: any row sees [lo, hi), every row [lo_all, hi_all).
+struct Span {
+  int lo, hi, lo_all, hi_all;
+};
+
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, const Seq& s, int group, int r0,
+                                        int r1) {
+  const int most = a.max_pages * a.cache.page_size;
+  const int64_t first = (int64_t)s.pos0 + r0 / group, last = (int64_t)s.pos0 + (r1 - 1) / group;
+  Span x;
+  x.hi = clamp_key(last + 1, most);
+  x.hi_all = clamp_key(first + 1, most);
+  x.lo = a.window > 0 ? clamp_key(first - a.window + 1, x.hi) : 0;
+  x.lo_all = a.window > 0 ? clamp_key(last - a.window + 1, most) : 0;
+  return x;
+}
+
+__device__ __forceinline__ int tile_rows(int rows) {
+  return rows <= kFewRows ? kFewRows : kTileRows;
+}
+
+// Units of a row tile; a tile that sees no key counts as one (its zeros are written).
+__device__ __forceinline__ int tile_units(const AttentionArgs& a, const Seq& s, int group,
+                                          int tile) {
+  const int rows = s.n * group, tr = tile_rows(rows), r0 = tile * tr;
+  const Span x = span_of(a, s, group, r0, rows < r0 + tr ? rows : r0 + tr);
+  const int units = (x.hi + kUnit - 1) / kUnit - x.lo / kUnit;
+  return units > 1 ? units : 1;
+}
+
+__device__ __forceinline__ int tiles_of(const Seq& s, int group) {
+  const int rows = s.n * group, tr = tile_rows(rows);
+  return (rows + tr - 1) / tr;
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = from_lane(v, lane - off);
+    if (lane >= off) v += o;
+  }
+  return v;
+}
+
+// What one workgroup does in one go: some units of one row tile.
+struct Segment {
+  int b, g;
+  Seq seq;
+  int r0, rows;       // the tile's first row, and its rows
+  Span span;
+  int k0, k1;         // keys of the segment, multiples of kUnit
+  int parts;          // workgroups that share the tile
+  int part, first;    // which of them this is, and the first one's index
+};
+
+// The same in every lane, and told so: the fields stay in scalar registers.
+__device__ __forceinline__ Segment uniform(const Segment& s) {
+  return {uniform(s.b), uniform(s.g),
+          {uniform(s.seq.row0), uniform(s.seq.n), uniform(s.seq.pos0)},
+          uniform(s.r0), uniform(s.rows),
+          {uniform(s.span.lo), uniform(s.span.hi), uniform(s.span.lo_all),
+           uniform(s.span.hi_all)},
+          uniform(s.k0), uniform(s.k1), uniform(s.parts), uniform(s.part), uniform(s.first)};
+}
+
+struct Shared {
+  float* partials;
+  uint32_t* counters;
+  int slot_floats;
+};
+
+// Device memory of a tile's part: workgroup `first + part` has two slots, for a tile that
+// came from the workgroup before and for one that goes on in the next.
+__device__ __forceinline__ uint32_t slot_at(const Shared& sh, const Segment& s, int part) {
+  return (uint32_t)((s.first + part) * 2 + (part == 0)) * (uint32_t)sh.slot_floats * 4u;
+}
+
+__device__ __forceinline__ bool last_to_arrive(const Shared& sh, const Segment& s, int* shared) {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0);  // this wave's part has reached the coherence point
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t* c = sh.counters + s.first * kCounterStride;
+    const int n = (int)__hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *shared = n;
+    if (n == s.parts - 1)  // nobody else comes: zero again for the next launch
+      __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  return *shared == s.parts - 1;
+}
+
+// Parts lie at `slot` + `at` bytes: what lanes share, and what they do not.
+__device__ __forceinline__ f32x4 load_part(__amdgpu_buffer_rsrc_t rs, uint32_t at, uint32_t slot) {
+  return __builtin_bit_cast(f32x4,
+                            __builtin_amdgcn_raw_buffer_load_b128(rs, at, slot, kDeviceScope));
+}
+__device__ __forceinline__ f32x2 load_part2(__amdgpu_buffer_rsrc_t rs, uint32_t at,
+                                            uint32_t slot) {
+  return __builtin_bit_cast(f32x2,
+                            __builtin_amdgcn_raw_buffer_load_b64(rs, at, slot, kDeviceScope));
+}
+__device__ __forceinline__ void store_part(f32x4 v, __amdgpu_buffer_rsrc_t rs, uint32_t at,
+                                           uint32_t slot) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, at, slot, kDeviceScope);
+}
+__device__ __forceinline__ void store_part2(f32x2 v, __amdgpu_buffer_rsrc_t rs, uint32_t at,
+                                            uint32_t slot) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), rs, at, slot, kDeviceScope);
+}
+
+// Weight of a partial result with maximum m beside the maximum M of all.
+__device__ __forceinline__ float weight(float m, float M) {
+  return M == -INFINITY ? 0.0f : exp2_of(m - M);
+}
+
+// The tiles of 64 lanes' places: tile index in the cache (of 16 tokens), and whether the
+// lane's tile is there at all.
+struct Tiles {
+  int64_t index;
+  bool bad;
+};
+
+__device__ __forceinline__ Tiles find_tile(const AttentionArgs& a, const Segment& s, int key) {
+  const int P = a.cache.page_size;
+  Tiles t{0, true};
+  if (key < s.span.hi) {
+    const int col = key / P;
+    const int page = a.table[(int64_t)s.b * a.max_pages + col];
+    t.bad = (uint32_t)page >= (uint32_t)a.cache.num_pages;
+    if (!t.bad)
+      t.index = (((int64_t)page * a.cache.kv_heads + s.g) * P + (key - col * P)) / kKvTile;
+  }
+  return t;
+}
+
+// ---- few rows: the workgroup's waves split the keys ----
+
+template <KvType T, int D>
+struct FewRows {
+  static constexpr int kTiles = kBytes<T> ? 4 : 2;    // cache tiles of a wave's step
+  static constexpr int kStep = kTiles * kKvTile;
+  static constexpr int KK = D / 32, DB = D / 16;
+  static constexpr int NQ = (4 * D + kThreads - 1) / kThreads;  // quads of the result a thread
+  using Raw = std::conditional_t<kBytes<T>, u32x2, u32x4>;
+
+  struct Loads {
+    Raw k[kTiles][KK];
+    Raw v[kTiles / 2][DB];
+    f32x4 ks[kBytes<T> ? kTiles : 1], vs[kBytes<T> ? kTiles : 1];
+  };
+
+  static __device__ __forceinline__ u32x4 operand(Raw r) {
+    if constexpr (kBytes<T>) return quants_to_f16(r);
+    else return r;
+  }
+
+  static __device__ __forceinline__ void load_k(const AttentionArgs& a, int lane,
+                                                const int64_t* tile, Loads& x) {
+    constexpr int E = kBytes<T> ? 1 : 2;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.cache.k) + tile[t] * (kKvTile * D * E);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        x.k[t][kk] = *reinterpret_cast<const Raw*>(p + (uint32_t)(kk * 512 * E + lane * 8 * E));
+      if constexpr (kBytes<T>)
+        x.ks[t] = *reinterpret_cast<const f32x4*>(a.cache.k_scale + tile[t] * kKvTile +
+                                                  (lane >> 4) * 4);
+    }
+  }
+
+  // Lane group l / 16 is (tile of the pair, half of the places of four tokens).
+  static __device__ __forceinline__ void load_v(const AttentionArgs& a, int lane,
+                                                const int64_t* tile, Loads& x) {
+    constexpr int E = kBytes<T> ? 1 : 2;
+#pragma unroll
+    for (int u = 0; u < kTiles / 2; ++u) {
+      const int64_t mine = lane < 32 ? tile[2 * u] : tile[2 * u + 1];
+      const uint8_t* p = static_cast<const uint8_t*>(a.cache.v) + mine * (kKvTile * D * E) +
+                         (uint32_t)(((lane >> 4 & 1) * D + (lane & 15)) * 8 * E);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        x.v[u][db] = *reinterpret_cast<const Raw*>(p + db * 128 * E);
+      if constexpr (kBytes<T>)
+#pragma unroll
+        for (int t = 2 * u; t < 2 * u + 2; ++t)
+          x.vs[t] = *reinterpret_cast<const f32x4*>(a.cache.v_scale + tile[t] * kKvTile +
+                                                    (lane >> 4) * 4);
+    }
+  }
+
+  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh,
+                                             uint8_t* smem) {
+    const AttentionArgs a = fresh_args();
+    const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
+    const int quad = lane >> 4;
+    const int group = a.heads / a.cache.kv_heads;
+    const int row = (lane & 15) < s.rows ? lane & 15 : s.rows - 1;
+    const int token = row / group;
+    const Span mine = span_of(a, s.seq, group, row, row + 1);
+    const uint32_t width = mine.hi > mine.lo ? (uint32_t)(mine.hi - mine.lo) : 0;
+
+    // Steps of this wave: s.k0 + (wave + 4 i) kStep.
+    const int hi = s.k1 < s.span.hi ? s.k1 : s.span.hi;
+    int base = s.k0 + wave * kStep;
+    const int held_from = base;
+    constexpr int kAhead = 64 / kTiles;  // steps whose tiles the lanes hold
+    auto look_up = [&](int from) {
+      return find_tile(a, s, from + (lane / kTiles) * 4 * kStep + (lane % kTiles) * kKvTile);
+    };
+    Tiles held = look_up(base);
+    uint64_t bad = __ballot(held.bad);
+    int at = 0;  // step among the held ones
+    Loads x;
+    int64_t tile[kTiles];
+    auto take = [&](int step) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) tile[t] = lane_of(held.index, step * kTiles + t);
+    };
+    auto start = [&] {
+      base = s.k0 + wave * kStep;
+      at = 0;
+      if (base >= hi) return;
+      take(0);
+      load_k(a, lane, tile, x);
+      load_v(a, lane, tile, x);
+    };
+    start();
+
+    // q as the right operand: element 8 (l / 16) + e of each run of 32.
+    const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                     (int64_t)(s.g * group + row - token * group) * D + quad * 8;
+    u32x4 qp[kParts<T>][KK];
+    float c;  // logits in units of log2 are S * c
+    {
+      f32x4 v[KK][2];
+      uint32_t amax = 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          v[kk][h] = *reinterpret_cast<const f32x4*>(q + kk * 32 + h * 4);
+          const uint32_t m = magnitude(v[kk][h]);
+          amax = m > amax ? m : amax;
+        }
+      amax = with_32(with_16(amax, max_bits), max_bits);
+      float up, down;
+      row_scale(amax, &up, &down);
+      if (a.scale < 0.0f) up = -up;
+      c = fmaxf(__builtin_fabsf(a.scale) * 1.44269504f * down, 0x1p-120f);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        uint32_t w[kParts<T>][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          split2<T>(v[kk][i >> 1][(i & 1) * 2] * up, v[kk][i >> 1][(i & 1) * 2 + 1] * up,
+                    &w[0][i], 4);
+#pragma unroll
+        for (int p = 0; p < kParts<T>; ++p) qp[p][kk] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+      }
+    }
+
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc[DB] = {};
+    bool careful = false;
+  again:
+    for (; base < hi; base += 4 * kStep) {
+      // The step's keys are whole for every row, or each lane's keys are checked.
+      const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
+      const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0 &&
+                         !careful;
+
+      float sc[kTiles][4];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        f32x4 r = {};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const u32x4 kf = operand(x.k[t][kk]);
+#pragma unroll
+          for (int p = 0; p < kParts<T>; ++p) r = mfma16<T>(kf, qp[p][kk], r);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][i] = r[i];
+      }
+      float inv[kTiles][4];
+      if constexpr (kBytes<T>)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float lv;
+            v_scale_parts(x.vs[t][i], &lv, &inv[t][i]);
+            sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], lv);
+          }
+
+      // The next step's K goes out before the softmax.
+      const bool more = base + 4 * kStep < hi;
+      int64_t tile_now[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) tile_now[t] = tile[t];
+      if (more) {
+        if (++at == kAhead) {
+          held = look_up(base + 4 * kStep);
+          bad = __ballot(held.bad);
+          at = 0;
+        }
+        take(at);
+        load_k(a, lane, tile, x);
+      }
+
+      if (!whole) {
+        const int from = fresh(base + quad * 4 - mine.lo);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool seen = (uint32_t)(from + t * kKvTile + i) < width && !(bad_now >> t & 1);
+            sc[t][i] = seen ? sc[t][i] : -INFINITY;
+          }
+      }
+      const float to_log2 = kBytes<T> ? 1.0f : c;
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
+      top *= to_log2;
+      if (__any(top > m + kSlack)) {
+        top = with_32(with_16(top, max_float), max_float);
+        const float to = fmaxf(m, top);
+        const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
+        m = to;
+        l *= keep;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] *= keep;
+      }
+      const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = exp2_of(__builtin_fmaf(sc[t][i], to_log2, -ref));
+          if constexpr (kBytes<T>) l = __builtin_fmaf(p, inv[t][i], l);
+          else l += p;
+          sc[t][i] = p;
+        }
+
+      bool odd = false;  // a value of V that is not finite
+      if constexpr (!kBytes<T>) {
+        if (!whole) {
+          // Values that no row sees count as zero.
+          const int from = fresh(base + (lane >> 4 & 1) * 4);
+#pragma unroll
+          for (int u = 0; u < kTiles / 2; ++u) {
+            const int t = 2 * u + (lane >> 5);
+            uint32_t keep[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int key = from + t * kKvTile + (w >> 1) * 8 + (w & 1) * 2;
+              const bool tile_ok = !(bad_now >> t & 1);
+              keep[w] = (tile_ok && key >= s.span.lo && key < s.span.hi ? 0x0000ffffu : 0u) |
+                        (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
+            }
+            uint32_t found = 0;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                x.v[u][db][w] &= keep[w];
+                found |= non_finite<T>(x.v[u][db][w]);
+              }
+            odd = odd || found != 0;
+          }
+          odd = __any(odd);
+          if (odd)
+#pragma unroll
+            for (int u = 0; u < kTiles / 2; ++u)
+#pragma unroll
+              for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                  x.v[u][db][w] &= ~((non_finite<T>(x.v[u][db][w]) >> 15) * 0xffffu);
+        }
+      }
+
+      // P as the right operand: tokens 4 h' .. of a pair of tiles, by one exchange of the
+      // wave's halves.
+#pragma unroll
+      for (int u = 0; u < kTiles / 2; ++u) {
+        uint32_t w[2][2][kParts<T>];  // [tile][pair][part]
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            split2<T>(sc[2 * u + t][2 * h], sc[2 * u + t][2 * h + 1], &w[t][h][0], 1);
+        u32x4 pp[kParts<T>];
+#pragma unroll
+        for (int p = 0; p < kParts<T>; ++p) {
+          const auto e0 = __builtin_amdgcn_permlane32_swap(w[0][0][p], w[1][0][p], false, false);
+          const auto e1 = __builtin_amdgcn_permlane32_swap(w[0][1][p], w[1][1][p], false, false);
+          pp[p] = u32x4{(uint32_t)e0[0], (uint32_t)e1[0], (uint32_t)e0[1], (uint32_t)e1[1]};
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u32x4 vf = operand(x.v[u][db]);
+#pragma unroll
+          for (int p = 0; p < kParts<T>; ++p) acc[db] = mfma16<T>(vf, pp[p], acc[db]);
+        }
+      }
+      if constexpr (!kBytes<T>) {
+        if (odd) {  // values that are not finite, for the rows that see them
+#pragma unroll 1
+          for (int j = 0; j < kStep; ++j) {
+            const int64_t ti = j < kKvTile ? tile_now[0] : tile_now[1];
+            const int tok = j % kKvTile, key = base + j;
+            const bool seen =
+                (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
+            const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
+                                (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t v = p[(db * 16 + quad * 4 + i) * 8];
+                if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
+              }
+          }
+        }
+      }
+      if (more) load_v(a, lane, tile, x);
+    }
+    if constexpr (!kBytes<T>) {
+      float zero = 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
+      if (!careful && __any(zero != zero && l - l == 0.0f)) {
+        careful = true;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = f32x4{};
+        held = look_up(held_from);
+        bad = __ballot(held.bad);
+        start();
+        goto again;
+      }
+    }
+    l = with_32(with_16(l, sum_float), sum_float);
+
+    // Join the four waves; thread tid has the quads tid + 256 i: row tid % 16.
+    f32x4* s_acc = reinterpret_cast<f32x4*>(smem);                // [wave][4 D]
+    f32x2* s_ml = reinterpret_cast<f32x2*>(smem + 4 * 4 * D * 16);  // [wave][16]
+    __syncthreads();  // the memory's earlier readers
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      s_acc[wave * 4 * D + (db * 4 + quad) * 16 + (lane & 15)] = acc[db];
+    if (lane < 16) s_ml[wave * 16 + lane] = f32x2{m, l};
+    __syncthreads();
+    const int r = tid & 15;
+    f32x4 out[NQ] = {};
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_ml[w * 16 + r].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const f32x2 ml = s_ml[w * 16 + r];
+      const float f = weight(ml.x, M);
+      // A NaN row's sum is NaN whatever its weight.
+      L = __builtin_fmaf(ml.y, f, L);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i)
+        if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
+          out[i] += s_acc[w * 4 * D + tid + i * kThreads] * f;
+    }
+
+    if (s.parts > 1) {
+      constexpr uint32_t kMl = kFewRows * D * 4;
+      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
+      const uint32_t to = slot_at(sh, s, s.part);
+      if (r < s.rows) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
+            store_part(out[i], rs, tid * 16, to + i * kThreads * 16);
+        if (tid < 16) store_part2(f32x2{M, L}, rs, tid * 8, to + kMl);
+      }
+      if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return;
+      M = -INFINITY;
+      L = 0.0f;
+#pragma unroll 4
+      for (int p = 0; p < s.parts; ++p)
+        M = fmaxf(M, load_part2(rs, r * 8, slot_at(sh, s, p) + kMl).x);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) out[i] = f32x4{};
+#pragma unroll 4
+      for (int p = 0; p < s.parts; ++p) {
+        const uint32_t from = slot_at(sh, s, p);
+        const f32x2 ml = load_part2(rs, r * 8, from + kMl);
+        const float f = weight(ml.x, M);
+        L = __builtin_fmaf(ml.y, f, L);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
+            out[i] += load_part(rs, tid * 16, from + i * kThreads * 16) * f;
+      }
+    }
+    if (r < s.rows) {
+      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+      const int tok = r / group;
+      float* o = a.out + (int64_t)(s.seq.row0 + tok) * a.out_stride +
+                 (int64_t)(s.g * group + r - tok * group) * D;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const int qd = tid + i * kThreads;
+        if (4 * D % kThreads == 0 || qd < 4 * D)
+          *reinterpret_cast<f32x4*>(o + qd / 16 * 4) = L != 0.0f ? out[i] * inv : f32x4{};
+      }
+    }
+  }
+};
+
+// 16 bytes a lane from global memory to LDS, a wave's 1024 in one run, without registers.
+// Not the builtin: with that every later read of LDS first waits for all loads in flight.
+// The caller waits (wait_for_loads) before the barrier behind which the bytes are read.
+// Nothing else here uses m0 (an asm cannot name it as overwritten).
+__device__ __forceinline__ void load_to_lds(const uint8_t* from, uint8_t* to) {
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(uniform((int)at)), "v"(from) : "memory");
+}
+
+__device__ __forceinline__ void wait_for_loads() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// ---- many rows: four waves of 32 rows share the keys in LDS ----
+
+template <KvType T, int D>
+struct ManyRows {
+  static constexpr int KK = D / 16, DB = D / 32;
+  static constexpr int kTilesUnit = kUnit / kKvTile;
+  static constexpr int kTileBytes = kKvTile * D * 2;         // in LDS: 16-bit elements
+  static constexpr int kHalf = kUnit * D * 2;                // K or V of a stage
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kScales = 2 * kStage;                 // [2][3][64] floats (8-bit caches)
+  static constexpr int kFlags = kScales + (kBytes<T> ? 2 * 3 * kUnit * 4 : 0);  // two of any_of
+  static constexpr int kLdsBytes = kFlags + 32;
+  // 16-byte loads of a stage's K, a thread (8-bit head sizes of 96: some threads none).
+  static constexpr int kChunks = kUnit * D * (kBytes<T> ? 1 : 2) / 16;
+  static constexpr int kLoads = (kChunks + kThreads - 1) / kThreads;
+
+  struct Staged {  // 8-bit caches: a stage on its way through registers
+    u32x4 k[kBytes<T> ? kLoads : 1], v[kBytes<T> ? kLoads : 1];
+    float ks, vs;
+  };
+
+  // Whether a thread of the workgroup has `mine`; a barrier.  `flags` is written again only
+  // behind a later barrier.
+  static __device__ __forceinline__ bool any_of(bool mine, int wave, uint8_t* flags) {
+    reinterpret_cast<uint32_t*>(flags)[wave] = __any(mine);
+    __syncthreads();
+    const u32x4 all = *reinterpret_cast<const u32x4*>(flags);
+    return uniform((int)(all.x | all.y | all.z | all.w)) != 0;
+  }
+
+  static __device__ __forceinline__ bool has_chunk(int chunk) {
+    return kChunks % kThreads == 0 || chunk < kChunks;
+  }
+
+  // Starts the loads of the unit whose first tile is lane `first` of `tiles`.
+  static __device__ __forceinline__ void issue(const AttentionArgs& a, int tid, int64_t tiles,
+                                               int first, uint8_t* stage, Staged& x) {
+    tid = fresh(tid);
+    const int lane = tid & 63, wave = uniform(tid >> 6);
+    if constexpr (kBytes<T>) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int chunk = tid + i * kThreads, tile = chunk / D;
+        const int64_t at = from_lane(tiles, first + tile) * (kKvTile * D) + (chunk - tile * D) * 16;
+        if (has_chunk(chunk)) {
+          x.k[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.cache.k) + at);
+          x.v[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.cache.v) + at);
+        }
+      }
+      if (wave == 0) {
+        const int64_t mine =
+            from_lane(tiles, first + lane / kKvTile) * kKvTile + lane % kKvTile;
+        x.ks = a.cache.k_scale[mine];
+        x.vs = a.cache.v_scale[mine];
+      }
+    } else {
+      constexpr int kPerTile = kTileBytes / 1024;  // wave loads of a tile
+      static_assert(kTileBytes % 1024 == 0 && kTilesUnit * kPerTile == 4 * kLoads);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int n = i * 4 + wave;  // the wave's load of the stage's K or V
+        const int tile = n / kPerTile, part = n - tile * kPerTile;
+        const int64_t at = lane_of(tiles, first + tile) * kTileBytes + part * 1024 + lane * 16;
+        uint8_t* to = stage + n * 1024;
+        load_to_lds(static_cast<const uint8_t*>(a.cache.k) + at, to);
+        load_to_lds(static_cast<const uint8_t*>(a.cache.v) + at, to + kHalf);
+      }
+    }
+  }
+
+  // 8-bit caches: the staged unit into LDS as f16.
+  static __device__ __forceinline__ void commit(int tid, uint8_t* smem, int buf,
+                                                const Staged& x) {
+    if constexpr (kBytes<T>) {
+      tid = fresh(tid);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int chunk = tid + i * kThreads;
+        if (!has_chunk(chunk)) break;
+        u32x4* k = reinterpret_cast<u32x4*>(smem + buf * kStage) + chunk * 2;
+        u32x4* v = reinterpret_cast<u32x4*>(smem + buf * kStage + kHalf) + chunk * 2;
+        k[0] = quants_to_f16(u32x2{x.k[i].x, x.k[i].y});
+        k[1] = quants_to_f16(u32x2{x.k[i].z, x.k[i].w});
+        v[0] = quants_to_f16(u32x2{x.v[i].x, x.v[i].y});
+        v[1] = quants_to_f16(u32x2{x.v[i].z, x.v[i].w});
+      }
+      if (tid < kUnit) {
+        float* sc = reinterpret_cast<float*>(smem + kScales) + buf * 3 * kUnit;
+        float lv, inv;
+        v_scale_parts(x.vs, &lv, &inv);
+        sc[tid] = x.ks;
+        sc[kUnit + tid] = lv;
+        sc[2 * kUnit + tid] = inv;
+      }
+    }
+  }
+
+  // A unit that some row does not see whole: V's places that no row sees become zero, and so
+  // do values that are not finite, which the caller adds to the rows that see them.  Returns
+  // whether there were any.
+  static __device__ __forceinline__ bool clear_v(const Segment& s, int tid, int base,
+                                                 uint32_t bad, uint8_t* stage) {
+    bool found = false;
+    if constexpr (!kBytes<T>) {
+      tid = fresh(tid);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int chunk = tid + i * kThreads;
+        const int tile = chunk / (2 * D), in = chunk - tile * 2 * D, half = in / D;
+        u32x4* p = reinterpret_cast<u32x4*>(stage + kHalf) + chunk;
+        u32x4 v = *p;
+        const bool tile_ok = !(bad >> tile & 1);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int key = base + tile * kKvTile + (w >> 1) * 8 + half * 4 + (w & 1) * 2;
+          v[w] &= (tile_ok && key >= s.span.lo && key < s.span.hi ? 0x0000ffffu : 0u) |
+                  (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
+          odd |= non_finite<T>(v[w]);
+        }
+        if (odd != 0) {
+          found = true;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[w] &= ~((non_finite<T>(v[w]) >> 15) * 0xffffu);
+        }
+        *p = v;
+      }
+    }
+    return found;
+  }
+
+  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh,
+                                             uint8_t* smem) {
+    const AttentionArgs a = fresh_args();
+    const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
+    const int half = lane >> 5;
+    const int group = a.heads / a.cache.kv_heads;
+    const int wrow = wave * 32 + (lane & 31);
+    const int row = s.r0 + (wrow < s.rows ? wrow : s.rows - 1);
+    const int token = row / group;
+    const bool live = wave * 32 < s.rows;
+    const Span mine = span_of(a, s.seq, group, row, row + 1);
+    const uint32_t width = mine.hi > mine.lo ? (uint32_t)(mine.hi - mine.lo) : 0;
+    // What the wave's rows see together and alone.
+    const int w0 = s.r0 + wave * 32, w1 = s.r0 + (s.rows < wave * 32 + 32 ? s.rows : wave * 32 + 32);
+    const Span ours = span_of(a, s.seq, group, live ? w0 : row, live ? w1 : row + 1);
+
+    const int hi = s.k1 < s.span.hi ? s.k1 : s.span.hi;
+    Staged staged;
+    Tiles held;
+    uint64_t bad = 0;
+    int at = 0;  // unit among the 16 whose tiles the lanes hold
+    auto look_up = [&](int from) {
+      held = find_tile(a, s, from + fresh(lane) * kKvTile);
+      bad = __ballot(held.bad);
+      at = 0;
+    };
+    look_up(s.k0);
+    __syncthreads();  // the memory's earlier readers
+    if (s.k0 < hi) issue(a, tid, held.index, 0, smem, staged);
+
+    u32x4 qp[kParts<T>][KK];
+    float c = 0.0f;
+    {
+      const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                       (int64_t)(s.g * group + row - token * group) * D + half * 8;
+      uint32_t amax = 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t m = magnitude(*reinterpret_cast<const f32x4*>(q + kk * 16 + h * 4));
+          amax = m > amax ? m : amax;
+        }
+      amax = with_32(amax, max_bits);
+      float up, down;
+      row_scale(amax, &up, &down);
+      if (a.scale < 0.0f) up = -up;
+      c = fmaxf(__builtin_fabsf(a.scale) * 1.44269504f * down, 0x1p-120f);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        uint32_t w[kParts<T>][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(q + kk * 16 + h * 4);
+          split2<T>(v.x * up, v.y * up, &w[0][2 * h], 4);
+          split2<T>(v.z * up, v.w * up, &w[0][2 * h + 1], 4);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts<T>; ++p) qp[p][kk] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+      }
+    }
+    if (s.k0 < hi) commit(tid, smem, 0, staged);
+
+    // Operands of 32 keys: K's of all steps, or V's of two tiles; as many either way, all at
+    // once or some of them, as registers allow.
+    constexpr bool kLean = kParts<T> == 3 || kBytes<T>;
+    constexpr int FB = KK / ((kLean ? 2 : 1) * (D > 128 ? 2 : 1));
+    u32x4 f[FB];
+    const uint32_t k_at = (lane >> 4 & 1) * kTileBytes + half * 256 + (lane & 15) * 16;
+    const uint32_t v_at = kHalf + (half * D + (lane & 31)) * 16;
+    auto read_k = [&](const uint8_t* stage, int u, int from) {
+#pragma unroll
+      for (int n = 0; n < FB; ++n)
+        f[n] = *reinterpret_cast<const u32x4*>(stage + k_at + 2 * u * kTileBytes +
+                                               (from + n) * 512);
+    };
+    auto read_v = [&](const uint8_t* stage, int u, int from) {
+#pragma unroll
+      for (int n = 0; n < FB; ++n)
+        f[n] = *reinterpret_cast<const u32x4*>(
+            stage + v_at + (2 * u + (from + n) / DB) * kTileBytes + (from + n) % DB * 512);
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    f32x16 acc[DB] = {};
+    bool careful = false;
+  again:
+    int buf = 0;
+    for (int base = s.k0; base < hi; base += kUnit, buf ^= 1) {
+      const uint32_t bad_now = (uint32_t)(bad >> (at * kTilesUnit)) & ((1u << kTilesUnit) - 1);
+      const int64_t tiles_now = held.index;
+      const int at_now = at;
+      uint8_t* stage = smem + buf * kStage;
+      wait_for_loads();  // this wave's loads of the stage
+      __syncthreads();   // everyone's; and the other stage's readers are done
+      const bool more = base + kUnit < hi;
+      if (more) {
+        if (++at == 64 / kTilesUnit) look_up(base + kUnit);
+        issue(a, tid, held.index, at * kTilesUnit, smem + (buf ^ 1) * kStage, staged);
+      }
+      bool odd = false;
+      if (!kBytes<T> && (careful || base < s.span.lo_all || base + kUnit > s.span.hi_all ||
+                         bad_now != 0))
+        odd = any_of(clear_v(s, tid, base, bad_now, stage), wave, smem + kFlags);
+
+      if (live && base < ours.hi && base + kUnit > ours.lo) {
+        const bool whole = base >= ours.lo_all && base + kUnit <= ours.hi_all && bad_now == 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // 32 keys: two tiles
+          f32x16 sc = {};
+#pragma unroll
+          for (int from = 0; from < KK; from += FB) {
+            read_k(stage, u, from);
+#pragma unroll
+            for (int n = 0; n < FB; ++n)
+#pragma unroll
+              for (int p = 0; p < kParts<T>; ++p) sc = mfma32<T>(f[n], qp[p][from + n], sc);
+          }
+          read_v(stage, u, 0);  // on its way during the softmax
+          __builtin_amdgcn_sched_barrier(0);
+          const float* ks = reinterpret_cast<const float*>(smem + kScales) + buf * 3 * kUnit +
+                            u * 32 + half * 4;
+          if constexpr (kBytes<T>) {
+#pragma unroll
+            for (int b4 = 0; b4 < 4; ++b4) {
+              const f32x4 k4 = *reinterpret_cast<const f32x4*>(ks + b4 * 8);
+              const f32x4 l4 = *reinterpret_cast<const f32x4*>(ks + kUnit + b4 * 8);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
+            }
+          }
+          if (!whole) {
+            const int from = fresh(base + half * 4 - mine.lo);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const bool seen = (uint32_t)(from + u * 32 + (i >> 2) * 8 + (i & 3)) < width &&
+                                !(bad_now >> (2 * u + (i >> 3)) & 1);
+              sc[i] = seen ? sc[i] : -INFINITY;
+            }
+          }
+          const float to_log2 = kBytes<T> ? 1.0f : c;
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
+          top *= to_log2;
+          if (__any(top > m + kSlack)) {
+            top = with_32(top, max_float);
+            const float to = fmaxf(m, top);
+            const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
+            m = to;
+            l *= keep;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= keep;
+          }
+          const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
+          uint32_t w[kParts<T>][8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float p0 = exp2_of(__builtin_fmaf(sc[i], to_log2, -ref));
+            const float p1 = exp2_of(__builtin_fmaf(sc[i + 1], to_log2, -ref));
+            if constexpr (kBytes<T>) {
+              const f32x2 inv = *reinterpret_cast<const f32x2*>(ks + 2 * kUnit + (i >> 2) * 8 +
+                                                                (i & 3));
+              l = __builtin_fmaf(p0, inv.x, l);
+              l = __builtin_fmaf(p1, inv.y, l);
+            } else {
+              l += p0;
+              l += p1;
+            }
+            split2<T>(p0, p1, &w[0][i / 2], 8);
+          }
+#pragma unroll
+          for (int from = 0; from < KK; from += FB) {
+            if (from > 0) read_v(stage, u, from);
+#pragma unroll
+            for (int n = 0; n < FB; ++n) {
+              const int t = (from + n) / DB, db = (from + n) % DB;
+#pragma unroll
+              for (int p = 0; p < kParts<T>; ++p)
+                acc[db] = mfma32<T>(
+                    f[n], u32x4{w[p][4 * t], w[p][4 * t + 1], w[p][4 * t + 2], w[p][4 * t + 3]},
+                    acc[db]);
+            }
+          }
+        }
+        if constexpr (!kBytes<T>) {
+          if (odd) {  // values that are not finite, for the rows that see them
+#pragma unroll 1
+            for (int j = 0; j < kUnit; ++j) {
+              const int tok = j % kKvTile, key = base + j;
+              const bool seen =
+                  (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
+              const int64_t ti = lane_of(tiles_now, at_now * kTilesUnit + j / kKvTile);
+              const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
+                                  (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
+#pragma unroll
+              for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const uint32_t v = p[(db * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * 8];
+                  if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
+                }
+            }
+          }
+        }
+      }
+      if (more) commit(tid, smem, buf ^ 1, staged);
+    }
+    if constexpr (!kBytes<T>) {
+      float zero = 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
+      if (!careful && any_of(zero != zero && l - l == 0.0f, wave, smem + kFlags + 16)) {
+        careful = true;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+        look_up(s.k0);
+        __syncthreads();
+        if (s.k0 < hi) issue(a, tid, held.index, 0, smem, staged);
+        goto again;
+      }
+    }
+    l = with_32(l, sum_float);
+
+    if (s.parts > 1) {
+      constexpr uint32_t kMl = kTileRows * D * 4;
+      const int at = fresh(tid);
+      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
+      const uint32_t to = slot_at(sh, s, s.part);
+      if (wrow < s.rows) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            store_part(f32x4{acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2],
+                             acc[db][4 * q + 3]},
+                       rs, at * 16, to + (db * 4 + q) * kThreads * 16);
+        store_part2(f32x2{m, l}, rs, at * 8, to + kMl);
+      }
+      if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return;
+      if (wrow >= s.rows) return;
+      m = -INFINITY;
+      l = 0.0f;
+#pragma unroll 4
+      for (int p = 0; p < s.parts; ++p)
+        m = fmaxf(m, load_part2(rs, at * 8, slot_at(sh, s, p) + kMl).x);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+#pragma unroll 1
+      for (int p = 0; p < s.parts; ++p) {
+        const uint32_t from = slot_at(sh, s, p);
+        const f32x2 ml = load_part2(rs, at * 8, from + kMl);
+        const float f = weight(ml.x, m);
+        l = __builtin_fmaf(ml.y, f, l);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = load_part(rs, at * 16, from + (db * 4 + q) * kThreads * 16) * f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[db][4 * q + i] += v[i];
+          }
+      }
+    }
+    if (wrow < s.rows) {
+      const float inv = 1.0f / l;
+      float* o = a.out + (int64_t)(s.seq.row0 + token) * a.out_stride +
+                 (int64_t)(s.g * group + row - token * group) * D + half * 4;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v = {acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2], acc[db][4 * q + 3]};
+          v = l != 0.0f ? v * inv : f32x4{};
+          *reinterpret_cast<f32x4*>(o + db * 32 + q * 8) = v;
+        }
+    }
+  }
+};
+
+// The segment that starts with unit *u of a workgroup's run, which *u then moves past.  *b is
+// the unit's sequence or one before it, *base the units before that one.
+__device__ __forceinline__ Segment segment_of(int w, uint64_t per, uint64_t u_end, uint64_t* u,
+                                              int* b, uint64_t* base) {
+  const AttentionArgs a = fresh_args();
+  asm volatile("" : "+s"(per));  // as above: no reciprocal of it is kept
+  const int lane = fresh_tid() & 63, G = a.cache.kv_heads, group = a.heads / G;
+  Segment s;
+  uint64_t of_head;
+  for (;; ++*b) {
+    s.seq = seq_of(a, *b);
+    const int tiles = tiles_of(s.seq, group);
+    int n = 0;
+    for (int t = lane; t < tiles; t += 64) n += tile_units(a, s.seq, group, t);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) n += from_lane(n, lane ^ off);
+    of_head = (uint64_t)(uint32_t)uniform(n);
+    if (*u < *base + of_head * G) break;
+    *base = uniform(*base + of_head * G);
+  }
+  s.b = *b;
+  s.g = (int)((*u - *base) / of_head);
+  const uint64_t head_start = *base + s.g * of_head;
+  const uint32_t in_head = (uint32_t)(*u - head_start);
+  const int rows = s.seq.n * group, tr = tile_rows(rows), tiles = tiles_of(s.seq, group);
+  uint32_t tile_start = 0;  // units of the head's tiles before the one sought
+  int tile = 0, units = 0;
+  for (int t0 = 0;; t0 += 64) {
+    const int mine = t0 + lane < tiles ? tile_units(a, s.seq, group, t0 + lane) : 0;
+    const int upto = wave_scan(mine, lane);
+    const uint64_t past = __ballot((uint32_t)upto + tile_start > in_head);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      tile = t0 + at;
+      units = __builtin_amdgcn_readlane(mine, at);
+      tile_start += (uint32_t)(__builtin_amdgcn_readlane(upto, at) - units);
+      break;
+    }
+    tile_start += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+  }
+  s.r0 = tile * tr;
+  s.rows = rows - s.r0 < tr ? rows - s.r0 : tr;
+  s.span = span_of(a, s.seq, group, s.r0, s.r0 + s.rows);
+  const uint64_t i0 = head_start + tile_start, i1 = i0 + units;
+  const uint64_t stop = u_end < i1 ? u_end : i1;
+  const int k_first = s.span.lo / kUnit * kUnit;
+  s.k0 = k_first + (int)(*u - i0) * kUnit;
+  s.k1 = k_first + (int)(stop - i0) * kUnit;
+  s.first = (int)(i0 / per);
+  s.part = w - s.first;
+  s.parts = (int)((i1 - 1) / per) - s.first + 1;
+  *u = uniform(stop);
+  *b = uniform(*b);
+  return uniform(s);
+}
+
+template <KvType T, int D>
+constexpr int kLds = ManyRows<T, D>::kLdsBytes > 4 * 16 * (D * 4 + 8)
+                         ? ManyRows<T, D>::kLdsBytes : 4 * 16 * (D * 4 + 8);
+
+template <KvType T, int D>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(AttentionArgs a,
+                                                                               Shared sh) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kLds<T, D>];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int G = a.cache.kv_heads, group = a.heads / G;
+
+  // Units of all sequences: inclusive sums over the threads, each with `chunk` sequences.
+  uint64_t* s_sum = reinterpret_cast<uint64_t*>(smem);
+  const int chunk = (a.sequences + kThreads - 1) / kThreads;
+  uint64_t sum = 0;
+  for (int i = 0; i < chunk; ++i) {
+    const int b = tid * chunk + i;
+    if (b >= a.sequences) break;
+    const Seq s = seq_of(a, b);
+    const int tiles = tiles_of(s, group);
+    for (int t = 0; t < tiles; ++t) sum += (uint64_t)tile_units(a, s, group, t) * G;
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_up((unsigned long long)sum, off);
+    if (lane >= off) sum += o;
+  }
+  if (lane == 63) s_sum[kThreads + wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += s_sum[kThreads + w];
+  s_sum[tid] = sum;
+  __syncthreads();
+  const uint64_t total = uniform(s_sum[kThreads - 1]);
+  if (total == 0) return;
+
+  // Equal runs of units; neighbouring runs on one XCD, whose L2 they share.
+  uint64_t per = (total + gridDim.x - 1) / gridDim.x;
+  per = uniform(per < 2 ? 2 : per);
+  const int used = (int)((total + per - 1) / per);
+  const int by_xcd = (used + 7) / 8;
+  const int w = (int)(blockIdx.x % 8) * by_xcd + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= by_xcd || w >= used) return;
+  uint64_t u = uniform((uint64_t)w * per);
+  const uint64_t u_end = uniform(u + per < total ? u + per : total);
+
+  const int before = __syncthreads_count(s_sum[tid] <= u);
+  int b = uniform(before * chunk);
+  uint64_t base = before > 0 ? uniform(s_sum[before - 1]) : 0;
+  __syncthreads();
+
+  while (u < u_end) {
+    const Segment s = segment_of(w, per, u_end, &u, &b, &base);
+    if (tile_rows(s.seq.n * (a.heads / a.cache.kv_heads)) == kFewRows)
+      FewRows<T, D>::run(s, sh, smem);
+    else
+      ManyRows<T, D>::run(s, sh, smem);
+  }
+}
+
+constexpr int kCus = 256;
+
+int grid_of(int head_dim) { return kCus * (head_dim <= 128 ? 2 : 1); }
+
+int slot_floats_of(int head_dim, int64_t rows) {
+  return (rows <= kFewRows ? kFewRows : kTileRows) * (head_dim + 4);
+}
+
+template <KvType T>
+hipError_t launch_typed(const AttentionArgs& a, const Shared& sh, hipStream_t stream) {
+  const dim3 grid((unsigned)grid_of(a.cache.head_dim)), block(kThreads);
+  switch (a.cache.head_dim) {
+    case 64: hipLaunchKernelGGL((attention_kernel<T, 64>), grid, block, 0, stream, a, sh); break;
+    case 96: hipLaunchKernelGGL((attention_kernel<T, 96>), grid, block, 0, stream, a, sh); break;
+    case 128: hipLaunchKernelGGL((attention_kernel<T, 128>), grid, block, 0, stream, a, sh); break;
+    default: hipLaunchKernelGGL((attention_kernel<T, 256>), grid, block, 0, stream, a, sh);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_paged_attention(const AttentionArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)a.tokens, (unsigned)a.heads), block(64);
+SplitKNeed paged_attention_workspace(int head_dim, int64_t rows) {
+  SplitKNeed need;
+  need.splits = grid_of(head_dim);
+  need.partial_floats = (size_t)need.splits * 2 * slot_floats_of(head_dim, rows);
+  need.counters = (size_t)need.splits * kCounterStride;
+  return need;
+}
+
+hipError_t launch_paged_attention(const AttentionArgs& a, const SplitKWorkspace& ws,
+                                  hipStream_t stream) {
+  const int64_t rows = (int64_t)a.tokens * (a.heads / a.cache.kv_heads);
+  const Shared sh{ws.partials, ws.counters, slot_floats_of(a.cache.head_dim, rows)};
   switch (a.cache.type) {
-    case KvType::kF16:
-      hipLaunchKernelGGL(attention_rows_kernel<KvType::kF16>, grid, block, 0, stream, a);
-      break;
-    case KvType::kBF16:
-      hipLaunchKernelGGL(attention_rows_kernel<KvType::kBF16>, grid, block, 0, stream, a);
-      break;
-    default:
-      hipLaunchKernelGGL(attention_rows_kernel<KvType::kInt8>, grid, block, 0, stream, a);
+    case KvType::kF16: return launch_typed<KvType::kF16>(a, sh, stream);
+    case KvType::kBF16: return launch_typed<KvType::kBF16>(a, sh, stream);
+    default: return launch_typed<KvType::kInt8>(a, sh, stream);
   }
-  return hipGetLastError();
 }
 
 }  // namespace mle

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "launch.hpp"
+
 namespace mle {
 
 constexpr int kKvTile = 16;  // tokens of a cache tile
@@ -78,6 +80,9 @@ struct AttentionArgs {
   int sequences;
   int tokens;
 };
-hipError_t launch_paged_attention(const AttentionArgs& a, hipStream_t stream);
+// Workspace of a call with `rows` rows of one KV head (new tokens * heads / kv_heads).
+SplitKNeed paged_attention_workspace(int head_dim, int64_t rows);
+hipError_t launch_paged_attention(const AttentionArgs& a, const SplitKWorkspace& ws,
+                                  hipStream_t stream);
 
 }  // namespace mle
