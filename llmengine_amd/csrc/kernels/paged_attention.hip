@@ -140,10 +140,11 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 // The scale of a V row as its logarithm and inverse; an all-zero row's scale of 0 counts as
 // a tiny one (its quants are 0).  NaN and infinity stay in the logarithm, which hidden keys
 // do not use; the inverse, times their weight of 0, is always finite.
-__device__ __forceinline__ void v_scale_parts(float v, float* log2v, float* inv) {
-  const float s = v <= kTinyScale ? kTinyScale : v;
-  *log2v = __builtin_amdgcn_logf(s);
-  *inv = s == s ? __builtin_amdgcn_rcpf(s) : 1.0f;
+__device__ __forceinline__ float scale_log2(float v) {
+  return __builtin_amdgcn_logf(v <= kTinyScale ? kTinyScale : v);
+}
+__device__ __forceinline__ float scale_inverse(float v) {
+  return __builtin_amdgcn_rcpf(v > kTinyScale ? v : v <= kTinyScale ? kTinyScale : 1.0f);
 }
 
 // Power of two that brings a row of q to [2^9, 2^10), and its inverse.
@@ -248,43 +249,75 @@ struct Span {
   int lo, hi, lo_all, hi_all;
 };
 
-__device__ __forceinline__ Span span_of(const AttentionArgs& a, const Seq& s, int group, int r0,
-                                        int r1) {
-  const int most = a.max_pages * a.cache.page_size;
-  const int64_t first = (int64_t)s.pos0 + r0 / group, last = (int64_t)s.pos0 + (r1 - 1) / group;
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, const Seq& s, int r0, int r1) {
+  const int64_t first = (int64_t)s.pos0 + (int)a.by_group.of(r0);
+  const int64_t last = (int64_t)s.pos0 + (int)a.by_group.of(r1 - 1);
   Span x;
-  x.hi = clamp_key(last + 1, most);
-  x.hi_all = clamp_key(first + 1, most);
+  x.hi = clamp_key(last + 1, a.most);
+  x.hi_all = clamp_key(first + 1, a.most);
   x.lo = a.window > 0 ? clamp_key(first - a.window + 1, x.hi) : 0;
-  x.lo_all = a.window > 0 ? clamp_key(last - a.window + 1, most) : 0;
+  x.lo_all = a.window > 0 ? clamp_key(last - a.window + 1, a.most) : 0;
   return x;
 }
 
-__device__ __forceinline__ int tile_rows(int rows) {
-  return rows <= kFewRows ? kFewRows : kTileRows;
-}
+// What the row tiles of a (sequence, KV head) cost: tile t counts min(first + t slope, cap),
+// a linear account of its units (causality adds keys from tile to tile, a window ends that)
+// and of its beginning and end.  Only the balance depends on how close it is.
+struct Cost {
+  int tiles;
+  int first, slope, cap;
 
-// Units of a row tile; a tile that sees no key counts as one (its zeros are written).
-__device__ __forceinline__ int tile_units(const AttentionArgs& a, const Seq& s, int group,
-                                          int tile) {
-  const int rows = s.n * group, tr = tile_rows(rows), r0 = tile * tr;
-  const Span x = span_of(a, s, group, r0, rows < r0 + tr ? rows : r0 + tr);
-  const int units = (x.hi + kUnit - 1) / kUnit - x.lo / kUnit;
-  return units > 1 ? units : 1;
-}
-
-__device__ __forceinline__ int tiles_of(const Seq& s, int group) {
-  const int rows = s.n * group, tr = tile_rows(rows);
-  return (rows + tr - 1) / tr;
-}
-
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = from_lane(v, lane - off);
-    if (lane >= off) v += o;
+  __device__ __forceinline__ int of(int t) const {
+    const int64_t v = (int64_t)first + (int64_t)t * slope;
+    return (int)(v < cap ? v : cap);
   }
-  return v;
+  // Of the tiles before t.
+  __device__ __forceinline__ uint64_t before(int t) const {
+    int ramp = t;  // tiles below the cap
+    if (first >= cap) ramp = 0;
+    else if (slope > 0 && (cap - first) / slope + 1 < t) ramp = (cap - first) / slope + 1;
+    return (uint64_t)ramp * first + (uint64_t)slope * ((uint64_t)ramp * (ramp - 1) / 2) +
+           (uint64_t)(t - ramp) * cap;
+  }
+};
+
+// Cost of a unit of many and of few rows, of a tile besides its units, and the least piece of
+// a tile worth a workgroup of its own: 64 keys of 128 rows take about 3.5 us beside another
+// workgroup (half as much again with three parts), of few rows 2 to 4; a tile's beginning and
+// end about three units.
+template <KvType T>
+struct Weights {
+  static constexpr int kMany = kParts<T> * 16;
+  static constexpr int kFew = kBytes<T> ? 16 : 24;
+  static constexpr int kTile = 64;
+  static constexpr int kLeast = 64;
+};
+
+template <KvType T>
+__device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Seq& s) {
+  constexpr int kMax = 1 << 29;
+  const int rows = s.n * a.group;
+  const bool few = rows <= kFewRows;
+  const int unit = few ? Weights<T>::kFew : Weights<T>::kMany;
+  auto units = [&](int64_t keys) {  // at least a partial one
+    const int64_t v = (keys > 0 ? (keys * unit) / kUnit : 0) + unit / 2 + Weights<T>::kTile;
+    return (int)(v < kMax ? v : kMax);
+  };
+  Cost c;
+  c.tiles = few ? rows > 0 : (rows + kTileRows - 1) / kTileRows;
+  const int tokens = c.tiles > 1 ? (int)a.by_group.of(kTileRows + a.group - 1) : s.n;
+  c.cap = a.window > 0 ? units((int64_t)a.window + tokens) : kMax;
+  c.first = units((int64_t)s.pos0 + tokens);
+  c.slope = (int)a.by_group.of(2 * Weights<T>::kMany);  // kTileRows / group keys
+  return c;
+}
+
+// floor(x / d) for quotients below 2^31.
+__device__ __forceinline__ uint32_t quotient(uint64_t x, uint64_t d) {
+  uint32_t q = (uint32_t)((double)x * __builtin_amdgcn_rcp((double)d));
+  while ((uint64_t)q * d > x) --q;
+  while ((uint64_t)(q + 1) * d <= x) ++q;
+  return q;
 }
 
 // What one workgroup does in one go: some units of one row tile.
@@ -312,6 +345,150 @@ struct Shared {
   float* partials;
   uint32_t* counters;
   int slot_floats;
+};
+
+// What is written to LDS before is read from there, not kept in registers.
+__device__ __forceinline__ void forget() { asm volatile("" ::: "memory"); }
+
+// The sequences as a workgroup keeps them: thread i those from i * chunk on.
+struct Schedule {
+  uint64_t sum[kThreads];  // of the costs up to and with the thread's
+  Seq seq[kThreads];       // where chunk is 1
+  uint64_t wave_sum[4];
+};
+
+// A workgroup's way through its run of the work.  The whole work, `total`, is cut at
+// w total / 2^k; a cut within kLeast of a tile's begin or end moves there, so that no tile is
+// split for less.
+template <KvType T>
+struct Cursor {
+  int b, g, t;
+  Seq seq;
+  Cost cost;
+  uint64_t i0, i1;         // the current tile's place in the work
+  uint64_t begin;          // where this workgroup takes it up
+  uint64_t end, total;
+  int w, k;
+  bool done;
+
+  // The sequence `b` or the first one after it that has rows; skips *base over the others.
+  __device__ __forceinline__ void seek(const AttentionArgs& a, const Schedule& sch, int chunk) {
+    for (;; ++b) {
+      seq = chunk == 1 ? sch.seq[b] : seq_of(a, b);
+      seq = {uniform(seq.row0), uniform(seq.n), uniform(seq.pos0)};
+      if (seq.n > 0) break;
+    }
+    cost = cost_of<T>(a, seq);
+  }
+
+  __device__ __forceinline__ void advance(const AttentionArgs& a, const Schedule& sch,
+                                          int chunk) {
+    if (++t == cost.tiles) {
+      t = 0;
+      if (++g == a.cache.kv_heads) {
+        g = 0;
+        ++b;
+        seek(a, sch, chunk);
+      }
+    }
+    i0 = i1;
+    begin = i0;
+    i1 = i0 + cost.of(t);
+  }
+
+  // The tile with the work's place `at`, and where in it the cut there lies.  `before`
+  // threads' sequences come wholly before it.
+  __device__ __forceinline__ void locate(const AttentionArgs& a, const Schedule& sch, int chunk,
+                                         int before, uint64_t at) {
+    b = before * chunk;
+    i0 = before > 0 ? uniform(sch.sum[before - 1]) : 0;
+    uint64_t of_head;
+    for (;;) {
+      seek(a, sch, chunk);
+      of_head = cost.before(cost.tiles);
+      if (at < i0 + of_head * a.cache.kv_heads) break;
+      i0 += of_head * a.cache.kv_heads;
+      ++b;
+    }
+    g = (int)quotient(at - i0, of_head);
+    i0 += g * of_head;
+    t = 0;
+    for (int past = cost.tiles; past - t > 1;) {
+      const int mid = t + (past - t) / 2;
+      if (i0 + cost.before(mid) <= at) t = mid; else past = mid;
+    }
+    i0 += cost.before(t);
+    i1 = i0 + cost.of(t);
+    done = false;
+    begin = i0;
+    if (at - i0 >= Weights<T>::kLeast) {
+      begin = at;
+      if (i1 - at < Weights<T>::kLeast) {
+        if (i1 < total) advance(a, sch, chunk);
+        else done = true;
+      }
+    }
+  }
+
+  // Units of the tile that lie before place x of it.
+  static __device__ __forceinline__ int units_at(uint64_t x, uint64_t of, int units) {
+    if (x >= of) return units;
+    const int u = (int)((float)(uint32_t)x *
+                        ((float)units * __builtin_amdgcn_rcpf((float)(uint32_t)of)));
+    return u < units ? u : units;
+  }
+
+  __device__ __forceinline__ Cursor uniform_copy() const {
+    Cursor c;
+    c.b = uniform(b);
+    c.g = uniform(g);
+    c.t = uniform(t);
+    c.seq = {uniform(seq.row0), uniform(seq.n), uniform(seq.pos0)};
+    c.cost = {uniform(cost.tiles), uniform(cost.first), uniform(cost.slope), uniform(cost.cap)};
+    c.i0 = uniform(i0);
+    c.i1 = uniform(i1);
+    c.begin = uniform(begin);
+    c.end = uniform(end);
+    c.total = uniform(total);
+    c.w = uniform(w);
+    c.k = uniform(k);
+    c.done = uniform((int)done) != 0;
+    return c;
+  }
+
+  // The next piece of this workgroup's run; false at its end.
+  __device__ __forceinline__ bool next(const AttentionArgs& a, const Schedule& sch, int chunk,
+                                       Segment* out) {
+    if (done || (int64_t)(end - i0) < Weights<T>::kLeast) return false;
+    const uint64_t stop = (int64_t)(i1 - end) < Weights<T>::kLeast ? i1 : end;
+    Segment s;
+    s.b = b;
+    s.g = g;
+    s.seq = seq;
+    const int rows = seq.n * a.group;
+    const int tr = rows <= kFewRows ? kFewRows : kTileRows;
+    s.r0 = t * tr;
+    s.rows = rows - s.r0 < tr ? rows - s.r0 : tr;
+    s.span = span_of(a, seq, s.r0, s.r0 + s.rows);
+    const int u0 = s.span.lo / kUnit, units = (s.span.hi + kUnit - 1) / kUnit - u0;
+    s.k0 = (u0 + (begin == i0 ? 0 : units_at(begin - i0, i1 - i0, units))) * kUnit;
+    s.k1 = (u0 + units_at(stop - i0, i1 - i0, units)) * kUnit;
+    s.parts = 1;
+    s.part = s.first = 0;
+    if (begin != i0 || stop != i1) {
+      // The cuts inside the tile.
+      const uint64_t lo = i0 + Weights<T>::kLeast, hi = i1 - Weights<T>::kLeast;
+      const int c0 = (int)quotient((lo << k) + total - 1, total);
+      const int c1 = (int)quotient(((hi + 1) << k) - 1, total);
+      s.first = c0 - 1;
+      s.part = w - s.first;
+      s.parts = c1 - c0 + 2;
+    }
+    *out = uniform(s);
+    if (stop != i1 || i1 >= end) done = true;
+    else advance(a, sch, chunk);
+    return true;
+  }
 };
 
 // Device memory of a tile's part: workgroup `first + part` has two slots, for a tile that
@@ -368,17 +545,25 @@ struct Tiles {
   bool bad;
 };
 
-__device__ __forceinline__ Tiles find_tile(const AttentionArgs& a, const Segment& s, int key) {
+// Finding them waits for the table; the load goes out with page_of, long before.
+__device__ __forceinline__ int page_of(const AttentionArgs& a, const Segment& s, int key) {
+  int page = -1;
+  if (key < s.span.hi) page = a.table[(int64_t)s.b * a.max_pages + a.by_page.of(key)];
+  return page;
+}
+
+__device__ __forceinline__ Tiles tile_of(const AttentionArgs& a, const Segment& s, int key,
+                                         int page) {
   const int P = a.cache.page_size;
-  Tiles t{0, true};
-  if (key < s.span.hi) {
-    const int col = key / P;
-    const int page = a.table[(int64_t)s.b * a.max_pages + col];
-    t.bad = (uint32_t)page >= (uint32_t)a.cache.num_pages;
-    if (!t.bad)
-      t.index = (((int64_t)page * a.cache.kv_heads + s.g) * P + (key - col * P)) / kKvTile;
-  }
+  Tiles t;
+  t.bad = (uint32_t)page >= (uint32_t)a.cache.num_pages;
+  const int64_t first = ((int64_t)page * a.cache.kv_heads + s.g) * P;
+  t.index = t.bad ? 0 : (first + (key - (int)a.by_page.of(key) * P)) / kKvTile;
   return t;
+}
+
+__device__ __forceinline__ Tiles find_tile(const AttentionArgs& a, const Segment& s, int key) {
+  return tile_of(a, s, key, page_of(a, s, key));
 }
 
 // ---- few rows: the workgroup's waves split the keys ----
@@ -396,6 +581,55 @@ struct FewRows {
     Raw v[kTiles / 2][DB];
     f32x4 ks[kBytes<T> ? kTiles : 1], vs[kBytes<T> ? kTiles : 1];
   };
+  // What goes out for a segment before the one in front of it has been joined and written.
+  struct Ahead {
+    Loads x;
+    Tiles held;     // the tiles of this wave's first steps, a lane each
+    bool started;
+  };
+  // No loads ahead.  The registers are said to be set here, to anything: left unset, they
+  // would be reserved throughout the kernel.
+  static __device__ __forceinline__ void none_ahead(Ahead& n) {
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "=v"(n.x.k[t][kk]));
+      if constexpr (kBytes<T>) asm volatile("" : "=v"(n.x.ks[t]), "=v"(n.x.vs[t]));
+    }
+#pragma unroll
+    for (int u = 0; u < kTiles / 2; ++u)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) asm volatile("" : "=v"(n.x.v[u][db]));
+    n.held = {0, true};
+    n.started = false;
+  }
+  static constexpr int kAhead = 64 / kTiles;  // steps whose tiles the lanes hold
+
+  static __device__ __forceinline__ Tiles look_up(const AttentionArgs& a, const Segment& s,
+                                                  int lane, int from) {
+    return find_tile(a, s, key_of(lane, from));
+  }
+  // First key of the lane's tile among the tiles of a wave's steps.
+  static __device__ __forceinline__ int key_of(int lane, int from) {
+    lane = fresh(lane);
+    return from + (lane / kTiles) * 4 * kStep + (lane % kTiles) * kKvTile;
+  }
+  static __device__ __forceinline__ void take(const Tiles& held, int step, int64_t* tile) {
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) tile[t] = lane_of(held.index, step * kTiles + t);
+  }
+  static __device__ __forceinline__ int last_key(const Segment& s) {
+    return s.k1 < s.span.hi ? s.k1 : s.span.hi;
+  }
+  // The first step's loads.
+  static __device__ __forceinline__ void start(const AttentionArgs& a, const Segment& s, int lane,
+                                               int wave, Ahead& n) {
+    if (s.k0 + wave * kStep >= last_key(s)) return;
+    int64_t tile[kTiles];
+    take(n.held, 0, tile);
+    load_k(a, lane, tile, n.x);
+    load_v(a, lane, tile, n.x);
+  }
 
   static __device__ __forceinline__ u32x4 operand(Raw r) {
     if constexpr (kBytes<T>) return quants_to_f16(r);
@@ -437,47 +671,42 @@ struct FewRows {
     }
   }
 
-  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh,
-                                             uint8_t* smem) {
+  // One segment; `n` holds its first loads if n.started, and at the end those of `then`.
+  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh, uint8_t* smem,
+                                             const Segment* then, bool go_on, Ahead& n) {
     const AttentionArgs a = fresh_args();
+    forget();
     const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
     const int quad = lane >> 4;
-    const int group = a.heads / a.cache.kv_heads;
     const int row = (lane & 15) < s.rows ? lane & 15 : s.rows - 1;
-    const int token = row / group;
-    const Span mine = span_of(a, s.seq, group, row, row + 1);
+    const int token = (int)a.by_group.of(row);
+    const Span mine = span_of(a, s.seq, row, row + 1);
     const uint32_t width = mine.hi > mine.lo ? (uint32_t)(mine.hi - mine.lo) : 0;
 
     // Steps of this wave: s.k0 + (wave + 4 i) kStep.
-    const int hi = s.k1 < s.span.hi ? s.k1 : s.span.hi;
+    const int hi = last_key(s);
+    bool careful = false;
+    Loads& x = n.x;
+    Tiles& held = n.held;
+  again:
     int base = s.k0 + wave * kStep;
-    const int held_from = base;
-    constexpr int kAhead = 64 / kTiles;  // steps whose tiles the lanes hold
-    auto look_up = [&](int from) {
-      return find_tile(a, s, from + (lane / kTiles) * 4 * kStep + (lane % kTiles) * kKvTile);
-    };
-    Tiles held = look_up(base);
+    if (!n.started) {
+      held = look_up(a, s, lane, base);
+      start(a, s, lane, wave, n);
+    }
     uint64_t bad = __ballot(held.bad);
     int at = 0;  // step among the held ones
-    Loads x;
     int64_t tile[kTiles];
-    auto take = [&](int step) {
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) tile[t] = lane_of(held.index, step * kTiles + t);
-    };
-    auto start = [&] {
-      base = s.k0 + wave * kStep;
-      at = 0;
-      if (base >= hi) return;
-      take(0);
-      load_k(a, lane, tile, x);
-      load_v(a, lane, tile, x);
-    };
-    start();
+    take(held, 0, tile);
+    int then_page = 0;
+    if (go_on) {
+      const Segment t = uniform(*then);
+      then_page = page_of(a, t, key_of(lane, t.k0 + wave * kStep));
+    }
 
     // q as the right operand: element 8 (l / 16) + e of each run of 32.
     const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                     (int64_t)(s.g * group + row - token * group) * D + quad * 8;
+                     (int64_t)(s.g * a.group + row - token * a.group) * D + quad * 8;
     u32x4 qp[kParts<T>][KK];
     float c;  // logits in units of log2 are S * c
     {
@@ -510,8 +739,6 @@ struct FewRows {
 
     float m = -INFINITY, l = 0.0f;
     f32x4 acc[DB] = {};
-    bool careful = false;
-  again:
     for (; base < hi; base += 4 * kStep) {
       // The step's keys are whole for every row, or each lane's keys are checked.
       const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
@@ -531,29 +758,23 @@ struct FewRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[t][i] = r[i];
       }
-      float inv[kTiles][4];
       if constexpr (kBytes<T>)
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float lv;
-            v_scale_parts(x.vs[t][i], &lv, &inv[t][i]);
-            sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], lv);
-          }
+          for (int i = 0; i < 4; ++i)
+            sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
 
       // The next step's K goes out before the softmax.
       const bool more = base + 4 * kStep < hi;
-      int64_t tile_now[kTiles];
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) tile_now[t] = tile[t];
+      const int64_t tile_now[2] = {tile[0], tile[1]};
       if (more) {
         if (++at == kAhead) {
-          held = look_up(base + 4 * kStep);
+          held = look_up(a, s, lane, base + 4 * kStep);
           bad = __ballot(held.bad);
           at = 0;
         }
-        take(at);
+        take(held, at, tile);
         load_k(a, lane, tile, x);
       }
 
@@ -589,7 +810,7 @@ struct FewRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float p = exp2_of(__builtin_fmaf(sc[t][i], to_log2, -ref));
-          if constexpr (kBytes<T>) l = __builtin_fmaf(p, inv[t][i], l);
+          if constexpr (kBytes<T>) l = __builtin_fmaf(p, scale_inverse(x.vs[t][i]), l);
           else l += p;
           sc[t][i] = p;
         }
@@ -686,15 +907,17 @@ struct FewRows {
         for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
       if (!careful && __any(zero != zero && l - l == 0.0f)) {
         careful = true;
-        m = -INFINITY;
-        l = 0.0f;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = f32x4{};
-        held = look_up(held_from);
-        bad = __ballot(held.bad);
-        start();
+        n.started = false;
         goto again;
       }
+    }
+    // The next segment's first loads are under way while this one is joined and written.
+    n.started = go_on;
+    if (go_on) {
+      forget();
+      const Segment t = uniform(*then);
+      held = tile_of(a, t, key_of(lane, t.k0 + wave * kStep), then_page);
+      start(a, t, lane, wave, n);
     }
     l = with_32(with_16(l, sum_float), sum_float);
 
@@ -736,30 +959,50 @@ struct FewRows {
         if (tid < 16) store_part2(f32x2{M, L}, rs, tid * 8, to + kMl);
       }
       if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return;
+      // In order, some at a time: their loads are in flight together.
+      constexpr int kAtOnce = 16 / NQ;
       M = -INFINITY;
       L = 0.0f;
-#pragma unroll 4
-      for (int p = 0; p < s.parts; ++p)
-        M = fmaxf(M, load_part2(rs, r * 8, slot_at(sh, s, p) + kMl).x);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) out[i] = f32x4{};
-#pragma unroll 4
-      for (int p = 0; p < s.parts; ++p) {
-        const uint32_t from = slot_at(sh, s, p);
-        const f32x2 ml = load_part2(rs, r * 8, from + kMl);
-        const float f = weight(ml.x, M);
-        L = __builtin_fmaf(ml.y, f, L);
+      for (int p0 = 0; p0 < s.parts; p0 += kAtOnce) {
+        f32x2 ml[kAtOnce];
+        f32x4 v[kAtOnce][NQ];
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-          if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
-            out[i] += load_part(rs, tid * 16, from + i * kThreads * 16) * f;
+        for (int p = 0; p < kAtOnce; ++p) {
+          // Past the last part: that one again, with no weight.
+          const uint32_t from = slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
+          ml[p] = load_part2(rs, r * 8, from + kMl);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
+              v[p][i] = load_part(rs, tid * 16, from + i * kThreads * 16);
+        }
+        float to = M;
+#pragma unroll
+        for (int p = 0; p < kAtOnce; ++p) to = fmaxf(to, ml[p].x);
+        const float keep = weight(M, to);
+        M = to;
+        L *= keep;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) out[i] *= keep;
+#pragma unroll
+        for (int p = 0; p < kAtOnce; ++p) {
+          if (p0 + p < s.parts) {
+            const float f = weight(ml[p].x, M);
+            L = __builtin_fmaf(ml[p].y, f, L);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+              if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D) out[i] += v[p][i] * f;
+          }
+        }
       }
     }
     if (r < s.rows) {
       const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-      const int tok = r / group;
+      const int tok = (int)a.by_group.of(r);
       float* o = a.out + (int64_t)(s.seq.row0 + tok) * a.out_stride +
-                 (int64_t)(s.g * group + r - tok * group) * D;
+                 (int64_t)(s.g * a.group + r - tok * a.group) * D;
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         const int qd = tid + i * kThreads;
@@ -872,11 +1115,9 @@ struct ManyRows {
       }
       if (tid < kUnit) {
         float* sc = reinterpret_cast<float*>(smem + kScales) + buf * 3 * kUnit;
-        float lv, inv;
-        v_scale_parts(x.vs, &lv, &inv);
         sc[tid] = x.ks;
-        sc[kUnit + tid] = lv;
-        sc[2 * kUnit + tid] = inv;
+        sc[kUnit + tid] = scale_log2(x.vs);
+        sc[2 * kUnit + tid] = scale_inverse(x.vs);
       }
     }
   }
@@ -920,16 +1161,15 @@ struct ManyRows {
     const AttentionArgs a = fresh_args();
     const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
     const int half = lane >> 5;
-    const int group = a.heads / a.cache.kv_heads;
     const int wrow = wave * 32 + (lane & 31);
     const int row = s.r0 + (wrow < s.rows ? wrow : s.rows - 1);
-    const int token = row / group;
+    const int token = (int)a.by_group.of(row);
     const bool live = wave * 32 < s.rows;
-    const Span mine = span_of(a, s.seq, group, row, row + 1);
+    const Span mine = span_of(a, s.seq, row, row + 1);
     const uint32_t width = mine.hi > mine.lo ? (uint32_t)(mine.hi - mine.lo) : 0;
     // What the wave's rows see together and alone.
-    const int w0 = s.r0 + wave * 32, w1 = s.r0 + (s.rows < wave * 32 + 32 ? s.rows : wave * 32 + 32);
-    const Span ours = span_of(a, s.seq, group, live ? w0 : row, live ? w1 : row + 1);
+    const int w0 = live ? wave * 32 : 0, w1 = s.rows < w0 + 32 ? s.rows : w0 + 32;
+    const Span ours = span_of(a, s.seq, s.r0 + w0, s.r0 + w1);
 
     const int hi = s.k1 < s.span.hi ? s.k1 : s.span.hi;
     Staged staged;
@@ -949,7 +1189,7 @@ struct ManyRows {
     float c = 0.0f;
     {
       const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                       (int64_t)(s.g * group + row - token * group) * D + half * 8;
+                       (int64_t)(s.g * a.group + row - token * a.group) * D + half * 8;
       uint32_t amax = 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
@@ -1161,33 +1401,50 @@ struct ManyRows {
       }
       if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return;
       if (wrow >= s.rows) return;
+      // In order, some at a time: their loads are in flight together.
+      constexpr int kAtOnce = D <= 64 ? 4 : D <= 128 ? 2 : 1, kQuads = D / 8;
       m = -INFINITY;
       l = 0.0f;
-#pragma unroll 4
-      for (int p = 0; p < s.parts; ++p)
-        m = fmaxf(m, load_part2(rs, at * 8, slot_at(sh, s, p) + kMl).x);
 #pragma unroll
       for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
 #pragma unroll 1
-      for (int p = 0; p < s.parts; ++p) {
-        const uint32_t from = slot_at(sh, s, p);
-        const f32x2 ml = load_part2(rs, at * 8, from + kMl);
-        const float f = weight(ml.x, m);
-        l = __builtin_fmaf(ml.y, f, l);
+      for (int p0 = 0; p0 < s.parts; p0 += kAtOnce) {
+        f32x2 ml[kAtOnce];
+        f32x4 v[kAtOnce][kQuads];
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int p = 0; p < kAtOnce; ++p) {
+          // Past the last part: that one again, with no weight.
+          const uint32_t from = slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
+          ml[p] = load_part2(rs, at * 8, from + kMl);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 v = load_part(rs, at * 16, from + (db * 4 + q) * kThreads * 16) * f;
+          for (int q = 0; q < kQuads; ++q)
+            v[p][q] = load_part(rs, at * 16, from + q * kThreads * 16);
+        }
+        float to = m;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[db][4 * q + i] += v[i];
+        for (int p = 0; p < kAtOnce; ++p) to = fmaxf(to, ml[p].x);
+        const float keep = weight(m, to);
+        m = to;
+        l *= keep;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] *= keep;
+#pragma unroll
+        for (int p = 0; p < kAtOnce; ++p) {
+          if (p0 + p < s.parts) {
+            const float f = weight(ml[p].x, m);
+            l = __builtin_fmaf(ml[p].y, f, l);
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[q / 4][q % 4 * 4 + i] += v[p][q][i] * f;
           }
+        }
       }
     }
     if (wrow < s.rows) {
       const float inv = 1.0f / l;
       float* o = a.out + (int64_t)(s.seq.row0 + token) * a.out_stride +
-                 (int64_t)(s.g * group + row - token * group) * D + half * 4;
+                 (int64_t)(s.g * a.group + row - token * a.group) * D + half * 4;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -1200,62 +1457,6 @@ struct ManyRows {
   }
 };
 
-// The segment that starts with unit *u of a workgroup's run, which *u then moves past.  *b is
-// the unit's sequence or one before it, *base the units before that one.
-__device__ __forceinline__ Segment segment_of(int w, uint64_t per, uint64_t u_end, uint64_t* u,
-                                              int* b, uint64_t* base) {
-  const AttentionArgs a = fresh_args();
-  asm volatile("" : "+s"(per));  // as above: no reciprocal of it is kept
-  const int lane = fresh_tid() & 63, G = a.cache.kv_heads, group = a.heads / G;
-  Segment s;
-  uint64_t of_head;
-  for (;; ++*b) {
-    s.seq = seq_of(a, *b);
-    const int tiles = tiles_of(s.seq, group);
-    int n = 0;
-    for (int t = lane; t < tiles; t += 64) n += tile_units(a, s.seq, group, t);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) n += from_lane(n, lane ^ off);
-    of_head = (uint64_t)(uint32_t)uniform(n);
-    if (*u < *base + of_head * G) break;
-    *base = uniform(*base + of_head * G);
-  }
-  s.b = *b;
-  s.g = (int)((*u - *base) / of_head);
-  const uint64_t head_start = *base + s.g * of_head;
-  const uint32_t in_head = (uint32_t)(*u - head_start);
-  const int rows = s.seq.n * group, tr = tile_rows(rows), tiles = tiles_of(s.seq, group);
-  uint32_t tile_start = 0;  // units of the head's tiles before the one sought
-  int tile = 0, units = 0;
-  for (int t0 = 0;; t0 += 64) {
-    const int mine = t0 + lane < tiles ? tile_units(a, s.seq, group, t0 + lane) : 0;
-    const int upto = wave_scan(mine, lane);
-    const uint64_t past = __ballot((uint32_t)upto + tile_start > in_head);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      tile = t0 + at;
-      units = __builtin_amdgcn_readlane(mine, at);
-      tile_start += (uint32_t)(__builtin_amdgcn_readlane(upto, at) - units);
-      break;
-    }
-    tile_start += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
-  }
-  s.r0 = tile * tr;
-  s.rows = rows - s.r0 < tr ? rows - s.r0 : tr;
-  s.span = span_of(a, s.seq, group, s.r0, s.r0 + s.rows);
-  const uint64_t i0 = head_start + tile_start, i1 = i0 + units;
-  const uint64_t stop = u_end < i1 ? u_end : i1;
-  const int k_first = s.span.lo / kUnit * kUnit;
-  s.k0 = k_first + (int)(*u - i0) * kUnit;
-  s.k1 = k_first + (int)(stop - i0) * kUnit;
-  s.first = (int)(i0 / per);
-  s.part = w - s.first;
-  s.parts = (int)((i1 - 1) / per) - s.first + 1;
-  *u = uniform(stop);
-  *b = uniform(*b);
-  return uniform(s);
-}
-
 template <KvType T, int D>
 constexpr int kLds = ManyRows<T, D>::kLdsBytes > 4 * 16 * (D * 4 + 8)
                          ? ManyRows<T, D>::kLdsBytes : 4 * 16 * (D * 4 + 8);
@@ -1264,54 +1465,90 @@ template <KvType T, int D>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(AttentionArgs a,
                                                                                Shared sh) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[kLds<T, D>];
+  __shared__ Schedule sch;
+  // A wave's cursor and next segment, here rather than in registers that its loops need.
+  __shared__ Cursor<T> s_cursor[4];
+  __shared__ Segment s_then[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int G = a.cache.kv_heads, group = a.heads / G;
 
-  // Units of all sequences: inclusive sums over the threads, each with `chunk` sequences.
-  uint64_t* s_sum = reinterpret_cast<uint64_t*>(smem);
+  // Costs of all sequences, summed over the threads.
   const int chunk = (a.sequences + kThreads - 1) / kThreads;
   uint64_t sum = 0;
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
-    if (b >= a.sequences) break;
-    const Seq s = seq_of(a, b);
-    const int tiles = tiles_of(s, group);
-    for (int t = 0; t < tiles; ++t) sum += (uint64_t)tile_units(a, s, group, t) * G;
+    Seq s{0, 0, 0};
+    if (b < a.sequences) s = seq_of(a, b);
+    sch.seq[tid] = s;
+    const Cost c = cost_of<T>(a, s);
+    sum += c.before(c.tiles) * a.cache.kv_heads;
   }
-#pragma unroll
+#pragma unroll 1
   for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_up((unsigned long long)sum, off);
+    const uint64_t o = (uint64_t)from_lane((int64_t)sum, lane - off);
     if (lane >= off) sum += o;
   }
-  if (lane == 63) s_sum[kThreads + wave] = sum;
+  if (lane == 63) sch.wave_sum[wave] = sum;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) sum += s_sum[kThreads + w];
-  s_sum[tid] = sum;
-  __syncthreads();
-  const uint64_t total = uniform(s_sum[kThreads - 1]);
-  if (total == 0) return;
-
-  // Equal runs of units; neighbouring runs on one XCD, whose L2 they share.
-  uint64_t per = (total + gridDim.x - 1) / gridDim.x;
-  per = uniform(per < 2 ? 2 : per);
-  const int used = (int)((total + per - 1) / per);
-  const int by_xcd = (used + 7) / 8;
-  const int w = (int)(blockIdx.x % 8) * by_xcd + (int)(blockIdx.x / 8);
-  if ((int)(blockIdx.x / 8) >= by_xcd || w >= used) return;
-  uint64_t u = uniform((uint64_t)w * per);
-  const uint64_t u_end = uniform(u + per < total ? u + per : total);
-
-  const int before = __syncthreads_count(s_sum[tid] <= u);
-  int b = uniform(before * chunk);
-  uint64_t base = before > 0 ? uniform(s_sum[before - 1]) : 0;
+  for (int i = 0; i < wave; ++i) sum += sch.wave_sum[i];
+  sch.sum[tid] = sum;
   __syncthreads();
 
-  while (u < u_end) {
-    const Segment s = segment_of(w, per, u_end, &u, &b, &base);
-    if (tile_rows(s.seq.n * (a.heads / a.cache.kv_heads)) == kFewRows)
-      FewRows<T, D>::run(s, sh, smem);
-    else
+  // Runs of equal cost; neighbours on one XCD, whose L2 they share.
+  Cursor<T> cur;
+  cur.total = uniform(sch.sum[kThreads - 1]);
+  cur.k = 31 - __builtin_clz(gridDim.x);
+  while (cur.k > 0 && cur.total >> cur.k < Weights<T>::kLeast) --cur.k;
+  const int used = 1 << cur.k;
+  cur.w = blockIdx.x;
+  if (used >= 8) cur.w = (int)(blockIdx.x % 8) * (used / 8) + (int)(blockIdx.x / 8);
+  if (cur.total == 0 || (int)blockIdx.x >= used) return;
+  const uint64_t from = cur.w * cur.total >> cur.k;
+  cur.end = (cur.w + 1) * cur.total >> cur.k;
+
+  // Threads whose sequences come wholly before the run.
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads; i += 64)
+    before += __builtin_popcountll(__ballot(sch.sum[i + lane] <= from));
+  cur.locate(fresh_args(), sch, chunk, uniform(before), from);
+
+  s_cursor[wave] = cur;
+  // The next segment into s_then; false at the run's end.
+  auto next = [&] {
+    forget();
+    const AttentionArgs args = fresh_args();
+    const int mine = uniform(fresh_tid() >> 6);
+    Cursor<T> c = s_cursor[mine].uniform_copy();
+    Segment then;
+    if (!c.next(args, sch, (args.sequences + kThreads - 1) / kThreads, &then)) return false;
+    s_cursor[mine] = c;
+    s_then[mine] = then;
+    forget();
+    return true;
+  };
+  auto take = [&] {
+    forget();
+    return uniform(s_then[uniform(fresh_tid() >> 6)]);
+  };
+  auto few = [](const Segment& s) { return s.seq.n * fresh_args().group <= kFewRows; };
+  for (bool have = false;; ) {
+    if (!have && !next()) return;
+    have = false;
+    Segment s = take();
+    if (few(s)) {
+      typename FewRows<T, D>::Ahead ahead;
+      FewRows<T, D>::none_ahead(ahead);
+      for (;;) {
+        have = next();
+        const bool go_on = have && few(take());
+        FewRows<T, D>::run(s, sh, smem, &s_then[uniform(fresh_tid() >> 6)], go_on, ahead);
+        if (!go_on) break;
+        s = take();
+      }
+      if (!have) return;
+    } else {
       ManyRows<T, D>::run(s, sh, smem);
+    }
   }
 }
 
@@ -1345,9 +1582,14 @@ SplitKNeed paged_attention_workspace(int head_dim, int64_t rows) {
   return need;
 }
 
-hipError_t launch_paged_attention(const AttentionArgs& a, const SplitKWorkspace& ws,
+hipError_t launch_paged_attention(const AttentionArgs& args, const SplitKWorkspace& ws,
                                   hipStream_t stream) {
-  const int64_t rows = (int64_t)a.tokens * (a.heads / a.cache.kv_heads);
+  AttentionArgs a = args;
+  a.group = a.heads / a.cache.kv_heads;
+  a.most = a.max_pages * a.cache.page_size;
+  a.by_group = Divisor(a.group);
+  a.by_page = Divisor(a.cache.page_size);
+  const int64_t rows = (int64_t)a.tokens * a.group;
   const Shared sh{ws.partials, ws.counters, slot_floats_of(a.cache.head_dim, rows)};
   switch (a.cache.type) {
     case KvType::kF16: return launch_typed<KvType::kF16>(a, sh, stream);

@@ -65,6 +65,19 @@ struct KvWriteArgs {
 };
 hipError_t launch_paged_kv_write(const KvWriteArgs& a, hipStream_t stream);
 
+// x / d for 0 <= x < 2^31 as a product and a shift.
+struct Divisor {
+  uint32_t magic = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) {
+    while ((1u << shift) < d) ++shift;
+    magic = (uint32_t)(((uint64_t(1) << (31 + shift)) + d - 1) / d);
+  }
+  __host__ __device__ uint32_t of(uint32_t x) const {
+    return (uint32_t)((uint64_t)x * magic >> 31) >> shift;
+  }
+};
+
 struct AttentionArgs {
   PagedCache cache;
   const float* q;
@@ -79,6 +92,10 @@ struct AttentionArgs {
   const int32_t* cu;
   int sequences;
   int tokens;
+  // Set by the launcher: heads of a KV head, keys of a table row.
+  int group;
+  int most;
+  Divisor by_group, by_page;
 };
 // Workspace of a call with `rows` rows of one KV head (new tokens * heads / kv_heads).
 SplitKNeed paged_attention_workspace(int head_dim, int64_t rows);
