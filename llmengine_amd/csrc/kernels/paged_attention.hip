@@ -16,10 +16,9 @@
 // bits where the row's contributions are; l gets p_j vs_j * (1 / vs_j).
 //
 // A value of V that is not finite must reach the rows that see it and no others, and 0 times
-// it, or the parts of P times it, are NaN.  Where rows of a tile do not all see a key, such
-// values are taken out of the product and added to the rows that see them; where the
-// product of keys that all rows see comes out non-finite, the keys are gone through again
-// that way.
+// it, or the parts of P times it, are NaN.  Where a sum comes out non-finite, the keys are gone
+// through again, with such values taken out of the product and added to the rows that see
+// them.  Places that no row sees, which may hold anything, always count as zero.
 //
 // The maximum moves only when a logit passes it by 2^8 (P and l stay far from their limits),
 // so that the rescaling of O is rare.
@@ -266,6 +265,8 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, const Seq& s, in
 struct Cost {
   int tiles;
   int first, slope, cap;
+  int fixed;  // of a tile's cost, what is not its units
+  int least;  // the least piece of a tile worth a workgroup of its own
 
   __device__ __forceinline__ int of(int t) const {
     const int64_t v = (int64_t)first + (int64_t)t * slope;
@@ -281,16 +282,16 @@ struct Cost {
   }
 };
 
-// Cost of a unit of many and of few rows, of a tile besides its units, and the least piece of
-// a tile worth a workgroup of its own: 64 keys of 128 rows take about 3.5 us beside another
-// workgroup (half as much again with three parts), of few rows 2 to 4; a tile's beginning and
-// end about three units.
+// Cost of a unit of many and of few rows, and of a tile besides its units: beside another
+// workgroup, 64 keys of 128 rows take 3.5 us (5.6 with three parts) and of few rows 1.2
+// (0.9 of 8 bits), 3 where all of them wait for memory; a tile's beginning and end 8 us.
 template <KvType T>
 struct Weights {
   static constexpr int kMany = kParts<T> * 16;
-  static constexpr int kFew = kBytes<T> ? 16 : 24;
-  static constexpr int kTile = 64;
-  static constexpr int kLeast = 64;
+  static constexpr int kFew = kBytes<T> ? 8 : 11;
+  static constexpr int kTileMany = 80, kTileFew = 40;
+  // The least piece of a tile worth a workgroup of its own.
+  static constexpr int kLeastMany = kTileMany + kMany, kLeastFew = kTileFew + 20;
 };
 
 template <KvType T>
@@ -299,8 +300,9 @@ __device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Seq& s) {
   const int rows = s.n * a.group;
   const bool few = rows <= kFewRows;
   const int unit = few ? Weights<T>::kFew : Weights<T>::kMany;
+  const int fixed = few ? Weights<T>::kTileFew : Weights<T>::kTileMany;
   auto units = [&](int64_t keys) {  // at least a partial one
-    const int64_t v = (keys > 0 ? (keys * unit) / kUnit : 0) + unit / 2 + Weights<T>::kTile;
+    const int64_t v = (keys > 0 ? (keys * unit) / kUnit : 0) + unit / 2 + fixed;
     return (int)(v < kMax ? v : kMax);
   };
   Cost c;
@@ -309,6 +311,8 @@ __device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Seq& s) {
   c.cap = a.window > 0 ? units((int64_t)a.window + tokens) : kMax;
   c.first = units((int64_t)s.pos0 + tokens);
   c.slope = (int)a.by_group.of(2 * Weights<T>::kMany);  // kTileRows / group keys
+  c.fixed = fixed;
+  c.least = few ? Weights<T>::kLeastFew : Weights<T>::kLeastMany;
   return c;
 }
 
@@ -358,8 +362,8 @@ struct Schedule {
 };
 
 // A workgroup's way through its run of the work.  The whole work, `total`, is cut at
-// w total / 2^k; a cut within kLeast of a tile's begin or end moves there, so that no tile is
-// split for less.
+// w total / 2^k; a cut that leaves less than cost.least of a tile before or behind it moves to
+// the tile's begin or end.
 template <KvType T>
 struct Cursor {
   int b, g, t;
@@ -421,21 +425,21 @@ struct Cursor {
     i1 = i0 + cost.of(t);
     done = false;
     begin = i0;
-    if (at - i0 >= Weights<T>::kLeast) {
+    if (at - i0 >= (uint64_t)cost.least) {
       begin = at;
-      if (i1 - at < Weights<T>::kLeast) {
+      if (i1 - at < (uint64_t)cost.least) {
         if (i1 < total) advance(a, sch, chunk);
         else done = true;
       }
     }
   }
 
-  // Units of the tile that lie before place x of it.
-  static __device__ __forceinline__ int units_at(uint64_t x, uint64_t of, int units) {
+  // Units of the tile that lie before place x of it; its fixed cost comes first.
+  __device__ __forceinline__ int units_at(uint64_t x, uint64_t of, int units) const {
     if (x >= of) return units;
-    const int u = (int)((float)(uint32_t)x *
-                        ((float)units * __builtin_amdgcn_rcpf((float)(uint32_t)of)));
-    return u < units ? u : units;
+    const float u = ((float)(uint32_t)x - (float)cost.fixed) *
+                    ((float)units * __builtin_amdgcn_rcpf((float)((uint32_t)of - cost.fixed)));
+    return u <= 0.0f ? 0 : u < (float)units ? (int)u : units;
   }
 
   __device__ __forceinline__ Cursor uniform_copy() const {
@@ -444,7 +448,8 @@ struct Cursor {
     c.g = uniform(g);
     c.t = uniform(t);
     c.seq = {uniform(seq.row0), uniform(seq.n), uniform(seq.pos0)};
-    c.cost = {uniform(cost.tiles), uniform(cost.first), uniform(cost.slope), uniform(cost.cap)};
+    c.cost = {uniform(cost.tiles), uniform(cost.first), uniform(cost.slope), uniform(cost.cap),
+              uniform(cost.fixed), uniform(cost.least)};
     c.i0 = uniform(i0);
     c.i1 = uniform(i1);
     c.begin = uniform(begin);
@@ -459,8 +464,8 @@ struct Cursor {
   // The next piece of this workgroup's run; false at its end.
   __device__ __forceinline__ bool next(const AttentionArgs& a, const Schedule& sch, int chunk,
                                        Segment* out) {
-    if (done || (int64_t)(end - i0) < Weights<T>::kLeast) return false;
-    const uint64_t stop = (int64_t)(i1 - end) < Weights<T>::kLeast ? i1 : end;
+    if (done || end <= i0 || (end < i1 && end - i0 < (uint64_t)cost.least)) return false;
+    const uint64_t stop = (int64_t)(i1 - end) < cost.least ? i1 : end;
     Segment s;
     s.b = b;
     s.g = g;
@@ -477,7 +482,7 @@ struct Cursor {
     s.part = s.first = 0;
     if (begin != i0 || stop != i1) {
       // The cuts inside the tile.
-      const uint64_t lo = i0 + Weights<T>::kLeast, hi = i1 - Weights<T>::kLeast;
+      const uint64_t lo = i0 + cost.least, hi = i1 - cost.least;
       const int c0 = (int)quotient((lo << k) + total - 1, total);
       const int c1 = (int)quotient(((hi + 1) << k) - 1, total);
       s.first = c0 - 1;
@@ -671,9 +676,11 @@ struct FewRows {
     }
   }
 
-  // One segment; `n` holds its first loads if n.started, and at the end those of `then`.
-  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh, uint8_t* smem,
-                                             const Segment* then, bool go_on, Ahead& n) {
+  // One segment; `n` holds its first loads if n.started.  find_next() puts the next one into
+  // `then`; if that is of few rows too, it comes next (true) and `n` gets its first loads.
+  template <class F>
+  static __device__ __forceinline__ bool run(const Segment& s, const Shared& sh, uint8_t* smem,
+                                             const Segment* then, F find_next, Ahead& n) {
     const AttentionArgs a = fresh_args();
     forget();
     const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
@@ -685,10 +692,19 @@ struct FewRows {
 
     // Steps of this wave: s.k0 + (wave + 4 i) kStep.
     const int hi = last_key(s);
-    bool careful = false;
+    bool careful = false, go_on = false;
     Loads& x = n.x;
     Tiles& held = n.held;
   again:
+    // Ahead of the first keys, which wait for the table.
+    const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                     (int64_t)(s.g * a.group + row - token * a.group) * D + quad * 8;
+    f32x4 qv[KK][2];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        qv[kk][h] = *reinterpret_cast<const f32x4*>(q + kk * 32 + h * 4);
     int base = s.k0 + wave * kStep;
     if (!n.started) {
       held = look_up(a, s, lane, base);
@@ -699,27 +715,21 @@ struct FewRows {
     int64_t tile[kTiles];
     take(held, 0, tile);
     int then_page = 0;
+    if (!careful) go_on = find_next();
     if (go_on) {
       const Segment t = uniform(*then);
       then_page = page_of(a, t, key_of(lane, t.k0 + wave * kStep));
     }
 
     // q as the right operand: element 8 (l / 16) + e of each run of 32.
-    const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                     (int64_t)(s.g * a.group + row - token * a.group) * D + quad * 8;
     u32x4 qp[kParts<T>][KK];
     float c;  // logits in units of log2 are S * c
     {
-      f32x4 v[KK][2];
       uint32_t amax = 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          v[kk][h] = *reinterpret_cast<const f32x4*>(q + kk * 32 + h * 4);
-          const uint32_t m = magnitude(v[kk][h]);
-          amax = m > amax ? m : amax;
-        }
+        for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(with_16(amax, max_bits), max_bits);
       float up, down;
       row_scale(amax, &up, &down);
@@ -730,7 +740,7 @@ struct FewRows {
         uint32_t w[kParts<T>][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          split2<T>(v[kk][i >> 1][(i & 1) * 2] * up, v[kk][i >> 1][(i & 1) * 2 + 1] * up,
+          split2<T>(qv[kk][i >> 1][(i & 1) * 2] * up, qv[kk][i >> 1][(i & 1) * 2 + 1] * up,
                     &w[0][i], 4);
 #pragma unroll
         for (int p = 0; p < kParts<T>; ++p) qp[p][kk] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
@@ -742,8 +752,7 @@ struct FewRows {
     for (; base < hi; base += 4 * kStep) {
       // The step's keys are whole for every row, or each lane's keys are checked.
       const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
-      const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0 &&
-                         !careful;
+      const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0;
 
       float sc[kTiles][4];
 #pragma unroll
@@ -817,31 +826,28 @@ struct FewRows {
 
       bool odd = false;  // a value of V that is not finite
       if constexpr (!kBytes<T>) {
-        if (!whole) {
+        if (careful || base < s.span.lo || base + kStep > s.span.hi || bad_now != 0) {
           // Values that no row sees count as zero.
           const int from = fresh(base + (lane >> 4 & 1) * 4);
+          uint32_t found = 0;
 #pragma unroll
           for (int u = 0; u < kTiles / 2; ++u) {
             const int t = 2 * u + (lane >> 5);
-            uint32_t keep[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const int key = from + t * kKvTile + (w >> 1) * 8 + (w & 1) * 2;
               const bool tile_ok = !(bad_now >> t & 1);
-              keep[w] = (tile_ok && key >= s.span.lo && key < s.span.hi ? 0x0000ffffu : 0u) |
-                        (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
-            }
-            uint32_t found = 0;
+              const uint32_t keep =
+                  (tile_ok && key >= s.span.lo && key < s.span.hi ? 0x0000ffffu : 0u) |
+                  (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                x.v[u][db][w] &= keep[w];
+              for (int db = 0; db < DB; ++db) {
+                x.v[u][db][w] &= keep;
                 found |= non_finite<T>(x.v[u][db][w]);
               }
-            odd = odd || found != 0;
+            }
           }
-          odd = __any(odd);
+          odd = careful && __any(found != 0);
           if (odd)
 #pragma unroll
             for (int u = 0; u < kTiles / 2; ++u)
@@ -958,7 +964,7 @@ struct FewRows {
             store_part(out[i], rs, tid * 16, to + i * kThreads * 16);
         if (tid < 16) store_part2(f32x2{M, L}, rs, tid * 8, to + kMl);
       }
-      if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return;
+      if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return go_on;
       // In order, some at a time: their loads are in flight together.
       constexpr int kAtOnce = 16 / NQ;
       M = -INFINITY;
@@ -1010,6 +1016,7 @@ struct FewRows {
           *reinterpret_cast<f32x4*>(o + qd / 16 * 4) = L != 0.0f ? out[i] * inv : f32x4{};
       }
     }
+    return go_on;
   }
 };
 
@@ -1122,11 +1129,10 @@ struct ManyRows {
     }
   }
 
-  // A unit that some row does not see whole: V's places that no row sees become zero, and so
-  // do values that are not finite, which the caller adds to the rows that see them.  Returns
-  // whether there were any.
+  // V's places that no row sees become zero; where asked for, so do values that are not
+  // finite, which the caller adds to the rows that see them.  Returns whether there were any.
   static __device__ __forceinline__ bool clear_v(const Segment& s, int tid, int base,
-                                                 uint32_t bad, uint8_t* stage) {
+                                                 uint32_t bad, bool careful, uint8_t* stage) {
     bool found = false;
     if constexpr (!kBytes<T>) {
       tid = fresh(tid);
@@ -1145,7 +1151,7 @@ struct ManyRows {
                   (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
           odd |= non_finite<T>(v[w]);
         }
-        if (odd != 0) {
+        if (careful && odd != 0) {
           found = true;
 #pragma unroll
           for (int w = 0; w < 4; ++w) v[w] &= ~((non_finite<T>(v[w]) >> 15) * 0xffffu);
@@ -1181,6 +1187,15 @@ struct ManyRows {
       bad = __ballot(held.bad);
       at = 0;
     };
+    // q ahead of the first keys, which wait for the table.
+    const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                     (int64_t)(s.g * a.group + row - token * a.group) * D + half * 8;
+    f32x4 qv[KK][2];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        qv[kk][h] = *reinterpret_cast<const f32x4*>(q + kk * 16 + h * 4);
     look_up(s.k0);
     __syncthreads();  // the memory's earlier readers
     if (s.k0 < hi) issue(a, tid, held.index, 0, smem, staged);
@@ -1188,16 +1203,11 @@ struct ManyRows {
     u32x4 qp[kParts<T>][KK];
     float c = 0.0f;
     {
-      const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                       (int64_t)(s.g * a.group + row - token * a.group) * D + half * 8;
       uint32_t amax = 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t m = magnitude(*reinterpret_cast<const f32x4*>(q + kk * 16 + h * 4));
-          amax = m > amax ? m : amax;
-        }
+        for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(amax, max_bits);
       float up, down;
       row_scale(amax, &up, &down);
@@ -1208,7 +1218,7 @@ struct ManyRows {
         uint32_t w[kParts<T>][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(q + kk * 16 + h * 4);
+          const f32x4 v = qv[kk][h];
           split2<T>(v.x * up, v.y * up, &w[0][2 * h], 4);
           split2<T>(v.z * up, v.w * up, &w[0][2 * h + 1], 4);
         }
@@ -1256,9 +1266,8 @@ struct ManyRows {
         issue(a, tid, held.index, at * kTilesUnit, smem + (buf ^ 1) * kStage, staged);
       }
       bool odd = false;
-      if (!kBytes<T> && (careful || base < s.span.lo_all || base + kUnit > s.span.hi_all ||
-                         bad_now != 0))
-        odd = any_of(clear_v(s, tid, base, bad_now, stage), wave, smem + kFlags);
+      if (!kBytes<T> && (careful || base < s.span.lo || base + kUnit > s.span.hi || bad_now != 0))
+        odd = any_of(clear_v(s, tid, base, bad_now, careful, stage), wave, smem + kFlags);
 
       if (live && base < ours.hi && base + kUnit > ours.lo) {
         const bool whole = base >= ours.lo_all && base + kUnit <= ours.hi_all && bad_now == 0;
@@ -1497,7 +1506,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   Cursor<T> cur;
   cur.total = uniform(sch.sum[kThreads - 1]);
   cur.k = 31 - __builtin_clz(gridDim.x);
-  while (cur.k > 0 && cur.total >> cur.k < Weights<T>::kLeast) --cur.k;
+  while (cur.k > 0 && cur.total >> cur.k < Weights<T>::kLeastFew) --cur.k;
   const int used = 1 << cur.k;
   cur.w = blockIdx.x;
   if (used >= 8) cur.w = (int)(blockIdx.x % 8) * (used / 8) + (int)(blockIdx.x / 8);
@@ -1539,9 +1548,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
       typename FewRows<T, D>::Ahead ahead;
       FewRows<T, D>::none_ahead(ahead);
       for (;;) {
-        have = next();
-        const bool go_on = have && few(take());
-        FewRows<T, D>::run(s, sh, smem, &s_then[uniform(fresh_tid() >> 6)], go_on, ahead);
+        const bool go_on = FewRows<T, D>::run(
+            s, sh, smem, &s_then[uniform(fresh_tid() >> 6)],
+            [&] {
+              have = next();
+              return have && few(take());
+            },
+            ahead);
         if (!go_on) break;
         s = take();
       }
