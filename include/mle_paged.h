@@ -71,9 +71,9 @@ typedef struct mle_paged_cache {
  *   2. The pages that a request needs past the ones it has are popped from the top,
  *      requests in order, and written to its row of block_table.  A request whose pages
  *      are not there (the pages asked for up to and including it are more than the
- *      stack holds), that would outgrow max_pages or whose rows pass `tokens` is refused
- *      and its table row left as it is; requests that need no page are never short of
- *      one.
+ *      stack holds), that would outgrow max_pages or 2^31 - 1 tokens or whose rows pass
+ *      `tokens` is refused and its table row left as it is; requests that need no page
+ *      are never short of one.
  *   3. kv_lens[b] = cached + new (refused or finished: 0).  cu_tokens[sequences + 1] =
  *      the first row of each request among the step's rows: prefix sums of the
  *      requested new tokens, refused requests included, at most `tokens`.
@@ -82,7 +82,10 @@ typedef struct mle_paged_cache {
  *      sequence, slots[r] = page * page_size + offset; 0 and -1 where the request was
  *      refused and for rows that no request has.
  * A page number outside [0, num_pages) in table or stack gives slot -1.  Deterministic;
- * with free_count_out apart from free_count a repeated call gives the same again.
+ * with free_count_out apart from free_count a repeated call gives the same again.  But
+ * for those two no output may overlap another array.  A plan of more than 1024 rows takes
+ * a counter of the per-stream workspace (before a graph is captured: 256 bytes and 32
+ * counters, or what mle_paged_attention_workspace_size says for as many rows).
  * Errors: NULL pointers, sequences or sizes <= 0, tokens < 0 -> InvalidArgument;
  * sequences * max_pages or num_pages * page_size above 2^31 - 1 -> Unsupported.
  * tokens == 0: positions and slots may be NULL.

@@ -1246,8 +1246,11 @@ int mle_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int sequ
   const mle::PlanArgs a{cached_lens, new_lens,   sequences,  block_table,    max_pages,
                         page_size,   num_pages,  free_pages, free_count,     free_count_out,
                         tokens,      kv_lens,    cu_tokens,  positions,      slots,
-                        granted};
-  return check_launch(mle::launch_paged_plan(a, stream), "hip paged_plan launch failed");
+                        granted,     {}};
+  mle::SplitKWorkspace ws;
+  std::unique_lock<std::mutex> hold;
+  MLE_TRY(get_workspace(mle::paged_plan_workspace(tokens, sequences), stream, &ws, &hold));
+  return check_launch(mle::launch_paged_plan(a, ws, stream), "hip paged_plan launch failed");
 }
 
 int mle_rope_table(float* table, int positions, int rope_dim, double theta,

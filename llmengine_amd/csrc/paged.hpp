@@ -24,6 +24,19 @@ struct PagedCache {
   int head_dim;
 };
 
+// x / d for 0 <= x < 2^31 as a product and a shift.
+struct Divisor {
+  uint32_t magic = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) {
+    while ((1u << shift) < d) ++shift;
+    magic = (uint32_t)(((uint64_t(1) << (31 + shift)) + d - 1) / d);
+  }
+  __host__ __device__ uint32_t of(uint32_t x) const {
+    return (uint32_t)((uint64_t)x * magic >> 31) >> shift;
+  }
+};
+
 struct PlanArgs {
   const int32_t* cached;
   const int32_t* fresh;  // new tokens, or negative: finished
@@ -41,8 +54,11 @@ struct PlanArgs {
   int32_t* positions;
   int32_t* slots;
   int32_t* granted;
+  Divisor by_page;  // set by the launcher
 };
-hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream);
+// Many rows take a counter of the workspace.
+SplitKNeed paged_plan_workspace(int tokens, int sequences);
+hipError_t launch_paged_plan(const PlanArgs& a, const SplitKWorkspace& ws, hipStream_t stream);
 
 hipError_t launch_rope_table(float* table, int positions, int rope_dim, double theta,
                              const float* freq_factors, hipStream_t stream);
@@ -64,19 +80,6 @@ struct KvWriteArgs {
   int tokens;
 };
 hipError_t launch_paged_kv_write(const KvWriteArgs& a, hipStream_t stream);
-
-// x / d for 0 <= x < 2^31 as a product and a shift.
-struct Divisor {
-  uint32_t magic = 0, shift = 0;
-  Divisor() = default;
-  explicit Divisor(uint32_t d) {
-    while ((1u << shift) < d) ++shift;
-    magic = (uint32_t)(((uint64_t(1) << (31 + shift)) + d - 1) / d);
-  }
-  __host__ __device__ uint32_t of(uint32_t x) const {
-    return (uint32_t)((uint64_t)x * magic >> 31) >> shift;
-  }
-};
 
 struct AttentionArgs {
   PagedCache cache;
