@@ -113,13 +113,14 @@ __device__ __forceinline__ void put1(void* base, int64_t at, uint32_t c) {
 template <KvType T, int LPR>
 __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const int G = a.cache.kv_heads, D = a.cache.head_dim, P = a.cache.page_size;
-  const int per_row = a.heads + 2 * G;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  // The first workgroups take k and v, head by head, the others q, token by token.
+  const bool is_q = blockIdx.x >= a.kv_blocks;
+  const uint32_t item = ((blockIdx.x - (is_q ? a.kv_blocks : 0)) * 256 + threadIdx.x) / LPR;
   const int s = threadIdx.x % LPR;
   // A group's lanes share `item`, and no path below parts them across an exchange.
-  if (item >= (int64_t)a.tokens * per_row) return;
-  const int t = (int)(item / per_row);
-  const int h = (int)(item - (int64_t)t * per_row);
+  if (item >= (uint32_t)a.tokens * (uint32_t)(is_q ? a.heads : 2 * G)) return;
+  const int t = (int)(is_q ? item / (uint32_t)a.heads : item % (uint32_t)a.tokens);
+  const int h = (int)(is_q ? item % (uint32_t)a.heads : item / (uint32_t)a.tokens);
   const bool live = s * 8 < D;
   const bool halves = a.rope_halves != 0;
   int pos = 0;
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const float* rope_row = a.rope + (int64_t)pos * a.rope_dim;
   const bool turns = a.rope != nullptr && placed && s * 8 < a.rope_dim;
 
-  if (h < a.heads) {  // q
+  if (is_q) {
     if (!live) return;
     const Span sp = span_of(s, a.rope_dim, halves);
     Row8 r = load8(a.q + t * a.q_stride + (int64_t)h * D, sp);
@@ -148,8 +149,8 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   if (!placed || slot < 0 || slot >= cells) return;
   const int page = slot / P, off = slot - page * P, row = off % kKvTile;
 
-  if (h < a.heads + G) {  // K
-    const int g = h - a.heads;
+  if (h < G) {  // K
+    const int g = h;
     const Span sp = span_of(s, a.rope_dim, halves);
     Row8 r = {};
     if (live) r = load8(a.k + t * a.k_stride + (int64_t)g * D, sp);
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   }
 
   // V: does this row's place of four tokens lie whole in four rows of the step?
-  const int g = h - a.heads - G;
+  const int g = h - G;
   const int quad = off % 4, first = t - quad;
   bool whole = first >= 0 && first + 4 <= a.tokens;
   if (whole)
@@ -219,16 +220,20 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
 template <KvType T>
 hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
   const int lpr = a.cache.head_dim <= 64 ? 8 : a.cache.head_dim <= 128 ? 16 : 32;
-  const int64_t threads = (int64_t)a.tokens * (a.heads + 2 * a.cache.kv_heads) * lpr;
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  auto blocks_of = [&](int64_t rows) { return (a.tokens * rows * lpr + 255) / 256; };
+  KvWriteArgs b = a;
+  const int64_t kv_blocks = blocks_of(2 * a.cache.kv_heads);
+  const int64_t blocks = kv_blocks + blocks_of(a.heads);
+  // Rows of heads are counted in 32 bits.
+  if (blocks > (int64_t(1) << 27)) return hipErrorInvalidValue;
+  b.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((unsigned)blocks), block(256);
   if (lpr == 8)
-    hipLaunchKernelGGL((paged_kv_write_kernel<T, 8>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_kv_write_kernel<T, 8>), grid, block, 0, stream, b);
   else if (lpr == 16)
-    hipLaunchKernelGGL((paged_kv_write_kernel<T, 16>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_kv_write_kernel<T, 16>), grid, block, 0, stream, b);
   else
-    hipLaunchKernelGGL((paged_kv_write_kernel<T, 32>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_kv_write_kernel<T, 32>), grid, block, 0, stream, b);
   return hipGetLastError();
 }
 

@@ -78,6 +78,7 @@ struct KvWriteArgs {
   int rope_dim;
   int rope_halves;
   int tokens;
+  uint32_t kv_blocks;  // set by the launcher
 };
 hipError_t launch_paged_kv_write(const KvWriteArgs& a, hipStream_t stream);
 
