@@ -109,6 +109,9 @@ __device__ __forceinline__ void put1(void* base, int64_t at, uint32_t c) {
   else static_cast<uint16_t*>(base)[at] = (uint16_t)c;
 }
 
+// Heads of q that a group of lanes takes: their loads are in flight together.
+constexpr int kQHeads = 2;
+
 // LPR lanes (a power of two, at least head_dim / 8) take one head's row of one token.
 template <KvType T, int LPR>
 __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
@@ -118,9 +121,10 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const uint32_t item = ((blockIdx.x - (is_q ? a.kv_blocks : 0)) * 256 + threadIdx.x) / LPR;
   const int s = threadIdx.x % LPR;
   // A group's lanes share `item`, and no path below parts them across an exchange.
-  if (item >= (uint32_t)a.tokens * (uint32_t)(is_q ? a.heads : 2 * G)) return;
-  const int t = (int)(is_q ? item / (uint32_t)a.heads : item % (uint32_t)a.tokens);
-  const int h = (int)(is_q ? item % (uint32_t)a.heads : item / (uint32_t)a.tokens);
+  const uint32_t q_items = (uint32_t)(a.heads + kQHeads - 1) / kQHeads;  // of a token
+  if (item >= (uint32_t)a.tokens * (is_q ? q_items : 2 * G)) return;
+  const int t = (int)(is_q ? item / q_items : item % (uint32_t)a.tokens);
+  const int h = (int)(is_q ? item % q_items : item / (uint32_t)a.tokens);
   const bool live = s * 8 < D;
   const bool halves = a.rope_halves != 0;
   int pos = 0;
@@ -135,12 +139,24 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   if (is_q) {
     if (!live) return;
     const Span sp = span_of(s, a.rope_dim, halves);
-    Row8 r = load8(a.q + t * a.q_stride + (int64_t)h * D, sp);
-    if (turns) rotate8(r, rope_row, s, halves);
-    if (!placed) r = {};
-    float* o = a.q_out + t * a.q_out_stride + (int64_t)h * D;
-    *reinterpret_cast<f32x4*>(o + sp.a) = f32x4{r.x[0], r.x[1], r.x[2], r.x[3]};
-    *reinterpret_cast<f32x4*>(o + sp.b) = f32x4{r.x[4], r.x[5], r.x[6], r.x[7]};
+    const float* q = a.q + t * a.q_stride + (int64_t)h * kQHeads * D;
+    float* o = a.q_out + t * a.q_out_stride + (int64_t)h * kQHeads * D;
+    const int n = a.heads - h * kQHeads;  // heads from here on
+    Row8 r[kQHeads];
+#pragma unroll
+    for (int i = 0; i < kQHeads; ++i)
+      if (i < n) r[i] = load8(q + i * D, sp);
+#pragma unroll
+    for (int i = 0; i < kQHeads; ++i) {
+      if (i >= n) continue;
+      if (turns) rotate8(r[i], rope_row, s, halves);
+      if (!placed) r[i] = {};
+      float* to = o + i * D;
+      *reinterpret_cast<f32x4*>(to + sp.a) =
+          f32x4{r[i].x[0], r[i].x[1], r[i].x[2], r[i].x[3]};
+      *reinterpret_cast<f32x4*>(to + sp.b) =
+          f32x4{r[i].x[4], r[i].x[5], r[i].x[6], r[i].x[7]};
+    }
     return;
   }
 
@@ -223,9 +239,9 @@ hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
   auto blocks_of = [&](int64_t rows) { return (a.tokens * rows * lpr + 255) / 256; };
   KvWriteArgs b = a;
   const int64_t kv_blocks = blocks_of(2 * a.cache.kv_heads);
-  const int64_t blocks = kv_blocks + blocks_of(a.heads);
+  const int64_t blocks = kv_blocks + blocks_of((a.heads + kQHeads - 1) / kQHeads);
   // Rows of heads are counted in 32 bits.
-  if (blocks > (int64_t(1) << 27)) return hipErrorInvalidValue;
+  if (blocks > (int64_t(1) << 26)) return hipErrorInvalidValue;
   b.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((unsigned)blocks), block(256);
   if (lpr == 8)
