@@ -316,11 +316,13 @@ __device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Seq& s) {
   return c;
 }
 
-// floor(x / d) for quotients below 2^31.
-__device__ __forceinline__ uint32_t quotient(uint64_t x, uint64_t d) {
-  uint32_t q = (uint32_t)((double)x * __builtin_amdgcn_rcp((double)d));
-  while ((uint64_t)q * d > x) --q;
-  while ((uint64_t)(q + 1) * d <= x) ++q;
+// floor(x / d).
+__device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t d) {
+  double r = __builtin_amdgcn_rcp((double)d);
+  r = __builtin_fma(r, __builtin_fma(-(double)d, r, 1.0), r);
+  uint64_t q = (uint64_t)((double)x * r);
+  while (q * d > x) --q;
+  while ((q + 1) * d <= x) ++q;
   return q;
 }
 
@@ -359,10 +361,11 @@ struct Schedule {
   uint64_t sum[kThreads];  // of the costs up to and with the thread's
   Seq seq[kThreads];       // where chunk is 1
   uint64_t wave_sum[4];
+  int wave_tiles[4];
 };
 
 // A workgroup's way through its run of the work.  The whole work, `total`, is cut at
-// w total / 2^k; a cut that leaves less than cost.least of a tile before or behind it moves to
+// multiples of `run`; a cut that leaves less than cost.least of a tile before or behind it moves to
 // the tile's begin or end.
 template <KvType T>
 struct Cursor {
@@ -371,8 +374,8 @@ struct Cursor {
   Cost cost;
   uint64_t i0, i1;         // the current tile's place in the work
   uint64_t begin;          // where this workgroup takes it up
-  uint64_t end, total;
-  int w, k;
+  uint64_t end, total, run;
+  int w;
   bool done;
 
   // The sequence `b` or the first one after it that has rows; skips *base over the others.
@@ -456,7 +459,7 @@ struct Cursor {
     c.end = uniform(end);
     c.total = uniform(total);
     c.w = uniform(w);
-    c.k = uniform(k);
+    c.run = uniform(run);
     c.done = uniform((int)done) != 0;
     return c;
   }
@@ -483,8 +486,7 @@ struct Cursor {
     if (begin != i0 || stop != i1) {
       // The cuts inside the tile.
       const uint64_t lo = i0 + cost.least, hi = i1 - cost.least;
-      const int c0 = (int)quotient((lo << k) + total - 1, total);
-      const int c1 = (int)quotient(((hi + 1) << k) - 1, total);
+      const int c0 = (int)quotient(lo + run - 1, run), c1 = (int)quotient(hi, run);
       s.first = c0 - 1;
       s.part = w - s.first;
       s.parts = c1 - c0 + 2;
@@ -1483,6 +1485,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   // Costs of all sequences, summed over the threads.
   const int chunk = (a.sequences + kThreads - 1) / kThreads;
   uint64_t sum = 0;
+  int tiles = 0;
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
     Seq s{0, 0, 0};
@@ -1490,13 +1493,22 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     sch.seq[tid] = s;
     const Cost c = cost_of<T>(a, s);
     sum += c.before(c.tiles) * a.cache.kv_heads;
+    tiles += c.tiles * a.cache.kv_heads < kThreads ? c.tiles * a.cache.kv_heads : kThreads;
   }
+  tiles = tiles < (1 << 20) ? tiles : 1 << 20;
 #pragma unroll 1
   for (int off = 1; off < 64; off <<= 1) {
     const uint64_t o = (uint64_t)from_lane((int64_t)sum, lane - off);
-    if (lane >= off) sum += o;
+    const int n = from_lane(tiles, lane - off);
+    if (lane >= off) {
+      sum += o;
+      tiles += n;
+    }
   }
-  if (lane == 63) sch.wave_sum[wave] = sum;
+  if (lane == 63) {
+    sch.wave_sum[wave] = sum;
+    sch.wave_tiles[wave] = tiles;
+  }
   __syncthreads();
   for (int i = 0; i < wave; ++i) sum += sch.wave_sum[i];
   sch.sum[tid] = sum;
@@ -1505,14 +1517,18 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   // Runs of equal cost; neighbours on one XCD, whose L2 they share.
   Cursor<T> cur;
   cur.total = uniform(sch.sum[kThreads - 1]);
-  cur.k = 31 - __builtin_clz(gridDim.x);
-  while (cur.k > 0 && cur.total >> cur.k < Weights<T>::kLeastFew) --cur.k;
-  const int used = 1 << cur.k;
-  cur.w = blockIdx.x;
-  if (used >= 8) cur.w = (int)(blockIdx.x % 8) * (used / 8) + (int)(blockIdx.x / 8);
-  if (cur.total == 0 || (int)blockIdx.x >= used) return;
-  const uint64_t from = cur.w * cur.total >> cur.k;
-  cur.end = (cur.w + 1) * cur.total >> cur.k;
+  if (cur.total == 0) return;
+  // One for each tile, or each least piece of the work if that is more, in eights.
+  tiles = sch.wave_tiles[0] + sch.wave_tiles[1] + sch.wave_tiles[2] + sch.wave_tiles[3];
+  const uint64_t pieces = cur.total / Weights<T>::kLeastFew;
+  uint64_t used = (uint64_t)tiles > pieces ? (uint64_t)tiles : pieces;
+  used = used < gridDim.x ? (used + 7) / 8 * 8 : gridDim.x;
+  if (blockIdx.x >= used) return;
+  cur.run = uniform(quotient(cur.total + used - 1, used));
+  cur.w = (int)(blockIdx.x % 8) * (int)(used / 8) + (int)(blockIdx.x / 8);
+  const uint64_t from = cur.w * cur.run;
+  if (from >= cur.total) return;
+  cur.end = from + cur.run < cur.total ? from + cur.run : cur.total;
 
   // Threads whose sequences come wholly before the run.
   int before = 0;
