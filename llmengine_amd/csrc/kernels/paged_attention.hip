@@ -678,6 +678,91 @@ struct FewRows {
     }
   }
 
+  static __device__ __forceinline__ float* out_row(const AttentionArgs& a, const Segment& s,
+                                                   int r) {
+    const int tok = (int)a.by_group.of(r);
+    return a.out + (int64_t)(s.seq.row0 + tok) * a.out_stride +
+           (int64_t)(s.g * a.group + r - tok * a.group) * D;
+  }
+  static constexpr uint32_t kMl = kFewRows * D * 4;  // of a part: where its (m, l) are
+
+  // Joins and writes a tile of up to 8 rows that came in many parts: groups of threads as many
+  // as there is room for, (rows to a power of two) D / 4 threads each, take some parts each.
+  static __device__ __forceinline__ void join_many(const AttentionArgs& a, const Segment& s,
+                                                   const Shared& sh, int tid, uint8_t* smem) {
+    constexpr int NJ = D > 128 ? 2 : 1, kAtOnce = 16 / NJ;
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
+    const int bits = s.rows > 4 ? 3 : s.rows > 2 ? 2 : s.rows > 1 ? 1 : 0;
+    const int quads = (D / 4) << bits;
+    const int groups = quads < kThreads ? kThreads / quads : 1;
+    const int group =
+        groups > 1 ? (int)(((float)tid + 0.5f) * __builtin_amdgcn_rcpf((float)quads)) : 0;
+    const int at = tid - group * quads, r = at & ((1 << bits) - 1);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 out[NJ] = {};
+    for (int p0 = group; p0 < s.parts && group < groups; p0 += kAtOnce * groups) {
+      f32x2 ml[kAtOnce];
+      f32x4 v[kAtOnce][NJ];
+#pragma unroll
+      for (int p = 0; p < kAtOnce; ++p) {
+        // Past the last part: that one again, not used.
+        const int part = p0 + p * groups < s.parts ? p0 + p * groups : s.parts - 1;
+        const uint32_t from = slot_at(sh, s, part);
+        ml[p] = load_part2(rs, from + r * 8, kMl);
+#pragma unroll
+        for (int i = 0; i < NJ; ++i)
+          v[p][i] = load_part(rs, from + ((at >> bits) * 16 + r) * 16,
+                              (i * kThreads >> bits) * 256);
+      }
+      float top = M;
+#pragma unroll
+      for (int p = 0; p < kAtOnce; ++p) top = fmaxf(top, ml[p].x);
+      const float keep = weight(M, top);
+      M = top;
+      L *= keep;
+#pragma unroll
+      for (int i = 0; i < NJ; ++i) out[i] *= keep;
+#pragma unroll
+      for (int p = 0; p < kAtOnce; ++p) {
+        if (p0 + p * groups < s.parts) {
+          const float f = weight(ml[p].x, M);
+          L = __builtin_fmaf(ml[p].y, f, L);
+#pragma unroll
+          for (int i = 0; i < NJ; ++i) out[i] += v[p][i] * f;
+        }
+      }
+    }
+    if (groups > 1) {  // NJ's first quad is all there is
+      f32x4* g_acc = reinterpret_cast<f32x4*>(smem + 1024);
+      f32x2* g_ml = reinterpret_cast<f32x2*>(smem + 1024 + kThreads * 16);
+      __syncthreads();  // the arrival count has been read
+      g_acc[tid] = out[0];
+      g_ml[tid] = f32x2{M, L};
+      __syncthreads();
+      M = -INFINITY;
+      L = 0.0f;
+      out[0] = f32x4{};
+      if (group == 0) {
+        for (int g = 0; g < groups; ++g) M = fmaxf(M, g_ml[g * quads + tid].x);
+        for (int g = 0; g < groups; ++g) {
+          const f32x2 ml = g_ml[g * quads + tid];
+          const float f = weight(ml.x, M);
+          L = __builtin_fmaf(ml.y, f, L);
+          out[0] += g_acc[g * quads + tid] * f;
+        }
+      }
+    }
+    if (group == 0 && r < s.rows) {
+      float* o = out_row(a, s, r);
+      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+      for (int i = 0; i < NJ; ++i)
+        if (at + i * kThreads < quads)
+          *reinterpret_cast<f32x4*>(o + (at + i * kThreads >> bits) * 4) =
+              L != 0.0f ? out[i] * inv : f32x4{};
+    }
+  }
+
   // One segment; `n` holds its first loads if n.started.  find_next() puts the next one into
   // `then`; if that is of few rows too, it comes next (true) and `n` gets its first loads.
   template <class F>
@@ -933,12 +1018,15 @@ struct FewRows {
     f32x4* s_acc = reinterpret_cast<f32x4*>(smem);                // [wave][4 D]
     f32x2* s_ml = reinterpret_cast<f32x2*>(smem + 4 * 4 * D * 16);  // [wave][16]
     __syncthreads();  // the memory's earlier readers
+    const int here = fresh(tid);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
-      s_acc[wave * 4 * D + (db * 4 + quad) * 16 + (lane & 15)] = acc[db];
-    if (lane < 16) s_ml[wave * 16 + lane] = f32x2{m, l};
+      s_acc[wave * 4 * D + db * 64 + (here & 63)] = acc[db];
+    if ((here & 63) < 16) s_ml[wave * 16 + (here & 15)] = f32x2{m, l};
     __syncthreads();
-    const int r = tid & 15;
+    // Thread tid has the quads tid + 256 i of the result: row tid % 16.
+    const int r = here & 15;
+    auto in_range = [&](int i) { return 4 * D % kThreads == 0 || here + i * kThreads < 4 * D; };
     f32x4 out[NQ] = {};
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -951,24 +1039,25 @@ struct FewRows {
       L = __builtin_fmaf(ml.y, f, L);
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
-        if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
-          out[i] += s_acc[w * 4 * D + tid + i * kThreads] * f;
+        if (in_range(i)) out[i] += s_acc[w * 4 * D + here + i * kThreads] * f;
     }
 
     if (s.parts > 1) {
-      constexpr uint32_t kMl = kFewRows * D * 4;
       const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
       const uint32_t to = slot_at(sh, s, s.part);
       if (r < s.rows) {
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-          if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
-            store_part(out[i], rs, tid * 16, to + i * kThreads * 16);
-        if (tid < 16) store_part2(f32x2{M, L}, rs, tid * 8, to + kMl);
+          if (in_range(i)) store_part(out[i], rs, here * 16, to + i * kThreads * 16);
+        if (here < 16) store_part2(f32x2{M, L}, rs, here * 8, to + kMl);
       }
       if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return go_on;
-      // In order, some at a time: their loads are in flight together.
-      constexpr int kAtOnce = 16 / NQ;
+      if (s.rows <= 8 && s.parts > 8) {
+        join_many(a, s, sh, here, smem);
+        return go_on;
+      }
+      // In order, some at a time, whose loads are in flight together.
+      constexpr int kAtOnce = 12 / NQ;
       M = -INFINITY;
       L = 0.0f;
 #pragma unroll
@@ -978,19 +1067,18 @@ struct FewRows {
         f32x4 v[kAtOnce][NQ];
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) {
-          // Past the last part: that one again, with no weight.
+          // Past the last part: that one again, not used.
           const uint32_t from = slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
           ml[p] = load_part2(rs, r * 8, from + kMl);
 #pragma unroll
           for (int i = 0; i < NQ; ++i)
-            if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D)
-              v[p][i] = load_part(rs, tid * 16, from + i * kThreads * 16);
+            if (in_range(i)) v[p][i] = load_part(rs, here * 16, from + i * kThreads * 16);
         }
-        float to = M;
+        float top = M;
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) to = fmaxf(to, ml[p].x);
-        const float keep = weight(M, to);
-        M = to;
+        for (int p = 0; p < kAtOnce; ++p) top = fmaxf(top, ml[p].x);
+        const float keep = weight(M, top);
+        M = top;
         L *= keep;
 #pragma unroll
         for (int i = 0; i < NQ; ++i) out[i] *= keep;
@@ -1001,22 +1089,19 @@ struct FewRows {
             L = __builtin_fmaf(ml[p].y, f, L);
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
-              if (4 * D % kThreads == 0 || tid + i * kThreads < 4 * D) out[i] += v[p][i] * f;
+              if (in_range(i)) out[i] += v[p][i] * f;
           }
         }
       }
     }
     if (r < s.rows) {
+      float* o = out_row(a, s, r);
       const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-      const int tok = (int)a.by_group.of(r);
-      float* o = a.out + (int64_t)(s.seq.row0 + tok) * a.out_stride +
-                 (int64_t)(s.g * a.group + r - tok * a.group) * D;
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const int qd = tid + i * kThreads;
-        if (4 * D % kThreads == 0 || qd < 4 * D)
-          *reinterpret_cast<f32x4*>(o + qd / 16 * 4) = L != 0.0f ? out[i] * inv : f32x4{};
-      }
+      for (int i = 0; i < NQ; ++i)
+        if (in_range(i))
+          *reinterpret_cast<f32x4*>(o + (here + i * kThreads) / 16 * 4) =
+              L != 0.0f ? out[i] * inv : f32x4{};
     }
     return go_on;
   }

@@ -129,6 +129,44 @@ def test_plan_matches_host_loop(dev, B, page, longest, most_new, short, finished
         np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("tokens_of_one", [3, 700])
+def test_plan_captured(dev, tokens_of_one):
+    """Replays follow the lengths on the device, with one workgroup and with several; the new
+    free count takes the place of the old one."""
+    import torch
+    rng = np.random.default_rng(tokens_of_one)
+    B, page = 12, 16
+    cached = rng.integers(0, 200, B)
+    new = np.full(B, tokens_of_one)
+    new[[2, 7]] = -1
+    tokens, max_pages = 10 * tokens_of_one, 64
+    table, stack, num_pages = plan_case(rng, B, page, cached, new, 480, max_pages)
+    held = [i32(x, dev) for x in (cached, new, table, stack, [480])]
+    start = [x.clone() for x in held]
+    out = [torch.zeros(n, dtype=torch.int32, device=dev) for n in (B, B + 1, tokens, tokens, B)]
+    stream = torch.cuda.Stream()
+    capi.workspace_reserve(256, 32, stream=stream)
+    torch.cuda.synchronize()
+    note(f"plan captured {tokens}")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        capi.paged_plan(held[0], held[1], B, held[2], max_pages, page, num_pages, held[3],
+                        held[4], held[4], tokens, *out, stream=stream)
+    for rep in range(4):
+        lens = (cached + 5 * rep) * (new >= 0) + cached * (new < 0)
+        for x, y in zip(held, start):
+            x.copy_(y)
+        held[0].copy_(i32(lens, dev))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [held[2], held[3], held[4], *out]
+        want = plan_host(lens, new, table, page, num_pages, stack, 480, tokens)
+        for g, w in zip(got, want):
+            np.testing.assert_array_equal(g.cpu().numpy().reshape(-1),
+                                          np.asarray(w).reshape(-1))
+
+
 def test_plan_refuses_what_does_not_fit(dev):
     """Requests past max_pages, rows past `tokens`, negative lengths and bad page numbers."""
     rng = np.random.default_rng(5)
@@ -443,6 +481,17 @@ def test_attention(dev, kv_type, H, G, D, lens, page, window):
 def test_attention_lengths(dev, kv_type, lens, page, window):
     note(f"attention lengths {kv_type} lens={lens} page={page} window={window}")
     b = Batch(dev, kv_type, 8, 2, 64, page, lens, window, seed=sum(t for _, t in lens))
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("H,G,D", [(2, 2, 64), (2, 1, 96), (3, 1, 128), (5, 1, 64), (8, 1, 256),
+                                   (1, 1, 256), (16, 1, 128), (24, 1, 96), (7, 1, 96)])
+@pytest.mark.parametrize("new,total,window", [(1, 6000, 0), (2, 5000, 0), (1, 7000, 3000)])
+def test_attention_of_few_rows_in_many_parts(dev, kv_type, H, G, D, new, total, window):
+    """One sequence: its keys go to as many workgroups as they are worth, then are joined."""
+    note(f"attention in parts {kv_type} H={H} G={G} D={D} {new} of {total} window={window}")
+    b = Batch(dev, kv_type, H, G, D, 32, [(new, total)], window, seed=total + D)
     b.check(b.run())
 
 
