@@ -678,6 +678,50 @@ def test_attention_far_pages(dev, kv_type):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("H,G,D,lens,window", [
+    (8, 2, 128, [(1, 700), (1, 64)], 0), (14, 2, 64, [(60, 400), (20, 20)], 100),
+    (4, 4, 96, [(130, 130)], 0), (8, 1, 256, [(40, 300), (1, 50)], 0)])
+def test_attention_relative_error(dev, kv_type, H, G, D, lens, window):
+    """The whole output within 2^-16 relative L2: a lost part of q (2^-12 of it in f16, 2^-17
+    in bf16 with two of three) or of the weights, or a value rounded to 16 bits anywhere, is
+    above or at that, while rounding errors of logits below 32 (2^-24 each, a few hundred of
+    them at random) are near 2^-19."""
+    import torch
+    note(f"attention relative error {kv_type} H={H} G={G} D={D} lens={lens}")
+    b = Batch(dev, kv_type, H, G, D, 32, lens, window, seed=D)
+    out = b.run()
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(b.want.shape).astype(np.float64)
+    assert np.linalg.norm(got - b.want) <= 2.0 ** -16 * np.linalg.norm(b.want)
+
+
+@pytest.mark.parametrize("n,total", [(1, 90), (3, 90), (60, 200)])
+@pytest.mark.parametrize("which,value", [("k", float("nan")), ("v", float("nan")),
+                                         ("v", float("inf"))])
+def test_attention_non_finite_scales(dev, n, total, which, value):
+    """An 8-bit row whose scale is not finite makes NaN of the rows that see it, no others."""
+    import torch
+    H, G, D, page = 4, 2, 64, 16
+    note(f"attention scale {which}={value} n={n}")
+    b = Batch(dev, "int8", H, G, D, page, [(n, total)], seed=n)
+    at = total - n + n // 2
+    slot = int(b.table[0, at // page]) * page + at % page
+    scales = b.cache.k_scale if which == "k" else b.cache.v_scale
+    scales.view(-1, G, page)[slot // page, 1, slot % page] = value
+    if value == float("inf"):  # what a row with an infinity stores
+        r, tile = slot % 16, slot % page // 16
+        b.cache.v.view(-1, G, page // 16, 2, D, 2, 4)[slot // page, 1, tile, r // 4 % 2, :,
+                                                      r // 8, r % 4] = 0
+    out = b.run()
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(n, H, D)
+    first, hit = n // 2, slice(H // G, H)
+    assert np.isnan(got[first:, hit]).all()
+    got[first:, hit] = b.want[first:, hit]
+    assert np.abs(got - b.want).max() <= b.tol
+
+
 # ---- the step as a whole ----
 
 @pytest.mark.parametrize("kv_type", TYPES)
