@@ -125,7 +125,8 @@ int mle_rope_table(float* table, int positions, int rope_dim, double theta,
  * Errors: NULL pointers, tokens < 0, sizes <= 0, misalignment -> InvalidArgument;
  * strides too small or not a multiple of 4, rope_dim not a multiple of 8 or above
  * head_dim, unknown type or mode -> InvalidArgument; a head_dim or page_size the cache
- * does not take -> Unsupported.  tokens == 0 is a no-op.
+ * does not take, tokens * (heads + 2 kv_heads) above 2^30 -> Unsupported.  tokens == 0 is a
+ * no-op.
  */
 int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_stride,
                        float* q_out, int q_out_stride, int heads, const float* k, int k_stride,
@@ -140,22 +141,25 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
  * window > 0 only those with j > p - window.  Query head h reads KV head
  * h / (heads / kv_heads).
  *   out[row][h] = sum_j softmax_j(scale * q . k_j) v_j
- * in fp32 accuracy: q and the probabilities go to the matrix cores as exact sums of
- * 16-bit parts, the cache's values are taken as they are, sums are fp32.  A row that sees
- * no key is zero; a key in a page outside [0, num_pages) counts as hidden, hidden keys
- * and values may hold anything, NaN included.  Rows outside every sequence are not
+ * in fp32 accuracy: q and the probabilities go to the matrix cores as sums of 16-bit
+ * parts (two of f16, 22 bits, three of bf16 over a bf16 cache), the cache's values are
+ * taken as they are, sums are fp32.  A row that sees no key is zero; a key in a page
+ * outside [0, num_pages) counts as hidden, hidden keys and values may hold anything, NaN
+ * included; a NaN or an infinity that a row sees reaches that row alone.  Rows outside every sequence are not
  * written.  Long sequences with few rows are split over the keys and joined in a fixed
  * order: deterministic run to run.
  * Row strides in floats, multiples of 4; out must not overlap q unless it is q with the
  * same stride.  `sequences` may include some without new rows.
  * Errors: NULL pointers, sizes <= 0, tokens < 0, heads not a multiple of kv_heads, a
  * window < 0, a scale that is not finite, bad strides or alignment -> InvalidArgument;
- * a head_dim or page_size the cache does not take, heads / kv_heads above 64 ->
- * Unsupported.  tokens == 0 is a no-op.
+ * a head_dim or page_size the cache does not take, heads / kv_heads above 64, more than
+ * 31 bits of max_pages * page_size or tokens * heads / kv_heads -> Unsupported.
+ * tokens == 0 is a no-op.
  *
  * mle_paged_attention_workspace_size: what any call of 1 .. tokens rows in 1 ..
  * sequences sequences takes of the per-stream workspace (mle_workspace_reserve; to be
- * reserved before a graph is captured).
+ * reserved before a graph is captured): 9 MB for up to 16 rows of a KV head, 69 MB above
+ * (head_dim 128), whatever the lengths.
  */
 int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stride, float* out,
                         int out_stride, int heads, float scale, int window,

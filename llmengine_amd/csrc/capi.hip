@@ -1304,6 +1304,9 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
       return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": unknown rope_mode " +
                                             std::to_string(rope_mode));
   }
+  if ((int64_t)tokens * (heads + 2LL * cache->kv_heads) > kPagedMax)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": tokens * (heads + 2 kv_heads) must fit 30 bits");
   if (tokens == 0) return ok();
   a.q = q;
   a.q_out = q_out;

@@ -1553,6 +1553,8 @@ struct ManyRows {
   }
 };
 
+constexpr int kCus = 256, kMostGroups = 2 * kCus;  // workgroups: two a CU up to size 128
+
 template <KvType T, int D>
 constexpr int kLds = ManyRows<T, D>::kLdsBytes > 4 * 16 * (D * 4 + 8)
                          ? ManyRows<T, D>::kLdsBytes : 4 * 16 * (D * 4 + 8);
@@ -1578,9 +1580,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     sch.seq[tid] = s;
     const Cost c = cost_of<T>(a, s);
     sum += c.before(c.tiles) * a.cache.kv_heads;
-    tiles += c.tiles * a.cache.kv_heads < kThreads ? c.tiles * a.cache.kv_heads : kThreads;
+    // More than workgroups are no matter.
+    const int64_t n = (int64_t)c.tiles * a.cache.kv_heads;
+    tiles = tiles + n < kMostGroups ? tiles + (int)n : kMostGroups;
   }
-  tiles = tiles < (1 << 20) ? tiles : 1 << 20;
 #pragma unroll 1
   for (int off = 1; off < 64; off <<= 1) {
     const uint64_t o = (uint64_t)from_lane((int64_t)sum, lane - off);
@@ -1666,9 +1669,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   }
 }
 
-constexpr int kCus = 256;
-
-int grid_of(int head_dim) { return kCus * (head_dim <= 128 ? 2 : 1); }
+int grid_of(int head_dim) { return head_dim <= 128 ? kMostGroups : kCus; }
 
 int slot_floats_of(int head_dim, int64_t rows) {
   return (rows <= kFewRows ? kFewRows : kTileRows) * (head_dim + 4);

@@ -240,8 +240,6 @@ hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
   KvWriteArgs b = a;
   const int64_t kv_blocks = blocks_of(2 * a.cache.kv_heads);
   const int64_t blocks = kv_blocks + blocks_of((a.heads + kQHeads - 1) / kQHeads);
-  // Rows of heads are counted in 32 bits.
-  if (blocks > (int64_t(1) << 26)) return hipErrorInvalidValue;
   b.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((unsigned)blocks), block(256);
   if (lpr == 8)

@@ -668,6 +668,25 @@ def test_attention_graph_replays(dev, kv_type):
         assert torch.equal(extra, eager[1])
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_capture_without_reservation_is_refused(dev):
+    """Attention, and a plan of many rows, that would allocate their workspace in a capture."""
+    import torch
+    b = Batch(dev, "f16", 4, 2, 64, 16, [(1, 40)])
+    out = empty_f32(b.q.shape, dev)
+    words = [torch.zeros(5000, dtype=torch.int32, device=dev) for _ in range(11)]
+    torch.cuda.synchronize()
+    for call in (lambda s: b.run(out=out, stream=s),
+                 lambda s: capi.paged_plan(*words[:2], 2, words[2], 4, 16, 8, *words[3:6], 5000,
+                                           *words[6:11], stream=s)):
+        stream = torch.cuda.Stream()
+        with pytest.raises(capi.Q8_0Error) as err:
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                call(stream)
+        assert "reserve it before capture" in str(err.value)
+        assert capi.workspace_info(stream)[2] == 0
+
+
 @pytest.mark.parametrize("kv_type", TYPES)
 def test_attention_far_pages(dev, kv_type):
     """Pages whose elements lie past 2^31 of the cache's buffers."""

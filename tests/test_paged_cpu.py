@@ -128,6 +128,7 @@ def test_rope_table_refusals(bad, code, text):
     (dict(v_stride=129), INVALID, "v stride"), (dict(rope_positions=0), INVALID, "rope_pos"),
     (dict(rope_dim=0), INVALID, "rope_dim"), (dict(rope_dim=12), INVALID, "multiple of 8"),
     (dict(rope_dim=72), INVALID, "at most head_dim"), (dict(rope_mode=2), INVALID, "rope_mode"),
+    (dict(tokens=1 << 28), UNSUPPORTED, "30 bits"),
 ])
 def test_write_refusals(bad, code, text):
     got, msg = write(**bad)
@@ -146,6 +147,7 @@ def test_write_refusals(bad, code, text):
     (dict(scale=float("nan")), INVALID, "scale"), (dict(scale=float("inf")), INVALID, "scale"),
     (dict(q_stride=250), INVALID, "q stride"), (dict(out_stride=257), INVALID, "out stride"),
     (dict(tokens=-2), INVALID, "tokens"),
+    (dict(heads=128, tokens=1 << 25), UNSUPPORTED, "31 bits"),
 ])
 def test_attention_refusals(bad, code, text):
     got, msg = attention(**bad)
