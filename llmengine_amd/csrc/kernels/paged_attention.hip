@@ -15,6 +15,11 @@
 // 2^(s_j + log2 vs_j - m), with m the maximum of those sums, so that the parts have their
 // bits where the row's contributions are; l gets p_j vs_j * (1 / vs_j).
 //
+// A workgroup is four waves, two workgroups a CU (one at head size 256), so that one's softmax
+// runs beside the other's products; the loop over segments makes what it can anew in each
+// (fresh, fresh_args, forget), since values kept across it cost the inner loops their
+// registers: with them kept the 128-wide kernels spilled.
+//
 // A value of V that is not finite must reach the rows that see it and no others, and 0 times
 // it, or the parts of P times it, are NaN.  Where a sum comes out non-finite, the keys are gone
 // through again, with such values taken out of the product and added to the rows that see
@@ -23,10 +28,22 @@
 // The maximum moves only when a logit passes it by 2^8 (P and l stay far from their limits),
 // so that the rescaling of O is rare.
 //
-// Work is laid out on the device, from the lengths there: units of 64 keys of one (sequence,
+// Work is laid out on the device, from the lengths there (the host knows only bounds, and a
+// launch shaped by those would be mostly empty workgroups): units of 64 keys of one (sequence,
 // KV head, row tile), cut into as many equal runs as there are workgroups, whatever the mix
 // of short and long sequences, decoding and prompts.  A tile cut by a run's end is joined,
 // in order, by the workgroup that finishes last.
+//
+// What bounds it (MI355X; a large copy reaches 4.9 TB/s, a large f16 product 1.15 PFLOP/s):
+//   decoding: HBM.  32 sequences of up to 4096 tokens, 32 heads of 128, 181 us = 5.3 TB/s;
+//     8 of up to 32768 of 8 bits, 8 KV heads, 64 us = 4.1 TB/s, of which about 10 are the
+//     beginning and 5 the joins.
+//   prompts: the matrix cores at the clock they leave.  2048 tokens over 10240, 32 heads over
+//     8, 554-585 us = 1.06-1.12 PFLOP/s of parts; 56% of the cycles at 1.9 GHz.  Priorities
+//     of the waves, a second accumulator for the low parts, and loads issued between the
+//     matrix instructions changed nothing.
+//   short calls: a chain of latencies (lengths, run, page table, keys) of 6 us for few rows
+//     and 12 for many: 129 tokens of 14 heads 8.9 us.
 #include "../launch.hpp"
 #include "../paged.hpp"
 #include "../q8_0_device.hpp"
@@ -574,6 +591,12 @@ __device__ __forceinline__ Tiles find_tile(const AttentionArgs& a, const Segment
 }
 
 // ---- few rows: the workgroup's waves split the keys ----
+//
+// Bound by HBM, so by bytes in flight: a wave has a step's K and V (16 KB of 32 keys, or of 64
+// of 8 bits, at head size 128) under way in registers, straight from the cache, whose layout
+// makes each load one run of memory.  16 columns of q are 16 rows or copies of the last one:
+// the matrix cores are idle for most of the time anyway.  The next tile's first loads go out
+// before the present one is joined and written (32 x <= 4096: 200 -> 182 us).
 
 template <KvType T, int D>
 struct FewRows {
@@ -1122,6 +1145,11 @@ __device__ __forceinline__ void wait_for_loads() {
 }
 
 // ---- many rows: four waves of 32 rows share the keys in LDS ----
+//
+// 32 rows a wave, so that a fragment of K or V from LDS feeds all parts' products (32 KB of
+// LDS reads for 2048 cycles of the matrix cores a unit); stages of 64 keys, two of them, one
+// loading while the other is used; one barrier a stage.  8-bit stages go through registers
+// and become f16 on the way, once for all four waves.
 
 template <KvType T, int D>
 struct ManyRows {
@@ -1370,7 +1398,6 @@ struct ManyRows {
               for (int p = 0; p < kParts<T>; ++p) sc = mfma32<T>(f[n], qp[p][from + n], sc);
           }
           read_v(stage, u, 0);  // on its way during the softmax
-          __builtin_amdgcn_sched_barrier(0);
           const float* ks = reinterpret_cast<const float*>(smem + kScales) + buf * 3 * kUnit +
                             u * 32 + half * 4;
           if constexpr (kBytes<T>) {
