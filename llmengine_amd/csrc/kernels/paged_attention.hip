@@ -1385,9 +1385,12 @@ struct ManyRows {
         odd = any_of(clear_v(s, tid, base, bad_now, careful, stage), wave, smem + kFlags);
 
       if (live && base < ours.hi && base + kUnit > ours.lo) {
-        const bool whole = base >= ours.lo_all && base + kUnit <= ours.hi_all && bad_now == 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {  // 32 keys: two tiles
+          const int from_key = base + u * 32;
+          if (from_key >= ours.hi || from_key + 32 <= ours.lo) continue;
+          const bool whole =
+              from_key >= ours.lo_all && from_key + 32 <= ours.hi_all && bad_now == 0;
           f32x16 sc = {};
 #pragma unroll
           for (int from = 0; from < KK; from += FB) {
