@@ -39,7 +39,7 @@
 //     8 of up to 32768 of 8 bits, 8 KV heads, 64 us = 4.1 TB/s, of which about 10 are the
 //     beginning and 5 the joins.
 //   prompts: the matrix cores at the clock they leave.  2048 tokens over 10240, 32 heads over
-//     8, 554-585 us = 1.06-1.12 PFLOP/s of parts; 56% of the cycles at 1.9 GHz.  Priorities
+//     8, 546-585 us = 1.06-1.13 PFLOP/s of parts; 56% of the cycles at 1.9 GHz.  Priorities
 //     of the waves, a second accumulator for the low parts, and loads issued between the
 //     matrix instructions changed nothing.
 //   short calls: a chain of latencies (lengths, run, page table, keys) of 6 us for few rows
@@ -53,7 +53,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnit = 64;         // keys of a unit of work, and of a stage in LDS
-constexpr int kFewRows = 16;      // up to this many rows the waves split the keys
+// Up to this many rows the waves split the keys; it is what one matrix instruction holds.  At
+// 16 rows over 32 sequences of 4096 (f16, 8 KV heads of 128) 37 us against 42 with the tiles
+// of many rows, at 7 over 32768 of 8 bits (2 heads of 64) 22 against 148, and nowhere slower.
+constexpr int kFewRows = 16;
 constexpr int kTileRows = 128;    // above: four waves of 32 rows share the keys in LDS
 constexpr float kSlack = 8.0f;    // log2 of what a logit may pass the kept maximum by
 constexpr float kTinyScale = 0x1p-100f;
