@@ -39,7 +39,7 @@
 //     8 of up to 32768 of 8 bits, 8 KV heads, 64 us = 4.1 TB/s, of which about 10 are the
 //     beginning and 5 the joins.
 //   prompts: the matrix cores at the clock they leave.  2048 tokens over 10240, 32 heads over
-//     8, 546-585 us = 1.06-1.13 PFLOP/s of parts; 56% of the cycles at 1.9 GHz.  Priorities
+//     8, 546-585 us = 1.06-1.13 PFLOP/s of parts; 55% of 1.07 million cycles.  Priorities
 //     of the waves, a second accumulator for the low parts, and loads issued between the
 //     matrix instructions changed nothing.
 //   short calls: a chain of latencies (lengths, run, page table, keys) of 6 us for few rows
