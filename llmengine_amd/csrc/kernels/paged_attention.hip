@@ -51,13 +51,12 @@
 namespace mle {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kAttentionThreads;
 constexpr int kUnit = 64;         // keys of a unit of work, and of a stage in LDS
-// Up to this many rows the waves split the keys; it is what one matrix instruction holds.  At
-// 16 rows over 32 sequences of 4096 (f16, 8 KV heads of 128) 37 us against 42 with the tiles
-// of many rows, at 7 over 32768 of 8 bits (2 heads of 64) 22 against 148, and nowhere slower.
-constexpr int kFewRows = 16;
-constexpr int kTileRows = 128;    // above: four waves of 32 rows share the keys in LDS
+// kFewRows is what one matrix instruction holds.  At 16 rows over 32 sequences of 4096 (f16, 8
+// KV heads of 128) that form takes 37 us against 42 with the tiles of many rows, at 7 over
+// 32768 of 8 bits (2 heads of 64) 22 against 148, and nowhere longer.
+constexpr int kTileRows = 128;    // above kFewRows: four waves of 32 rows share the keys in LDS
 constexpr float kSlack = 8.0f;    // log2 of what a logit may pass the kept maximum by
 constexpr float kTinyScale = 0x1p-100f;
 constexpr int kDeviceScope = 16;  // cache policy of loads and stores
@@ -371,6 +370,7 @@ struct Shared {
   float* partials;
   uint32_t* counters;
   int slot_floats;
+  uint32_t bytes;  // of the partials: no access of a part goes past them
 };
 
 // What is written to LDS before is read from there, not kept in registers.
@@ -710,20 +710,25 @@ struct FewRows {
     return a.out + (int64_t)(s.seq.row0 + tok) * a.out_stride +
            (int64_t)(s.g * a.group + r - tok * a.group) * D;
   }
-  static constexpr uint32_t kMl = kFewRows * D * 4;  // of a part: where its (m, l) are
+  using Part = FewPart<D>;
+  static constexpr uint32_t kMl = Part::kMl;  // of a part: where its (m, l) are
 
   // Joins and writes a tile of up to 8 rows that came in many parts: groups of threads as many
   // as there is room for, (rows to a power of two) D / 4 threads each, take some parts each.
   static __device__ __forceinline__ void join_many(const AttentionArgs& a, const Segment& s,
                                                    const Shared& sh, int tid, uint8_t* smem) {
-    constexpr int NJ = D > 128 ? 2 : 1, kAtOnce = 16 / NJ;
-    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
+    constexpr int NJ = Part::kQuadsOfThread, kAtOnce = 16 / NJ;
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
     const int bits = s.rows > 4 ? 3 : s.rows > 2 ? 2 : s.rows > 1 ? 1 : 0;
-    const int quads = (D / 4) << bits;
+    const int quads = Part::quads(bits);
     const int groups = quads < kThreads ? kThreads / quads : 1;
     const int group =
         groups > 1 ? (int)(((float)tid + 0.5f) * __builtin_amdgcn_rcpf((float)quads)) : 0;
     const int at = tid - group * quads, r = at & ((1 << bits) - 1);
+    uint32_t quad_at[NJ];
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) quad_at[i] = Part::quad_at(at, i, bits);
+    const uint32_t ml_at = Part::ml_at(at, bits);
     float M = -INFINITY, L = 0.0f;
     f32x4 out[NJ] = {};
     for (int p0 = group; p0 < s.parts && group < groups; p0 += kAtOnce * groups) {
@@ -734,11 +739,9 @@ struct FewRows {
         // Past the last part: that one again, not used.
         const int part = p0 + p * groups < s.parts ? p0 + p * groups : s.parts - 1;
         const uint32_t from = slot_at(sh, s, part);
-        ml[p] = load_part2(rs, from + r * 8, kMl);
+        ml[p] = load_part2(rs, from + ml_at, 0);
 #pragma unroll
-        for (int i = 0; i < NJ; ++i)
-          v[p][i] = load_part(rs, from + ((at >> bits) * 16 + r) * 16,
-                              (i * kThreads >> bits) * 256);
+        for (int i = 0; i < NJ; ++i) v[p][i] = load_part(rs, from + quad_at[i], 0);
       }
       float top = M;
 #pragma unroll
@@ -783,7 +786,7 @@ struct FewRows {
       const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
       for (int i = 0; i < NJ; ++i)
-        if (at + i * kThreads < quads)
+        if (Part::has(at, i, bits))
           *reinterpret_cast<f32x4*>(o + (at + i * kThreads >> bits) * 4) =
               L != 0.0f ? out[i] * inv : f32x4{};
     }
@@ -1069,7 +1072,7 @@ struct FewRows {
     }
 
     if (s.parts > 1) {
-      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
+      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
       const uint32_t to = slot_at(sh, s, s.part);
       if (r < s.rows) {
 #pragma unroll
@@ -1516,7 +1519,7 @@ struct ManyRows {
     if (s.parts > 1) {
       constexpr uint32_t kMl = kTileRows * D * 4;
       const int at = fresh(tid);
-      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, 0xffffffffu);
+      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
       const uint32_t to = slot_at(sh, s, s.part);
       if (wrow < s.rows) {
 #pragma unroll
@@ -1738,7 +1741,9 @@ hipError_t launch_paged_attention(const AttentionArgs& args, const SplitKWorkspa
   a.by_group = Divisor(a.group);
   a.by_page = Divisor(a.cache.page_size);
   const int64_t rows = (int64_t)a.tokens * a.group;
-  const Shared sh{ws.partials, ws.counters, slot_floats_of(a.cache.head_dim, rows)};
+  const SplitKNeed need = paged_attention_workspace(a.cache.head_dim, rows);
+  const Shared sh{ws.partials, ws.counters, slot_floats_of(a.cache.head_dim, rows),
+                  (uint32_t)(need.partial_floats * sizeof(float))};
   switch (a.cache.type) {
     case KvType::kF16: return launch_typed<KvType::kF16>(a, sh, stream);
     case KvType::kBF16: return launch_typed<KvType::kBF16>(a, sh, stream);

@@ -101,6 +101,32 @@ struct AttentionArgs {
   int most;
   Divisor by_group, by_page;
 };
+constexpr int kAttentionThreads = 256;
+constexpr int kFewRows = 16;  // up to this many rows of a tile the waves split the keys
+
+// Places in a part of a tile of few rows: quads of a row's head_dim values, value quad c of
+// row r at 16 (16 c + r) bytes, behind them a (maximum, sum) a row.  A group of threads that
+// joins 2^bits rows takes quads() of them, thread `at` those of row at % 2^bits from
+// at >> bits on, kThreads further on each time.
+template <int D>
+struct FewPart {
+  static constexpr int kQuadsOfThread = D > 128 ? 2 : 1;
+  static constexpr uint32_t kMl = kFewRows * D * 4, kBytes = kFewRows * (D + 4) * 4;
+  static __host__ __device__ constexpr int quads(int bits) { return (D / 4) << bits; }
+  static __host__ __device__ constexpr bool has(int at, int i, int bits) {
+    return at + i * kAttentionThreads < quads(bits);
+  }
+  // Of a quad that the thread does not have, the part's first place: it is not used.
+  static __host__ __device__ constexpr uint32_t quad_at(int at, int i, int bits) {
+    if (!has(at, i, bits)) return 0;
+    const uint32_t quad = (uint32_t)(at + i * kAttentionThreads) >> bits;
+    return (quad * kFewRows + (uint32_t)(at & ((1 << bits) - 1))) * 16;
+  }
+  static __host__ __device__ constexpr uint32_t ml_at(int at, int bits) {
+    return kMl + (uint32_t)(at & ((1 << bits) - 1)) * 8;
+  }
+};
+
 // Workspace of a call with `rows` rows of one KV head (new tokens * heads / kv_heads).
 SplitKNeed paged_attention_workspace(int head_dim, int64_t rows);
 hipError_t launch_paged_attention(const AttentionArgs& a, const SplitKWorkspace& ws,

@@ -17,7 +17,7 @@ import math
 import numpy as np
 import pytest
 
-from helpers import empty_f32, note, to_dev
+from helpers import empty_f32, note, own_stream, to_dev
 from llmengine_amd import capi
 
 pytestmark = pytest.mark.gpu
@@ -793,3 +793,23 @@ def test_steps_together(dev, kv_type):
                 assert np.abs(got[row:row + n] - want).max() <= tol
             row += n
     assert count.item() == pages - sum(-(-int(n) // page) for n in lens)
+
+
+@pytest.mark.parametrize("kv_type,total", [("f16", 6069), ("bf16", 6069), ("int8", 8352)])
+@pytest.mark.parametrize("new", [1, 2])
+def test_attention_parts_up_to_the_workspace_end(dev, kv_type, total, new):
+    """One or two rows at head size 256 whose work is 256 equal runs, 16 of them a head: the
+    last part lies at the end of a workspace of exactly the stated size."""
+    import torch
+    note(f"attention parts to the workspace's end {kv_type} {new} of {total}")
+    b = Batch(dev, kv_type, 16, 16, 256, 32, [(new, total)], seed=new)
+    stream = own_stream()
+    size = capi.paged_attention_workspace_size(b.cache, 16, 1, new)
+    capi.workspace_reserve(*size, stream=stream)
+    assert capi.workspace_info(stream)[0] >= size[0]
+    out = empty_f32((b.T, b.H * b.D), dev)
+    torch.cuda.synchronize()
+    b.run(out=out, stream=stream)
+    stream.synchronize()
+    b.check(out)
+    assert torch.equal(b.run(), out)

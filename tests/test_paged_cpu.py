@@ -170,3 +170,16 @@ def test_workspace_size():
         a.update(kw)
         with pytest.raises(capi.Q8_0Error):
             capi.paged_attention_workspace_size(cache(), **a)
+
+
+def test_places_of_joined_parts():
+    """The threads that join a tile's parts read inside them: built from the kernel's header."""
+    import os
+    import subprocess
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin",
+                       "test_paged_parts")
+    if not os.path.exists(exe):
+        pytest.fail(f"{exe} not built: run `python -m llmengine_amd.build`")
+    p = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True,
+                       timeout=60)
+    assert p.returncode == 0, p.stdout
