@@ -102,7 +102,7 @@ int mle_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int sequ
  * 64 bits, rounded once.  freq_factors are a GGUF file's rope_freqs.  table is
  * 16-byte aligned, [positions][rope_dim / 2][2] fp32.
  * Errors: NULL table, positions or rope_dim <= 0, odd rope_dim, theta not positive and
- * finite -> InvalidArgument.
+ * finite -> InvalidArgument; positions * rope_dim / 2 above 2^32 - 256 -> Unsupported.
  */
 int mle_rope_table(float* table, int positions, int rope_dim, double theta,
                    const float* freq_factors, hipStream_t stream);
@@ -125,8 +125,9 @@ int mle_rope_table(float* table, int positions, int rope_dim, double theta,
  * Errors: NULL pointers, tokens < 0, sizes <= 0, misalignment -> InvalidArgument;
  * strides too small or not a multiple of 4, rope_dim not a multiple of 8 or above
  * head_dim, unknown type or mode -> InvalidArgument; a head_dim or page_size the cache
- * does not take, tokens * (heads + 2 kv_heads) above 2^30 -> Unsupported.  tokens == 0 is a
- * no-op.
+ * does not take, tokens * (heads + 2 kv_heads) above 2^30, or as many threads as a launch
+ * does not hold (8, 16 or 32 lanes for each k and v row and each two rows of q at head_dim
+ * 64, up to 128, 256: above 2^32 - 256) -> Unsupported.  tokens == 0 is a no-op.
  */
 int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_stride,
                        float* q_out, int q_out_stride, int heads, const float* k, int k_stride,

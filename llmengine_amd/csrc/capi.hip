@@ -1266,6 +1266,9 @@ int mle_rope_table(float* table, int positions, int rope_dim, double theta,
                 std::string("hip ") + ctx + ": theta must be positive and finite");
   MLE_TRY(check_align(ctx, table, 16, "table"));
   MLE_TRY(check_align(ctx, freq_factors, 4, "freq_factors"));
+  if (mle::rope_table_blocks(positions, rope_dim) > mle::kMostBlocks)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": positions * rope_dim / 2 must be below 2^32 - 256");
   return check_launch(
       mle::launch_rope_table(table, positions, rope_dim, theta, freq_factors, stream),
       "hip rope_table launch failed");
@@ -1307,6 +1310,13 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
   if ((int64_t)tokens * (heads + 2LL * cache->kv_heads) > kPagedMax)
     return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
                                      ": tokens * (heads + 2 kv_heads) must fit 30 bits");
+  const mle::KvWriteBlocks blocks =
+      mle::paged_kv_write_blocks(tokens, heads, cache->kv_heads, cache->head_dim);
+  if (blocks.kv + blocks.q > mle::kMostBlocks)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": tokens * (2 kv_heads + heads / 2) rows of " +
+                                     std::to_string(cache->head_dim) +
+                                     " take more than 2^32 threads");
   if (tokens == 0) return ok();
   a.q = q;
   a.q_out = q_out;

@@ -278,13 +278,15 @@ hipError_t launch_paged_plan(const PlanArgs& args, const SplitKWorkspace& ws, hi
   return hipGetLastError();
 }
 
+int64_t rope_table_blocks(int positions, int rope_dim) {
+  return ((int64_t)positions * (rope_dim / 2) + 255) / 256;
+}
+
 hipError_t launch_rope_table(float* table, int positions, int rope_dim, double theta,
                              const float* freq_factors, hipStream_t stream) {
   const int64_t n = (int64_t)positions * (rope_dim / 2);
-  const int64_t blocks = (n + 255) / 256;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, table, n,
-                     rope_dim / 2, theta, freq_factors);
+  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)rope_table_blocks(positions, rope_dim)),
+                     dim3(256), 0, stream, table, n, rope_dim / 2, theta, freq_factors);
   return hipGetLastError();
 }
 

@@ -240,15 +240,17 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   }
 }
 
+// Lanes of a head's row.
+int lanes_of(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32; }
+
 template <KvType T>
 hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
-  const int lpr = a.cache.head_dim <= 64 ? 8 : a.cache.head_dim <= 128 ? 16 : 32;
-  auto blocks_of = [&](int64_t rows) { return (a.tokens * rows * lpr + 255) / 256; };
+  const int lpr = lanes_of(a.cache.head_dim);
   KvWriteArgs b = a;
-  const int64_t kv_blocks = blocks_of(2 * a.cache.kv_heads);
-  const int64_t blocks = kv_blocks + blocks_of((a.heads + kQHeads - 1) / kQHeads);
-  b.kv_blocks = (uint32_t)kv_blocks;
-  const dim3 grid((unsigned)blocks), block(256);
+  const KvWriteBlocks n =
+      paged_kv_write_blocks(a.tokens, a.heads, a.cache.kv_heads, a.cache.head_dim);
+  b.kv_blocks = (uint32_t)n.kv;
+  const dim3 grid((unsigned)(n.kv + n.q)), block(256);
   if (lpr == 8)
     hipLaunchKernelGGL((paged_kv_write_kernel<T, 8>), grid, block, 0, stream, b);
   else if (lpr == 16)
@@ -259,6 +261,13 @@ hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+KvWriteBlocks paged_kv_write_blocks(int tokens, int heads, int kv_heads, int head_dim) {
+  auto blocks_of = [&](int64_t rows) {
+    return (tokens * rows * lanes_of(head_dim) + 255) / 256;
+  };
+  return {blocks_of(2 * (int64_t)kv_heads), blocks_of(((int64_t)heads + kQHeads - 1) / kQHeads)};
+}
 
 hipError_t launch_paged_kv_write(const KvWriteArgs& a, hipStream_t stream) {
   if (a.tokens <= 0) return hipSuccess;

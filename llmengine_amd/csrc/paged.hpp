@@ -11,6 +11,8 @@
 namespace mle {
 
 constexpr int kKvTile = 16;  // tokens of a cache tile
+// A launch of 256 threads a workgroup has fewer than 2^32 of them.
+constexpr int64_t kMostBlocks = (int64_t(1) << 24) - 1;
 enum class KvType { kF16 = 0, kBF16 = 1, kInt8 = 2 };
 struct PagedCache {
   void* k;
@@ -60,6 +62,7 @@ struct PlanArgs {
 SplitKNeed paged_plan_workspace(int tokens, int sequences);
 hipError_t launch_paged_plan(const PlanArgs& a, const SplitKWorkspace& ws, hipStream_t stream);
 
+int64_t rope_table_blocks(int positions, int rope_dim);
 hipError_t launch_rope_table(float* table, int positions, int rope_dim, double theta,
                              const float* freq_factors, hipStream_t stream);
 
@@ -80,6 +83,11 @@ struct KvWriteArgs {
   int tokens;
   uint32_t kv_blocks;  // set by the launcher
 };
+// Workgroups of the write: for k and v, then for q.
+struct KvWriteBlocks {
+  int64_t kv, q;
+};
+KvWriteBlocks paged_kv_write_blocks(int tokens, int heads, int kv_heads, int head_dim);
 hipError_t launch_paged_kv_write(const KvWriteArgs& a, hipStream_t stream);
 
 struct AttentionArgs {

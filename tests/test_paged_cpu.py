@@ -172,6 +172,23 @@ def test_workspace_size():
             capi.paged_attention_workspace_size(cache(), **a)
 
 
+@pytest.mark.parametrize("head_dim,heads,kv_heads,tokens", [
+    (64, 4, 2, (1 << 32) // (8 * 6)), (96, 2, 1, (1 << 32) // (16 * 3) + 1),
+    (128, 8, 8, (1 << 32) // (16 * 20)), (256, 8, 8, 1 << 23), (256, 1, 1, 1 << 26)])
+def test_write_of_more_threads_than_a_launch_has(head_dim, heads, kv_heads, tokens):
+    row, kv_row = heads * head_dim, kv_heads * head_dim
+    got, msg = write(cache(head_dim=head_dim, kv_heads=kv_heads), heads=heads, tokens=tokens,
+                     q_stride=row, q_out_stride=row, k_stride=kv_row, v_stride=kv_row)
+    assert got == UNSUPPORTED and "2^32 threads" in msg, (got, msg)
+
+
+@pytest.mark.parametrize("positions,rope_dim", [(1 << 27, 64), (1 << 30, 1 << 20),
+                                                (0x7fffffff, 0x7ffffffe)])
+def test_rope_table_of_more_threads_than_a_launch_has(positions, rope_dim):
+    got, msg = capi.rope_table_status(FAKE, positions, rope_dim, stream=0)
+    assert got == UNSUPPORTED and "2^32" in msg, (got, msg)
+
+
 def test_places_of_joined_parts():
     """The threads that join a tile's parts read inside them: built from the kernel's header."""
     import os
