@@ -174,7 +174,7 @@ def test_workspace_size():
 
 @pytest.mark.parametrize("head_dim,heads,kv_heads,tokens", [
     (64, 4, 2, (1 << 32) // (8 * 6)), (96, 2, 1, (1 << 32) // (16 * 3) + 1),
-    (128, 8, 8, (1 << 32) // (16 * 20)), (256, 8, 8, 1 << 23), (256, 1, 1, 1 << 26)])
+    (128, 8, 8, (1 << 32) // (16 * 20) + 1), (256, 8, 8, 1 << 23), (256, 1, 1, 1 << 26)])
 def test_write_of_more_threads_than_a_launch_has(head_dim, heads, kv_heads, tokens):
     row, kv_row = heads * head_dim, kv_heads * head_dim
     got, msg = write(cache(head_dim=head_dim, kv_heads=kv_heads), heads=heads, tokens=tokens,
