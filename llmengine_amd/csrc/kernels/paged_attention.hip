@@ -58,7 +58,6 @@ constexpr int kUnit = 64;         // keys of a unit of work, and of a stage in L
 // 32768 of 8 bits (2 heads of 64) 22 against 148, and nowhere longer.
 constexpr int kTileRows = 128;    // above kFewRows: four waves of 32 rows share the keys in LDS
 constexpr float kSlack = 8.0f;    // log2 of what a logit may pass the kept maximum by
-constexpr float kTinyScale = 0x1p-100f;
 constexpr int kDeviceScope = 16;  // cache policy of loads and stores
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -155,8 +154,8 @@ __device__ __forceinline__ bool is_non_finite(uint32_t half) {
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The scale of a V row as its logarithm and inverse; an all-zero row's scale of 0 counts as
-// a tiny one (its quants are 0).  NaN and infinity stay in the logarithm, which hidden keys
+// The scale of a V row as its logarithm and inverse; a scale of 0 counts as a tiny one (the
+// row's quants are 0).  NaN and infinity stay in the logarithm, which hidden keys
 // do not use; the inverse, times their weight of 0, is always finite.
 __device__ __forceinline__ float scale_log2(float v) {
   return __builtin_amdgcn_logf(v <= kTinyScale ? kTinyScale : v);

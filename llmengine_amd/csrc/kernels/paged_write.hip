@@ -221,6 +221,7 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
     for (int i = 0; i < 4; ++i) {
       if (i != 0 && !whole) break;
       scale[i] = amax_of<LPR>(r[i]) * (1.0f / 127.0f);
+      if (scale[i] <= kTinyScale) scale[i] = 0.0f;
       if (s == 0) a.cache.v_scale[cell + i] = scale[i];
     }
   }

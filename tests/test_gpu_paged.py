@@ -795,6 +795,48 @@ def test_steps_together(dev, kv_type):
     assert count.item() == pages - sum(-(-int(n) // page) for n in lens)
 
 
+@pytest.mark.parametrize("kv_type", ("bf16", "int8"))
+@pytest.mark.parametrize("new,total", [(1, 70), (3, 300), (40, 200)])
+@pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-29, 1e-27), (3e-28, 3e-28),
+                                      (1e-33, 1e-20), (1e-33, 1.0)])
+def test_tiny_values(dev, kv_type, new, total, low, high):
+    """V rows of any size down to 1e-33, written and attended: what comes out is what the cache
+    holds, within 2^-16 of it (see test_attention_relative_error), and 8-bit rows of scales at
+    or below 2^-100 are zeros of scale 0."""
+    import torch
+    note(f"tiny values {kv_type} {new} of {total} from {low} to {high}")
+    H, G, D, page = 4, 2, 64, 16
+    rng = np.random.default_rng(total)
+    q = (2 * rng.standard_normal((new, H, D))).astype(np.float32)
+    k, v = (rng.standard_normal((total, G, D)).astype(np.float32) for _ in range(2))
+    v *= np.exp(rng.uniform(np.log(low), np.log(high), (total, 1, 1))).astype(np.float32)
+    pages = -(-total // page)
+    slots = rng.permutation(pages)[np.arange(total) // page] * page + np.arange(total) % page
+    cache = capi.PagedCache.allocate(kv_type, pages, page, G, D, dev)
+    filler = torch.zeros(total, H * D, device=dev)
+    capi.paged_kv_write(cache, filler, filler, H, to_dev(k.reshape(total, -1), dev),
+                        to_dev(v.reshape(total, -1), dev), None, 0, D, "none", None,
+                        i32(slots, dev), total)
+    out = empty_f32((new, H * D), dev)
+    capi.paged_attention(cache, to_dev(q.reshape(new, -1), dev), out, H, D ** -0.5, 0,
+                         i32(slots[::page] // page, dev), pages, i32([total], dev),
+                         i32([0, new], dev), 1, new)
+    torch.cuda.synchronize()
+    ck, cv, ks, vs = (None if x is None else x.cpu()[slots] for x in
+                      cells_of(cache, pages, page, G, D))
+    if kv_type == "int8":
+        cells, scale = stored_host(v, kv_type)
+        zero = scale <= 2.0 ** -100
+        assert zero.any() == (low < 1e-28)
+        cells[zero], scale[zero] = 0, 0
+        assert torch.equal(cv, cells) and torch.equal(vs, scale)
+    held = [x.double().numpy() * (1 if s is None else s.double().numpy()[..., None])
+            for x, s in ((ck, ks), (cv, vs))]
+    want, _ = attention_host(q, *held, total - new + np.arange(new), 0, D ** -0.5)
+    got = out.cpu().numpy().reshape(want.shape).astype(np.float64)
+    assert np.linalg.norm(got - want) <= 2.0 ** -16 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("kv_type,total", [("f16", 6069), ("bf16", 6069), ("int8", 8352)])
 @pytest.mark.parametrize("new", [1, 2])
 def test_attention_parts_up_to_the_workspace_end(dev, kv_type, total, new):
