@@ -74,8 +74,8 @@ typedef struct mle_paged_cache {
  *      requests in order, and written to its row of block_table.  A request whose pages
  *      are not there (the pages asked for up to and including it are more than the
  *      stack holds), that would outgrow max_pages or 2^31 - 1 tokens or whose rows pass
- *      `tokens` is refused and its table row left as it is; requests that need no page
- *      are never short of one.
+ *      `tokens` (a request without new tokens has none) is refused and its table row left
+ *      as it is; requests that need no page are never short of one.
  *   3. kv_lens[b] = cached + new (refused or finished: 0).  cu_tokens[sequences + 1] =
  *      the first row of each request among the step's rows: prefix sums of the
  *      requested new tokens, refused requests included, at most `tokens`.

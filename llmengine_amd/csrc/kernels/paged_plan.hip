@@ -156,7 +156,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a, uint32
       valid = need <= (uint32_t)a.max_pages;
     }
     // Whether its rows fit is known once they are counted; one that is cut off there is
-    // refused with all after it, so that its pages in the sum do no harm.
+    // refused with all after it that have rows, so that its pages in the sum do no harm.
     Sums total;
     const Sums upto = scan<kThreads>({whole ? given_back(a, cached, fresh) : 0,
                                       want < kCap ? want : kCap, valid ? need - have : 0},
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a, uint32
       if (top > (uint32_t)a.num_pages) top = (uint32_t)a.num_pages;
     }
     const uint32_t end = sat_add(rows, upto.rows);
-    valid = valid && end <= (uint32_t)a.tokens;
+    valid = valid && (want == 0 || end <= (uint32_t)a.tokens);
     const uint32_t add = valid ? need - have : 0;
     const uint32_t until = sat_add(asked, upto.add);
     const bool granted = valid && (add == 0 || until <= top);

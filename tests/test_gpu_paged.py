@@ -180,6 +180,24 @@ def test_plan_refuses_what_does_not_fit(dev):
             np.testing.assert_array_equal(got, want)
 
 
+def test_plan_rows_past_the_end_refuse_only_requests_with_rows(dev):
+    """Requests without new tokens have no row that passes `tokens`: behind one that does,
+    they keep their lengths, and their pages where they hold any."""
+    cached, new = [20, 5, 33, 0, 7, 16], [3, 90, 0, 0, 2, -1]
+    table, stack, num_pages = plan_case(np.random.default_rng(2), 6, 16, cached, new, 12, 8)
+    for tokens in (95, 94, 10, 3, 2, 0):
+        note(f"plan rows past the end tokens={tokens}")
+        got = run_plan(dev, np.array(cached), np.array(new), table, 16, num_pages, stack, 12,
+                       tokens)
+        kv, cu, granted = got[3], got[4], got[7]
+        ok = [rows <= tokens for rows in (3, 93, 0, 0, 95)] + [True]
+        assert granted.tolist() == [int(x) for x in ok]
+        assert kv.tolist() == [(c + max(n, 0)) * (x and n >= 0)
+                               for c, n, x in zip(cached, new, ok)]
+        assert cu.tolist() == [0] + [min(r, tokens) for r in (3, 93, 93, 93, 95, 95)]
+        assert got[2] == 12 + 1 - 5 * ok[1]  # 5 to 95 tokens: 5 pages more
+
+
 # ---- rotations and the write ----
 
 @pytest.mark.parametrize("rope_dim,theta,factors", [(64, 10000.0, False), (128, 5e5, True),
