@@ -1138,11 +1138,12 @@ struct FewRows {
 // 16 bytes a lane from global memory to LDS, a wave's 1024 in one run, without registers.
 // Not the builtin: with that every later read of LDS first waits for all loads in flight.
 // The caller waits (wait_for_loads) before the barrier behind which the bytes are read.
-// Nothing else here uses m0 (an asm cannot name it as overwritten).
+// m0 holds the place in LDS: the compiler writes it there, so it knows what m0 holds.
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, uint8_t* to) {
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)to;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(uniform((int)at)), "v"(from) : "memory");
+  register int m0 asm("m0") = uniform((int)at);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(m0), "v"(from) : "memory");
 }
 
 __device__ __forceinline__ void wait_for_loads() {

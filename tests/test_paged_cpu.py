@@ -189,6 +189,22 @@ def test_rope_table_of_more_threads_than_a_launch_has(positions, rope_dim):
     assert got == UNSUPPORTED and "2^32" in msg, (got, msg)
 
 
+def test_no_asm_writes_m0_unseen():
+    """An asm statement cannot name m0 as overwritten, so none may write it: it gets m0 as an
+    operand, which the compiler sets."""
+    import glob
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    files = glob.glob(os.path.join(root, "llmengine_amd", "csrc", "**", "*.h*"), recursive=True)
+    assert len(files) > 10
+    for path in files:
+        with open(path) as f:
+            code = re.sub(r"//[^\n]*", "", f.read())
+        for text in re.findall(r"\basm\b[^;]*;", code):
+            assert not re.search(r"[\"\s]s_\w+ m0\b", text), (path, text)
+
+
 def test_places_of_joined_parts():
     """The threads that join a tile's parts read inside them: built from the kernel's header."""
     import os
