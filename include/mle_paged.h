@@ -148,8 +148,8 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
  * parts (two of f16, 22 bits, three of bf16 over a bf16 cache), the cache's values are
  * taken as they are, sums are fp32.  A row that sees no key is zero; a key in a page
  * outside [0, num_pages) counts as hidden, hidden keys and values may hold anything, NaN
- * included; a NaN or an infinity that a row sees reaches that row alone.  Rows outside every sequence are not
- * written.  Long sequences with few rows are split over the keys and joined in a fixed
+ * included; a NaN or an infinity that a row sees reaches that row alone, where a logit of
+ * minus infinity is a weight of 0.  Rows outside every sequence are not written.  Long sequences with few rows are split over the keys and joined in a fixed
  * order: deterministic run to run.
  * Row strides in floats, multiples of 4; out must not overlap q unless it is q with the
  * same stride.  `sequences` may include some without new rows.

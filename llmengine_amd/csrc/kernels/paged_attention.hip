@@ -154,6 +154,20 @@ __device__ __forceinline__ bool is_non_finite(uint32_t half) {
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// q . k of a key for which the matrix cores give NaN: they make that of an infinity in K,
+// times the low parts of q, whatever the product is.  It is not finite, so that the finite
+// terms do not count.
+template <KvType T, int D>
+__device__ __forceinline__ float product_of(const float* q, const uint16_t* k) {
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) {
+    const float term = q[d] * value_of<T>(k[d / 8 * (kKvTile * 8) + d % 8]);
+    if (term - term != 0.0f) sum += term;
+  }
+  return sum;
+}
+
 // The scale of a V row as its logarithm and inverse; a scale of 0 counts as a tiny one (the
 // row's quants are 0).  NaN and infinity stay in the logarithm, which hidden keys
 // do not use; the inverse, times their weight of 0, is always finite.
@@ -882,12 +896,25 @@ struct FewRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[t][i] = r[i];
       }
-      if constexpr (kBytes<T>)
+      if constexpr (kBytes<T>) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
+      } else if (careful) {
+#pragma unroll 1
+        for (int j = 0; j < kTiles * 4; ++j) {
+          const uint16_t* k = static_cast<const uint16_t*>(a.cache.k) +
+                              (j < 4 ? tile[0] : tile[1]) * (kKvTile * D) +
+                              (quad * 4 + j % 4) * 8;
+          const float exact = product_of<T, D>(q - quad * 8, k);
+#pragma unroll
+          for (int i = 0; i < kTiles * 4; ++i)
+            if (i == j && sc[i / 4][i % 4] != sc[i / 4][i % 4])
+              sc[i / 4][i % 4] = a.scale < 0.0f ? -exact : exact;
+        }
+      }
 
       // The next step's K goes out before the softmax.
       const bool more = base + 4 * kStep < hi;
@@ -1026,7 +1053,7 @@ struct FewRows {
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
-      if (!careful && __any(zero != zero && l - l == 0.0f)) {
+      if (!careful && __any(zero != zero)) {
         careful = true;
         n.started = false;
         goto again;
@@ -1419,6 +1446,24 @@ struct ManyRows {
                 sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
             }
           }
+          if (!kBytes<T> && careful) {
+            const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
+            const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
+            const int token = (int)a.by_group.of(row);
+            const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                             (int64_t)(s.g * a.group + row - token * a.group) * D;
+#pragma unroll 1
+            for (int j = 0; j < 16; ++j) {
+              const int key = (j >> 2) * 8 + (me >> 3 & 4) + (j & 3);
+              const uint16_t* k = reinterpret_cast<const uint16_t*>(
+                                      stage + (2 * u + key / kKvTile) * kTileBytes) +
+                                  key % kKvTile * 8;
+              const float exact = product_of<T, D>(q, k);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (i == j && sc[i] != sc[i]) sc[i] = a.scale < 0.0f ? -exact : exact;
+            }
+          }
           if (!whole) {
             const int from = fresh(base + half * 4 - mine.lo);
 #pragma unroll
@@ -1502,7 +1547,7 @@ struct ManyRows {
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
-      if (!careful && any_of(zero != zero && l - l == 0.0f, wave, smem + kFlags + 16)) {
+      if (!careful && any_of(zero != zero, wave, smem + kFlags + 16)) {
         careful = true;
         m = -INFINITY;
         l = 0.0f;

@@ -813,6 +813,63 @@ def test_steps_together(dev, kv_type):
     assert count.item() == pages - sum(-(-int(n) // page) for n in lens)
 
 
+@pytest.mark.parametrize("kv_type", ("f16", "bf16"))
+@pytest.mark.parametrize("H,G,D,new,total,window", [
+    (4, 2, 64, 1, 70, 0), (4, 2, 128, 3, 300, 0), (3, 1, 256, 5, 90, 40), (2, 2, 96, 2, 5000, 0),
+    (4, 2, 64, 60, 200, 0), (4, 1, 128, 70, 300, 90), (2, 1, 96, 40, 130, 0),
+    (2, 1, 256, 40, 130, 0)])
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_attention_infinities_in_k(dev, kv_type, H, G, D, new, total, window, scale):
+    """An infinity in K makes a logit infinite: minus infinity gives its key the weight 0, plus
+    infinity makes NaN of the rows that see it, and the other heads and rows stay."""
+    import torch
+    page = 16
+    rng = np.random.default_rng(new + D)
+    q = (2 * rng.standard_normal((new, H, D))).astype(np.float32)
+    k, v = (rng.standard_normal((total, G, D)).astype(np.float32) for _ in range(2))
+    pos = total - new + np.arange(new)
+    _, tol = attention_host(q, *(x.astype(np.float64) for x in (k, v)), pos, window, scale)
+    finite_k = k.copy()
+    for at in rng.choice(total, 1 + total // 40, replace=False):
+        k[at, rng.integers(G), rng.integers(D)] = rng.choice([-np.inf, np.inf])
+    at = total - new + new // 2    # among the keys that some of the rows do not see
+    k[at, 0, 7], k[at, 0, D - 1] = np.inf, -np.inf
+    for case in ("many", "one"):
+        note(f"attention infinities in K {kv_type} {case} D={D} {new} of {total} scale={scale}")
+        if case == "one":
+            k = finite_k.copy()
+            k[total - new, 0, 11] = np.inf
+        pages = -(-total // page)
+        slots = rng.permutation(pages)[np.arange(total) // page] * page + np.arange(total) % page
+        cache = make_cache(rng, dev, kv_type, pages, page, G, D)
+        held = put(cache, kv_type, page, slots, k, v)
+        out = empty_f32((new, H * D), dev)
+        capi.paged_attention(cache, to_dev(q.reshape(new, -1), dev), out, H, scale, window,
+                             i32(slots[::page] // page, dev), pages, i32([total], dev),
+                             i32([0, new], dev), 1, new)
+        torch.cuda.synchronize()
+        with np.errstate(invalid="ignore"):
+            want = infinite_host(q, *held, pos, window, scale)
+        got = out.cpu().numpy().reshape(want.shape).astype(np.float64)
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+        ok = ~np.isnan(want)
+        assert np.abs(got[ok] - want[ok]).max(initial=0) <= tol
+
+
+def infinite_host(q, k, v, pos, window, scale):
+    """Attention in 64 bits with infinities in K; a row whose weights are all 0 is zero."""
+    H, R, out = q.shape[1], q.shape[1] // k.shape[1], []
+    j = np.arange(len(k))
+    seen = (j <= pos[:, None]) & ((j > pos[:, None] - window) if window else True)
+    for h in range(H):
+        s = np.where(seen, scale * (q[:, h].astype(np.float64) @ k[:, h // R].T), -np.inf)
+        top = s.max(-1, keepdims=True)
+        e = np.exp(s - np.where(top == -np.inf, 0, top))
+        z = e.sum(-1, keepdims=True)
+        out.append(e @ v[:, h // R] / np.where(z == 0, 1, z))
+    return np.stack(out, 1)
+
+
 @pytest.mark.parametrize("kv_type", ("bf16", "int8"))
 @pytest.mark.parametrize("new,total", [(1, 70), (3, 300), (40, 200)])
 @pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-29, 1e-27), (3e-28, 3e-28),
