@@ -902,13 +902,18 @@ struct FewRows {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
-      } else if (careful) {
+      } else if (__builtin_expect(careful, false)) {
+        const AttentionArgs a = fresh_args();
+        const int me = fresh(lane), in = (me & 15) < s.rows ? me & 15 : s.rows - 1;
+        const int tok = (int)a.by_group.of(in);
+        const float* q = a.q + (int64_t)(s.seq.row0 + tok) * a.q_stride +
+                         (int64_t)(s.g * a.group + in - tok * a.group) * D;
 #pragma unroll 1
         for (int j = 0; j < kTiles * 4; ++j) {
           const uint16_t* k = static_cast<const uint16_t*>(a.cache.k) +
                               (j < 4 ? tile[0] : tile[1]) * (kKvTile * D) +
-                              (quad * 4 + j % 4) * 8;
-          const float exact = product_of<T, D>(q - quad * 8, k);
+                              ((me >> 4) * 4 + j % 4) * 8;
+          const float exact = product_of<T, D>(q, k);
 #pragma unroll
           for (int i = 0; i < kTiles * 4; ++i)
             if (i == j && sc[i / 4][i % 4] != sc[i / 4][i % 4])
@@ -1446,7 +1451,8 @@ struct ManyRows {
                 sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
             }
           }
-          if (!kBytes<T> && careful) {
+          if (!kBytes<T> && __builtin_expect(careful, false)) {
+            const AttentionArgs a = fresh_args();
             const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
             const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
             const int token = (int)a.by_group.of(row);
