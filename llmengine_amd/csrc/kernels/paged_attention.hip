@@ -8,8 +8,8 @@
 //
 // fp32 accuracy from 16-bit matrix instructions: q and P go in as sums of 16-bit parts, two
 // f16 (22 bits) against f16 and 8-bit caches, three bf16 (24 bits) against bf16, whose
-// range f16 does not have.  A row of q is first scaled by a power of two to [2^9, 2^10), P
-// carries a factor 2^6, so the f16 parts keep 22 bits down to 2^-13 of the largest.
+// range f16 does not have.  A row of q is first brought near 2^10 (row_scale), P carries a
+// factor 2^6, so the f16 parts keep 22 bits down to 2^-12 of the largest.
 //
 // 8-bit caches: s_j = (q . k_j) ks_j; the V row's scale goes into the exponent, p_j vs_j =
 // 2^(s_j + log2 vs_j - m), with m the maximum of those sums, so that the parts have their
@@ -26,7 +26,8 @@
 // them.  Places that no row sees, which may hold anything, always count as zero.
 //
 // The maximum moves only when a logit passes it by 2^8 (P and l stay far from their limits),
-// so that the rescaling of O is rare.
+// so that the rescaling of O is rare.  It stays finite, so that a logit past 2^128 makes NaN of
+// its row, not a row of no weights.
 //
 // Work is laid out on the device, from the lengths there (the host knows only bounds, and a
 // launch shaped by those would be mostly empty workgroups): units of 64 keys of one (sequence,
@@ -57,6 +58,7 @@ constexpr int kUnit = 64;         // keys of a unit of work, and of a stage in L
 // KV heads of 128) that form takes 37 us against 42 with the tiles of many rows, at 7 over
 // 32768 of 8 bits (2 heads of 64) 22 against 148, and nowhere longer.
 constexpr int kTileRows = 128;    // above kFewRows: four waves of 32 rows share the keys in LDS
+constexpr float kLargest = 0x1.fffffep127f;
 constexpr float kSlack = 8.0f;    // log2 of what a logit may pass the kept maximum by
 constexpr int kDeviceScope = 16;  // cache policy of loads and stores
 
@@ -178,13 +180,21 @@ __device__ __forceinline__ float scale_inverse(float v) {
   return __builtin_amdgcn_rcpf(v > kTinyScale ? v : v <= kTinyScale ? kTinyScale : 1.0f);
 }
 
-// Power of two that brings a row of q to [2^9, 2^10), and its inverse.
-__device__ __forceinline__ void row_scale(uint32_t amax_bits, float* up, float* down) {
+// Factor that brings a row of q to some 2^9 or 2^10, the mantissa of scale log2(e) in it, so that
+// logits in units of log2 are products times a power of two, c: they have no rounding of their
+// own then, and the largest one, less itself, is 0 however large it is.
+__device__ __forceinline__ void row_scale(uint32_t amax_bits, float scale, float* up, float* c) {
   const int ex = (int)(amax_bits >> 23);
+  const int es = __builtin_amdgcn_frexp_expf(scale);  // mantissa in [1/2, 1); 0 of a scale of 0
   int f = 0;  // non-finite rows: any
-  if (amax_bits != 0 && ex != 255) f = 136 - ex < 126 ? 136 - ex : 126;
-  *up = __builtin_bit_cast(float, (uint32_t)(127 + f) << 23);
-  *down = __builtin_bit_cast(float, (uint32_t)(127 - f) << 23);
+  if (amax_bits != 0 && ex != 255) {
+    f = 136 - ex < 126 ? 136 - ex : 126;
+    f = f < es + 126 ? f : es + 126;  // c is at least 2^-126
+  }
+  int e = es - f < 127 ? es - f : 127;
+  e = e > -126 ? e : -126;
+  *up = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(scale) * 1.44269504f, f);
+  *c = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
 }
 
 __device__ __forceinline__ uint32_t magnitude(f32x4 v) {
@@ -860,10 +870,8 @@ struct FewRows {
 #pragma unroll
         for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(with_16(amax, max_bits), max_bits);
-      float up, down;
-      row_scale(amax, &up, &down);
-      if (a.scale < 0.0f) up = -up;
-      c = fmaxf(__builtin_fabsf(a.scale) * 1.44269504f * down, 0x1p-120f);
+      float up;
+      row_scale(amax, a.scale, &up, &c);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[kParts<T>][4];
@@ -917,7 +925,7 @@ struct FewRows {
 #pragma unroll
           for (int i = 0; i < kTiles * 4; ++i)
             if (i == j && sc[i / 4][i % 4] != sc[i / 4][i % 4])
-              sc[i / 4][i % 4] = a.scale < 0.0f ? -exact : exact;
+              sc[i / 4][i % 4] = exact * a.scale;
         }
       }
 
@@ -951,9 +959,9 @@ struct FewRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
       top *= to_log2;
-      if (__any(top > m + kSlack)) {
+      if (__any(top - m > kSlack)) {
         top = with_32(with_16(top, max_float), max_float);
-        const float to = fmaxf(m, top);
+        const float to = fminf(fmaxf(m, top), kLargest);
         const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
         m = to;
         l *= keep;
@@ -1362,10 +1370,8 @@ struct ManyRows {
 #pragma unroll
         for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(amax, max_bits);
-      float up, down;
-      row_scale(amax, &up, &down);
-      if (a.scale < 0.0f) up = -up;
-      c = fmaxf(__builtin_fabsf(a.scale) * 1.44269504f * down, 0x1p-120f);
+      float up;
+      row_scale(amax, a.scale, &up, &c);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[kParts<T>][4];
@@ -1467,7 +1473,7 @@ struct ManyRows {
               const float exact = product_of<T, D>(q, k);
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                if (i == j && sc[i] != sc[i]) sc[i] = a.scale < 0.0f ? -exact : exact;
+                if (i == j && sc[i] != sc[i]) sc[i] = exact * a.scale;
             }
           }
           if (!whole) {
@@ -1484,9 +1490,9 @@ struct ManyRows {
 #pragma unroll
           for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
           top *= to_log2;
-          if (__any(top > m + kSlack)) {
+          if (__any(top - m > kSlack)) {
             top = with_32(top, max_float);
-            const float to = fmaxf(m, top);
+            const float to = fminf(fmaxf(m, top), kLargest);
             const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
             m = to;
             l *= keep;

@@ -870,6 +870,64 @@ def infinite_host(q, k, v, pos, window, scale):
     return np.stack(out, 1)
 
 
+def check_rows_of_any_logits(got, q, k, v, pos, window, scale):
+    """Rows against 64 bits whatever their logits' size.  A logit is off by less than ds (see the
+    module's head), so weights by factors of up to e^ds and a row by expm1(2 ds) of the largest
+    value.  Where that is not small, rows whose two largest logits differ by more than the
+    errors and 30 have the value of one key (the others' weights are below e^-30 each), and
+    rows of which that cannot be said are passed over.  Returns the number of rows compared."""
+    n, H, D = q.shape
+    R, j, compared = H // k.shape[1], np.arange(len(k)), 0
+    want, _ = attention_host(q, k, v, pos, window, scale)
+    seen = (j <= pos[:, None]) & ((j > pos[:, None] - window) if window else True)
+    assert np.isfinite(got).all()
+    for h in range(H):
+        kk, most = k[:, h // R], np.abs(v[:, h // R]).max()
+        s = np.where(seen, scale * (q[:, h].astype(np.float64) @ kk.T), -np.inf)
+        ds = (D + 16) * 2.0 ** -22 * abs(scale) * (np.abs(q[:, h]).astype(np.float64)
+                                                   @ np.abs(kk).T).max(-1)
+        top = np.sort(s, -1)[:, -2:]
+        for i in range(n):
+            tol = most * (np.expm1(2 * min(ds[i], 1)) + 2.0 ** -19
+                          + (len(k) / 8 + 64) * 2.0 ** -23)
+            if ds[i] > 2.0 ** -3:
+                if top[i, 1] - top[i, 0] <= 2 * ds[i] + 30:
+                    continue
+                tol = most * 2.0 ** -20
+            compared += 1
+            assert np.abs(got[i, h] - want[i, h]).max() <= tol, (i, h)
+    return compared
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("H,G,D,new,total,window", [
+    (4, 2, 64, 1, 300, 0), (4, 2, 128, 3, 90, 40), (2, 2, 256, 1, 6000, 0), (4, 2, 96, 60, 200, 0),
+    (4, 1, 128, 70, 300, 0), (2, 1, 256, 40, 130, 0)])
+@pytest.mark.parametrize("scale,size", [(0.11, 1e6), (-0.11, 1e9), (0.11, 1e10), (0.11, 1e15),
+                                        (0.11, 1e30), (5e30, 1.0), (0.0, 1e30), (1e-37, 1e37),
+                                        (1e-30, 1e-30)])
+def test_attention_logits_of_any_size(dev, kv_type, H, G, D, new, total, window, scale, size):
+    """Logits from 0 to 1e33: the largest one's weight is 1 however many bits it has."""
+    import torch
+    note(f"attention logits {kv_type} D={D} {new} of {total} scale={scale} q={size}")
+    rng = np.random.default_rng(new + D)
+    page, pages = 16, -(-total // 16)
+    q = (size * rng.uniform(0.5, 2, (new, H, D)) * rng.choice([-1, 1], (new, H, D))
+         ).astype(np.float32)
+    k, v = (rng.standard_normal((total, G, D)).astype(np.float32) for _ in range(2))
+    slots = rng.permutation(pages)[np.arange(total) // page] * page + np.arange(total) % page
+    cache = make_cache(rng, dev, kv_type, pages, page, G, D)
+    held = put(cache, kv_type, page, slots, k, v)
+    out = empty_f32((new, H * D), dev)
+    capi.paged_attention(cache, to_dev(q.reshape(new, -1), dev), out, H, scale, window,
+                         i32(slots[::page] // page, dev), pages, i32([total], dev),
+                         i32([0, new], dev), 1, new)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(new, H, D).astype(np.float64)
+    compared = check_rows_of_any_logits(got, q, *held, total - new + np.arange(new), window, scale)
+    assert compared >= new * H // 2
+
+
 @pytest.mark.parametrize("kv_type", ("bf16", "int8"))
 @pytest.mark.parametrize("new,total", [(1, 70), (3, 300), (40, 200)])
 @pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-29, 1e-27), (3e-28, 3e-28),
