@@ -8,8 +8,8 @@
 //
 // fp32 accuracy from 16-bit matrix instructions: q and P go in as sums of 16-bit parts, two
 // f16 (22 bits) against f16 and 8-bit caches, three bf16 (24 bits) against bf16, whose
-// range f16 does not have.  A row of q is first brought near 2^10 (row_scale), P carries a
-// factor 2^6, so the f16 parts keep 22 bits down to 2^-12 of the largest.
+// range f16 does not have.  For f16 a row of q is first brought near 2^10 (row_scale) and P
+// carries a factor 2^6, so the parts keep 22 bits down to 2^-12 of the largest.
 //
 // 8-bit caches: s_j = (q . k_j) ks_j; the V row's scale goes into the exponent, p_j vs_j =
 // 2^(s_j + log2 vs_j - m), with m the maximum of those sums, so that the parts have their
@@ -182,13 +182,17 @@ __device__ __forceinline__ float scale_inverse(float v) {
 
 // Factor that brings a row of q to some 2^9 or 2^10, the mantissa of scale log2(e) in it, so that
 // logits in units of log2 are products times a power of two, c: they have no rounding of their
-// own then, and the largest one, less itself, is 0 however large it is.
+// own then, and the largest one, less itself, is 0 however large it is.  Over a bf16 cache it
+// brings it to 2^-12 or 2^-11: the products of 256 elements with the largest values of the cache
+// stay below 2^126, and no part loses bits to the type's range.
+template <KvType T>
 __device__ __forceinline__ void row_scale(uint32_t amax_bits, float scale, float* up, float* c) {
+  constexpr int kTop = T == KvType::kBF16 ? 115 : 136;
   const int ex = (int)(amax_bits >> 23);
   const int es = __builtin_amdgcn_frexp_expf(scale);  // mantissa in [1/2, 1); 0 of a scale of 0
   int f = 0;  // non-finite rows: any
   if (amax_bits != 0 && ex != 255) {
-    f = 136 - ex < 126 ? 136 - ex : 126;
+    f = kTop - ex < 126 ? kTop - ex : 126;
     f = f < es + 126 ? f : es + 126;  // c is at least 2^-126
   }
   int e = es - f < 127 ? es - f : 127;
@@ -871,7 +875,7 @@ struct FewRows {
         for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(with_16(amax, max_bits), max_bits);
       float up;
-      row_scale(amax, a.scale, &up, &c);
+      row_scale<T>(amax, a.scale, &up, &c);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[kParts<T>][4];
@@ -1371,7 +1375,7 @@ struct ManyRows {
         for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(amax, max_bits);
       float up;
-      row_scale(amax, a.scale, &up, &c);
+      row_scale<T>(amax, a.scale, &up, &c);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[kParts<T>][4];

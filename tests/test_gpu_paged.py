@@ -928,6 +928,38 @@ def test_attention_logits_of_any_size(dev, kv_type, H, G, D, new, total, window,
     assert compared >= new * H // 2
 
 
+@pytest.mark.parametrize("D,new,total,window", [(64, 1, 300, 0), (256, 2, 90, 0), (128, 3, 90, 40),
+                                                (64, 60, 200, 0), (96, 40, 100, 0),
+                                                (128, 50, 90, 0), (256, 40, 100, 30)])
+@pytest.mark.parametrize("size,scale", [(-6, 0.11), (-20, 0.11), (-122, 0.11), (-6, 1e-37),
+                                        (-20, 1e-30)])
+def test_attention_largest_keys(dev, D, new, total, window, size, scale):
+    """Keys up to the largest that bf16 holds, with rows of q of 2^size on which all products
+    and logits are finite."""
+    import torch
+    H, G, page = 4, 2, 16
+    note(f"attention largest keys D={D} {new} of {total} q=2^{size} scale={scale}")
+    rng = np.random.default_rng(new + D)
+    q = (2.0 ** size * rng.uniform(0.5, 2, (new, H, D)) * rng.choice([-1, 1], (new, H, D))
+         ).astype(np.float32)
+    k, v = (rng.standard_normal((total, G, D)).astype(np.float32) for _ in range(2))
+    k *= np.float32(2.0 ** 125)
+    k[::7] = np.sign(k[::7]) * np.float32(torch.finfo(torch.bfloat16).max)
+    k[3::7] *= np.float32(2.0 ** -120)
+    pages = -(-total // page)
+    slots = rng.permutation(pages)[np.arange(total) // page] * page + np.arange(total) % page
+    cache = make_cache(rng, dev, "bf16", pages, page, G, D)
+    held = put(cache, "bf16", page, slots, k, v)
+    out = empty_f32((new, H * D), dev)
+    capi.paged_attention(cache, to_dev(q.reshape(new, -1), dev), out, H, scale, window,
+                         i32(slots[::page] // page, dev), pages, i32([total], dev),
+                         i32([0, new], dev), 1, new)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(new, H, D).astype(np.float64)
+    compared = check_rows_of_any_logits(got, q, *held, total - new + np.arange(new), window, scale)
+    assert compared >= new * H // 2
+
+
 @pytest.mark.parametrize("kv_type", ("bf16", "int8"))
 @pytest.mark.parametrize("new,total", [(1, 70), (3, 300), (40, 200)])
 @pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-29, 1e-27), (3e-28, 3e-28),
