@@ -146,7 +146,9 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
  *   out[row][h] = sum_j softmax_j(scale * q . k_j) v_j
  * in fp32 accuracy: q and the probabilities go to the matrix cores as sums of 16-bit
  * parts (two of f16, 22 bits, three of bf16 over a bf16 cache), the cache's values are
- * taken as they are, sums are fp32.  A row that sees no key is zero; a key in a page
+ * taken as they are, sums are fp32: a logit of 2^127 or more makes its row NaN, and sums
+ * of more than 256 values within 2^8 of the largest bf16 may overflow.  A row that sees no
+ * key is zero; a key in a page
  * outside [0, num_pages) counts as hidden, hidden keys and values may hold anything, NaN
  * included; a NaN or an infinity that a row sees reaches that row alone, where a logit of
  * minus infinity is a weight of 0.  Rows outside every sequence are not written.  Long sequences with few rows are split over the keys and joined in a fixed

@@ -74,9 +74,11 @@ template <KvType T>
 constexpr int kParts = T == KvType::kBF16 ? 3 : 2;
 template <KvType T>
 constexpr bool kBytes = T == KvType::kInt8;
-// log2 of P's factor: f16 parts reach further down with it, bf16 parts need none.
+// log2 of P's factor: f16 parts reach further down with 6.  bf16 parts need none for that; with
+// -16, P is at most 2^-8, and sums over 256 keys of the largest bf16 values stay finite (over
+// 65536 where the maximum does not lag).
 template <KvType T>
-constexpr float kHeadroom = T == KvType::kBF16 ? 0.0f : 6.0f;
+constexpr float kHeadroom = T == KvType::kBF16 ? -16.0f : 6.0f;
 
 // Two fp32 values as pairs of 16-bit parts that add up to them.
 template <KvType T>

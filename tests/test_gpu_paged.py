@@ -960,6 +960,35 @@ def test_attention_largest_keys(dev, D, new, total, window, size, scale):
     assert compared >= new * H // 2
 
 
+@pytest.mark.parametrize("D,new,total,window", [(64, 1, 1, 0), (64, 1, 200, 0), (256, 2, 90, 0),
+                                                (128, 3, 90, 40), (64, 60, 200, 0), (96, 40, 100, 1),
+                                                (128, 50, 190, 0), (256, 40, 100, 30)])
+@pytest.mark.parametrize("q_scale", [0.0, 2.0])
+def test_attention_largest_values(dev, D, new, total, window, q_scale):
+    """V as large as bf16 holds, of one sign in a dimension: the mean stays finite, over keys
+    of one weight and of different ones."""
+    import torch
+    H, G, page = 4, 2, 16
+    note(f"attention largest values D={D} {new} of {total} q={q_scale}")
+    rng = np.random.default_rng(new + D)
+    q = (q_scale * rng.standard_normal((new, H, D))).astype(np.float32)
+    k = rng.standard_normal((total, G, D)).astype(np.float32)
+    v = rng.uniform(0.9, 0.999, (total, G, D)) * rng.choice([-1, 1], (G, D))
+    v = (v * torch.finfo(torch.bfloat16).max).astype(np.float32)
+    pages = -(-total // page)
+    slots = rng.permutation(pages)[np.arange(total) // page] * page + np.arange(total) % page
+    cache = make_cache(rng, dev, "bf16", pages, page, G, D)
+    held = put(cache, "bf16", page, slots, k, v)
+    out = empty_f32((new, H * D), dev)
+    capi.paged_attention(cache, to_dev(q.reshape(new, -1), dev), out, H, D ** -0.5, window,
+                         i32(slots[::page] // page, dev), pages, i32([total], dev),
+                         i32([0, new], dev), 1, new)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(new, H, D).astype(np.float64)
+    want, tol = attention_host(q, *held, total - new + np.arange(new), window, D ** -0.5)
+    assert np.isfinite(got).all() and np.abs(got - want).max() <= tol
+
+
 @pytest.mark.parametrize("kv_type", ("bf16", "int8"))
 @pytest.mark.parametrize("new,total", [(1, 70), (3, 300), (40, 200)])
 @pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-29, 1e-27), (3e-28, 3e-28),
