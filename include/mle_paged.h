@@ -30,8 +30,8 @@ extern "C" {
  * with one fp32 scale s = amax * (1/127) per token and KV head (over its head_dim
  * values, for K after the rotation); the value is q * s.  A row that holds a NaN or an
  * infinity gets such a scale, so it reads back as NaN, not as finite numbers.  A V row
- * whose s is at or below 2^-100 is stored as zeros with s = 0: the attention takes no
- * smaller V scales but 0. */
+ * whose s is at or below 2^-64 is stored as zeros with s = 0: the attention takes no
+ * smaller V scales but 0, and V scales up to 2^40 beside that. */
 #define MLE_KV_F16 0
 #define MLE_KV_BF16 1
 #define MLE_KV_INT8 2

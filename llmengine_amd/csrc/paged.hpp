@@ -12,9 +12,9 @@ namespace mle {
 
 constexpr int kKvTile = 16;  // tokens of a cache tile
 // The write stores an 8-bit V row of this scale or a smaller one as zeros of scale 0, which
-// the attention counts as this one: so it has the logarithm of every scale, and a weight of
-// such a row keeps its bits beside rows of scales up to 2^8.
-constexpr float kTinyScale = 0x1p-100f;
+// the attention counts as this one: so it has the logarithm of every scale, and the weights
+// of such rows, down to 2^-24 of the largest, are there beside scales up to 2^40.
+constexpr float kTinyScale = 0x1p-64f;
 // A launch of 256 threads a workgroup has fewer than 2^32 of them.
 constexpr int64_t kMostBlocks = (int64_t(1) << 24) - 1;
 enum class KvType { kF16 = 0, kBF16 = 1, kInt8 = 2 };

@@ -989,14 +989,41 @@ def test_attention_largest_values(dev, D, new, total, window, q_scale):
     assert np.isfinite(got).all() and np.abs(got - want).max() <= tol
 
 
+@pytest.mark.parametrize("new,total", [(1, 500), (3, 300), (40, 400)])
+@pytest.mark.parametrize("size", [1e-17, 1e-6, 1.0, 1e4, 1e7, 1e10, 1e13])
+def test_attention_zero_value_rows(dev, new, total, size):
+    """8-bit V rows of zeros have their weights beside rows of any size (within 2^-16 as in
+    test_attention_relative_error)."""
+    import torch
+    H, G, D, page = 4, 2, 64, 16
+    note(f"attention zero V rows {new} of {total} beside {size}")
+    rng = np.random.default_rng(total)
+    q = (2 * rng.standard_normal((new, H, D))).astype(np.float32)
+    k, v = (rng.standard_normal((total, G, D)).astype(np.float32) for _ in range(2))
+    v *= np.float32(size)
+    v[rng.random(total) < 0.7] = 0
+    pages = -(-total // page)
+    slots = rng.permutation(pages)[np.arange(total) // page] * page + np.arange(total) % page
+    cache = make_cache(rng, dev, "int8", pages, page, G, D)
+    held = put(cache, "int8", page, slots, k, v)
+    out = empty_f32((new, H * D), dev)
+    capi.paged_attention(cache, to_dev(q.reshape(new, -1), dev), out, H, D ** -0.5, 0,
+                         i32(slots[::page] // page, dev), pages, i32([total], dev),
+                         i32([0, new], dev), 1, new)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(new, H, D).astype(np.float64)
+    want, _ = attention_host(q, *held, total - new + np.arange(new), 0, D ** -0.5)
+    assert np.linalg.norm(got - want) <= 2.0 ** -16 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("kv_type", ("bf16", "int8"))
 @pytest.mark.parametrize("new,total", [(1, 70), (3, 300), (40, 200)])
-@pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-29, 1e-27), (3e-28, 3e-28),
-                                      (1e-33, 1e-20), (1e-33, 1.0)])
+@pytest.mark.parametrize("low,high", [(1e-30, 1e-30), (1e-19, 1e-16), (3e-17, 3e-17),
+                                      (1e-33, 1e-10), (1e-33, 1.0)])
 def test_tiny_values(dev, kv_type, new, total, low, high):
     """V rows of any size down to 1e-33, written and attended: what comes out is what the cache
     holds, within 2^-16 of it (see test_attention_relative_error), and 8-bit rows of scales at
-    or below 2^-100 are zeros of scale 0."""
+    or below 2^-64 are zeros of scale 0."""
     import torch
     note(f"tiny values {kv_type} {new} of {total} from {low} to {high}")
     H, G, D, page = 4, 2, 64, 16
@@ -1020,8 +1047,8 @@ def test_tiny_values(dev, kv_type, new, total, low, high):
                       cells_of(cache, pages, page, G, D))
     if kv_type == "int8":
         cells, scale = stored_host(v, kv_type)
-        zero = scale <= 2.0 ** -100
-        assert zero.any() == (low < 1e-28)
+        zero = scale <= 2.0 ** -64
+        assert zero.any() == (low < 1e-18)
         cells[zero], scale[zero] = 0, 0
         assert torch.equal(cv, cells) and torch.equal(vs, scale)
     held = [x.double().numpy() * (1 if s is None else s.double().numpy()[..., None])
