@@ -813,6 +813,27 @@ def test_steps_together(dev, kv_type):
     assert count.item() == pages - sum(-(-int(n) // page) for n in lens)
 
 
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("H,G,D,prompts", [(8, 4, 96, 40), (8, 4, 128, 40), (8, 4, 256, 0),
+                                           (8, 4, 256, 30), (4, 4, 256, 90), (40, 2, 256, 20)])
+def test_attention_many_segments_of_a_workgroup(dev, kv_type, H, G, D, prompts):
+    """More tiles than workgroups at every head size, so that each goes through several of few
+    rows, of many, and of both in turn, with what one keeps for the next."""
+    rng = np.random.default_rng(D + prompts)
+    n = 700 if D < 256 else 400
+    lens = [(int(rng.integers(0, 3)), int(rng.integers(2, 90))) for _ in range(n)]
+    for b in rng.choice(n, prompts, replace=False):
+        new = int(rng.integers(10, 70))
+        lens[b] = (new, new + int(rng.integers(0, 60)))
+    lens[5], lens[n - 2] = (1, 1500), (90, 700)
+    note(f"attention many segments {kv_type} H={H} G={G} D={D} prompts={prompts}")
+    b = Batch(dev, kv_type, H, G, D, 16, lens)
+    out = b.run()
+    b.check(out)
+    got = out.cpu().numpy().reshape(b.want.shape).astype(np.float64)
+    assert np.linalg.norm(got - b.want) <= 2.0 ** -16 * np.linalg.norm(b.want)
+
+
 @pytest.mark.parametrize("kv_type", ("f16", "bf16"))
 @pytest.mark.parametrize("H,G,D,new,total,window", [
     (4, 2, 64, 1, 70, 0), (4, 2, 128, 3, 300, 0), (3, 1, 256, 5, 90, 40), (2, 2, 96, 2, 5000, 0),
