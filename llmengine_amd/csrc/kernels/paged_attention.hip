@@ -165,11 +165,28 @@ template <KvType T, int D>
 __device__ __forceinline__ float product_of(const float* q, const uint16_t* k) {
   float sum = 0.0f;
 #pragma unroll 1
-  for (int d = 0; d < D; ++d) {
-    const float term = q[d] * value_of<T>(k[d / 8 * (kKvTile * 8) + d % 8]);
-    if (term - term != 0.0f) sum += term;
+  for (int d = 0; d < D; d += 8) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(k + d * kKvTile);
+    const f32x4 v[2] = {*reinterpret_cast<const f32x4*>(q + d),
+                        *reinterpret_cast<const f32x4*>(q + d + 4)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float term = v[i / 4][i % 4] * value_of<T>(w[i / 2] >> (i % 2 * 16) & 0xffffu);
+      if (term - term != 0.0f) sum += term;
+    }
   }
   return sum;
+}
+
+// Bits where one of a lane's values of q, as parts, is not finite.
+template <KvType T, int N>
+__device__ __forceinline__ uint32_t non_finite(const u32x4 (&q)[N]) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int kk = 0; kk < N; ++kk)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= non_finite<T>(q[kk][i]);
+  return bits;
 }
 
 // The scale of a V row as its logarithm and inverse; a scale of 0 counts as a tiny one (the
@@ -693,6 +710,19 @@ struct FewRows {
     load_v(a, lane, tile, n.x);
   }
 
+  // Whether the lane's row of q is finite; lanes l, l + 16 .. have it, and all of them come here.
+  static __device__ __forceinline__ bool finite_q(const u32x4 (&qp)[kParts<T>][KK]) {
+    return with_32(with_16(non_finite<T>(qp[0]), max_bits), max_bits) == 0;
+  }
+  static __device__ __forceinline__ bool any_nan(const float (&sc)[kTiles][4]) {
+    bool nan = false;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nan |= sc[t][i] != sc[t][i];
+    return nan;
+  }
+
   static __device__ __forceinline__ u32x4 operand(Raw r) {
     if constexpr (kBytes<T>) return quants_to_f16(r);
     else return r;
@@ -916,7 +946,7 @@ struct FewRows {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
-      } else if (__builtin_expect(careful, false)) {
+      } else if (__builtin_expect(careful && __any(any_nan(sc) & finite_q(qp)), false)) {
         const AttentionArgs a = fresh_args();
         const int me = fresh(lane), in = (me & 15) < s.rows ? me & 15 : s.rows - 1;
         const int tok = (int)a.by_group.of(in);
@@ -1072,7 +1102,8 @@ struct FewRows {
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
-      if (!careful && __any(zero != zero)) {
+      // A row of q that is not finite is NaN either way.
+      if (!careful && __any(zero != zero) && __any((zero != zero) & finite_q(qp))) {
         careful = true;
         n.started = false;
         goto again;
@@ -1229,6 +1260,17 @@ struct ManyRows {
     __syncthreads();
     const u32x4 all = *reinterpret_cast<const u32x4*>(flags);
     return uniform((int)(all.x | all.y | all.z | all.w)) != 0;
+  }
+
+  // Whether the lane's row of q is finite; lanes l and l + 32 have it, and both come here.
+  static __device__ __forceinline__ bool finite_q(const u32x4 (&qp)[kParts<T>][KK]) {
+    return with_32(non_finite<T>(qp[0]), max_bits) == 0;
+  }
+  static __device__ __forceinline__ bool any_nan(const f32x16& sc) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) nan |= sc[i] != sc[i];
+    return nan;
   }
 
   static __device__ __forceinline__ bool has_chunk(int chunk) {
@@ -1463,7 +1505,8 @@ struct ManyRows {
                 sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
             }
           }
-          if (!kBytes<T> && __builtin_expect(careful, false)) {
+          if (!kBytes<T> &&
+              __builtin_expect(careful && __any(any_nan(sc) & finite_q(qp)), false)) {
             const AttentionArgs a = fresh_args();
             const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
             const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
@@ -1565,7 +1608,10 @@ struct ManyRows {
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
-      if (!careful && any_of(zero != zero, wave, smem + kFlags + 16)) {
+      // A row of q that is not finite is NaN either way.
+      bool odd = false;
+      if (__any(zero != zero)) odd = (zero != zero) & finite_q(qp);
+      if (!careful && any_of(odd, wave, smem + kFlags + 16)) {
         careful = true;
         m = -INFINITY;
         l = 0.0f;

@@ -17,7 +17,7 @@ import math
 import numpy as np
 import pytest
 
-from helpers import empty_f32, note, own_stream, to_dev
+from helpers import empty_f32, note, own_stream, slower_by, to_dev
 from llmengine_amd import capi
 
 pytestmark = pytest.mark.gpu
@@ -875,6 +875,22 @@ def test_attention_infinities_in_k(dev, kv_type, H, G, D, new, total, window, sc
         np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
         ok = ~np.isnan(want)
         assert np.abs(got[ok] - want[ok]).max(initial=0) <= tol
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("lens", [[(1, 3000)] * 8, [(500, 3000)]])
+def test_attention_of_non_finite_q_takes_no_longer(dev, kv_type, lens):
+    """Rows whose q is not finite are NaN after one pass over the keys: twice the time of finite
+    ones is well above what they take, a pass more with products one by one far above that."""
+    import torch
+    note(f"attention time of NaN in q {kv_type} {lens}")
+    b = Batch(dev, kv_type, 8, 2, 128, 32, lens)
+    bad = b.q.clone()
+    bad.view(b.T, 8, 128)[::3, ::2, 5] = float("nan")
+    out = [empty_f32(b.q.shape, dev) for _ in range(2)]
+    assert slower_by(lambda: b.run(out=out[0], q=bad), lambda: b.run(out=out[1])) <= 2
+    got = torch.isnan(out[0].view(b.T, 8, 128))
+    assert got[::3, ::2].all() and not got[1::3].any() and not got[:, 1::2].any()
 
 
 def infinite_host(q, k, v, pos, window, scale):
