@@ -867,10 +867,8 @@ struct FewRows {
 
     // Steps of this wave: s.k0 + (wave + 4 i) kStep.
     const int hi = last_key(s);
-    bool careful = false, go_on = false;
     Loads& x = n.x;
     Tiles& held = n.held;
-  again:
     // Ahead of the first keys, which wait for the table.
     const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
                      (int64_t)(s.g * a.group + row - token * a.group) * D + quad * 8;
@@ -890,7 +888,7 @@ struct FewRows {
     int64_t tile[kTiles];
     take(held, 0, tile);
     int then_page = 0;
-    if (!careful) go_on = find_next();
+    const bool go_on = find_next();
     if (go_on) {
       const Segment t = uniform(*then);
       then_page = page_of(a, t, key_of(lane, t.k0 + wave * kStep));
@@ -922,180 +920,185 @@ struct FewRows {
 
     float m = -INFINITY, l = 0.0f;
     f32x4 acc[DB] = {};
-    for (; base < hi; base += 4 * kStep) {
-      // The step's keys are whole for every row, or each lane's keys are checked.
-      const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
-      const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0;
+    // Twice in the code, so that the first pass has nothing of what only the second does.
+    auto pass = [&](auto second) __attribute__((always_inline)) {
+      constexpr bool careful = decltype(second)::value;
+      for (; base < hi; base += 4 * kStep) {
+        // The step's keys are whole for every row, or each lane's keys are checked.
+        const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
+        const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0;
 
-      float sc[kTiles][4];
+        float sc[kTiles][4];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        f32x4 r = {};
+        for (int t = 0; t < kTiles; ++t) {
+          f32x4 r = {};
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const u32x4 kf = operand(x.k[t][kk]);
+          for (int kk = 0; kk < KK; ++kk) {
+            const u32x4 kf = operand(x.k[t][kk]);
 #pragma unroll
-          for (int p = 0; p < kParts<T>; ++p) r = mfma16<T>(kf, qp[p][kk], r);
+            for (int p = 0; p < kParts<T>; ++p) r = mfma16<T>(kf, qp[p][kk], r);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[t][i] = r[i];
         }
+        if constexpr (kBytes<T>) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[t][i] = r[i];
-      }
-      if constexpr (kBytes<T>) {
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
+        } else if (careful && __any(any_nan(sc) & finite_q(qp))) {
+          const AttentionArgs a = fresh_args();
+          const int me = fresh(lane), in = (me & 15) < s.rows ? me & 15 : s.rows - 1;
+          const int tok = (int)a.by_group.of(in);
+          const float* q = a.q + (int64_t)(s.seq.row0 + tok) * a.q_stride +
+                           (int64_t)(s.g * a.group + in - tok * a.group) * D;
+#pragma unroll 1
+          for (int j = 0; j < kTiles * 4; ++j) {
+            const uint16_t* k = static_cast<const uint16_t*>(a.cache.k) +
+                                (j < 4 ? tile[0] : tile[1]) * (kKvTile * D) +
+                                ((me >> 4) * 4 + j % 4) * 8;
+            const float exact = product_of<T, D>(q, k);
+#pragma unroll
+            for (int i = 0; i < kTiles * 4; ++i)
+              if (i == j && sc[i / 4][i % 4] != sc[i / 4][i % 4])
+                sc[i / 4][i % 4] = exact * a.scale;
+          }
+        }
+
+        // The next step's K goes out before the softmax.
+        const bool more = base + 4 * kStep < hi;
+        const int64_t tile_now[2] = {tile[0], tile[1]};
+        if (more) {
+          if (++at == kAhead) {
+            held = look_up(a, s, lane, base + 4 * kStep);
+            bad = __ballot(held.bad);
+            at = 0;
+          }
+          take(held, at, tile);
+          load_k(a, lane, tile, x);
+        }
+
+        if (!whole) {
+          const int from = fresh(base + quad * 4 - mine.lo);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool seen = (uint32_t)(from + t * kKvTile + i) < width && !(bad_now >> t & 1);
+              sc[t][i] = seen ? sc[t][i] : -INFINITY;
+            }
+        }
+        const float to_log2 = kBytes<T> ? 1.0f : c;
+        float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
-      } else if (__builtin_expect(careful && __any(any_nan(sc) & finite_q(qp)), false)) {
-        const AttentionArgs a = fresh_args();
-        const int me = fresh(lane), in = (me & 15) < s.rows ? me & 15 : s.rows - 1;
-        const int tok = (int)a.by_group.of(in);
-        const float* q = a.q + (int64_t)(s.seq.row0 + tok) * a.q_stride +
-                         (int64_t)(s.g * a.group + in - tok * a.group) * D;
-#pragma unroll 1
-        for (int j = 0; j < kTiles * 4; ++j) {
-          const uint16_t* k = static_cast<const uint16_t*>(a.cache.k) +
-                              (j < 4 ? tile[0] : tile[1]) * (kKvTile * D) +
-                              ((me >> 4) * 4 + j % 4) * 8;
-          const float exact = product_of<T, D>(q, k);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
+        top *= to_log2;
+        if (__any(top - m > kSlack)) {
+          top = with_32(with_16(top, max_float), max_float);
+          const float to = fminf(fmaxf(m, top), kLargest);
+          const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
+          m = to;
+          l *= keep;
 #pragma unroll
-          for (int i = 0; i < kTiles * 4; ++i)
-            if (i == j && sc[i / 4][i % 4] != sc[i / 4][i % 4])
-              sc[i / 4][i % 4] = exact * a.scale;
+          for (int db = 0; db < DB; ++db) acc[db] *= keep;
         }
-      }
-
-      // The next step's K goes out before the softmax.
-      const bool more = base + 4 * kStep < hi;
-      const int64_t tile_now[2] = {tile[0], tile[1]};
-      if (more) {
-        if (++at == kAhead) {
-          held = look_up(a, s, lane, base + 4 * kStep);
-          bad = __ballot(held.bad);
-          at = 0;
-        }
-        take(held, at, tile);
-        load_k(a, lane, tile, x);
-      }
-
-      if (!whole) {
-        const int from = fresh(base + quad * 4 - mine.lo);
+        const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool seen = (uint32_t)(from + t * kKvTile + i) < width && !(bad_now >> t & 1);
-            sc[t][i] = seen ? sc[t][i] : -INFINITY;
+            const float p = exp2_of(__builtin_fmaf(sc[t][i], to_log2, -ref));
+            if constexpr (kBytes<T>) l = __builtin_fmaf(p, scale_inverse(x.vs[t][i]), l);
+            else l += p;
+            sc[t][i] = p;
           }
-      }
-      const float to_log2 = kBytes<T> ? 1.0f : c;
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
-      top *= to_log2;
-      if (__any(top - m > kSlack)) {
-        top = with_32(with_16(top, max_float), max_float);
-        const float to = fminf(fmaxf(m, top), kLargest);
-        const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
-        m = to;
-        l *= keep;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] *= keep;
-      }
-      const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = exp2_of(__builtin_fmaf(sc[t][i], to_log2, -ref));
-          if constexpr (kBytes<T>) l = __builtin_fmaf(p, scale_inverse(x.vs[t][i]), l);
-          else l += p;
-          sc[t][i] = p;
-        }
 
-      bool odd = false;  // a value of V that is not finite
-      if constexpr (!kBytes<T>) {
-        if (careful || base < s.span.lo || base + kStep > s.span.hi || bad_now != 0) {
-          // Values that no row sees count as zero.
-          const int from = fresh(base + (lane >> 4 & 1) * 4);
-          uint32_t found = 0;
+        bool odd = false;  // a value of V that is not finite
+        if constexpr (!kBytes<T>) {
+          if (careful || base < s.span.lo || base + kStep > s.span.hi || bad_now != 0) {
+            // Values that no row sees count as zero.
+            const int from = fresh(base + (lane >> 4 & 1) * 4);
+            uint32_t found = 0;
 #pragma unroll
-          for (int u = 0; u < kTiles / 2; ++u) {
-            const int t = 2 * u + (lane >> 5);
+            for (int u = 0; u < kTiles / 2; ++u) {
+              const int t = 2 * u + (lane >> 5);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int key = from + t * kKvTile + (w >> 1) * 8 + (w & 1) * 2;
-              const bool tile_ok = !(bad_now >> t & 1);
-              const uint32_t keep =
-                  (tile_ok && key >= s.span.lo && key < s.span.hi ? 0x0000ffffu : 0u) |
-                  (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
+              for (int w = 0; w < 4; ++w) {
+                const int key = from + t * kKvTile + (w >> 1) * 8 + (w & 1) * 2;
+                const bool tile_ok = !(bad_now >> t & 1);
+                const uint32_t keep =
+                    (tile_ok && key >= s.span.lo && key < s.span.hi ? 0x0000ffffu : 0u) |
+                    (tile_ok && key + 1 >= s.span.lo && key + 1 < s.span.hi ? 0xffff0000u : 0u);
 #pragma unroll
-              for (int db = 0; db < DB; ++db) {
-                x.v[u][db][w] &= keep;
-                found |= non_finite<T>(x.v[u][db][w]);
+                for (int db = 0; db < DB; ++db) {
+                  x.v[u][db][w] &= keep;
+                  found |= non_finite<T>(x.v[u][db][w]);
+                }
               }
             }
-          }
-          odd = careful && __any(found != 0);
-          if (odd)
+            odd = careful && __any(found != 0);
+            if (odd)
 #pragma unroll
-            for (int u = 0; u < kTiles / 2; ++u)
+              for (int u = 0; u < kTiles / 2; ++u)
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                  for (int w = 0; w < 4; ++w)
+                    x.v[u][db][w] &= ~((non_finite<T>(x.v[u][db][w]) >> 15) * 0xffffu);
+          }
+        }
+
+        // P as the right operand: tokens 4 h' .. of a pair of tiles, by one exchange of the
+        // wave's halves.
+#pragma unroll
+        for (int u = 0; u < kTiles / 2; ++u) {
+          uint32_t w[2][2][kParts<T>];  // [tile][pair][part]
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              split2<T>(sc[2 * u + t][2 * h], sc[2 * u + t][2 * h + 1], &w[t][h][0], 1);
+          u32x4 pp[kParts<T>];
+#pragma unroll
+          for (int p = 0; p < kParts<T>; ++p) {
+            const auto e0 = __builtin_amdgcn_permlane32_swap(w[0][0][p], w[1][0][p], false, false);
+            const auto e1 = __builtin_amdgcn_permlane32_swap(w[0][1][p], w[1][1][p], false, false);
+            pp[p] = u32x4{(uint32_t)e0[0], (uint32_t)e1[0], (uint32_t)e0[1], (uint32_t)e1[1]};
+          }
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const u32x4 vf = operand(x.v[u][db]);
+#pragma unroll
+            for (int p = 0; p < kParts<T>; ++p) acc[db] = mfma16<T>(vf, pp[p], acc[db]);
+          }
+        }
+        if constexpr (!kBytes<T>) {
+          if (odd) {  // values that are not finite, for the rows that see them
+#pragma unroll 1
+            for (int j = 0; j < kStep; ++j) {
+              const int64_t ti = j < kKvTile ? tile_now[0] : tile_now[1];
+              const int tok = j % kKvTile, key = base + j;
+              const bool seen =
+                  (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
+              const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
+                                  (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
 #pragma unroll
               for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
-                  x.v[u][db][w] &= ~((non_finite<T>(x.v[u][db][w]) >> 15) * 0xffffu);
-        }
-      }
-
-      // P as the right operand: tokens 4 h' .. of a pair of tiles, by one exchange of the
-      // wave's halves.
-#pragma unroll
-      for (int u = 0; u < kTiles / 2; ++u) {
-        uint32_t w[2][2][kParts<T>];  // [tile][pair][part]
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            split2<T>(sc[2 * u + t][2 * h], sc[2 * u + t][2 * h + 1], &w[t][h][0], 1);
-        u32x4 pp[kParts<T>];
-#pragma unroll
-        for (int p = 0; p < kParts<T>; ++p) {
-          const auto e0 = __builtin_amdgcn_permlane32_swap(w[0][0][p], w[1][0][p], false, false);
-          const auto e1 = __builtin_amdgcn_permlane32_swap(w[0][1][p], w[1][1][p], false, false);
-          pp[p] = u32x4{(uint32_t)e0[0], (uint32_t)e1[0], (uint32_t)e0[1], (uint32_t)e1[1]};
-        }
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const u32x4 vf = operand(x.v[u][db]);
-#pragma unroll
-          for (int p = 0; p < kParts<T>; ++p) acc[db] = mfma16<T>(vf, pp[p], acc[db]);
-        }
-      }
-      if constexpr (!kBytes<T>) {
-        if (odd) {  // values that are not finite, for the rows that see them
-#pragma unroll 1
-          for (int j = 0; j < kStep; ++j) {
-            const int64_t ti = j < kKvTile ? tile_now[0] : tile_now[1];
-            const int tok = j % kKvTile, key = base + j;
-            const bool seen =
-                (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
-            const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
-                                (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t v = p[(db * 16 + quad * 4 + i) * 8];
-                if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
-              }
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t v = p[(db * 16 + quad * 4 + i) * 8];
+                  if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
+                }
+            }
           }
         }
+        if (more) load_v(a, lane, tile, x);
       }
-      if (more) load_v(a, lane, tile, x);
-    }
+    };
+    pass(std::false_type{});
     if constexpr (!kBytes<T>) {
       float zero = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
@@ -1103,10 +1106,18 @@ struct FewRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
       // A row of q that is not finite is NaN either way.
-      if (!careful && __any(zero != zero) && __any((zero != zero) & finite_q(qp))) {
-        careful = true;
-        n.started = false;
-        goto again;
+      if (__any(zero != zero) && __any((zero != zero) & finite_q(qp))) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = f32x4{};
+        base = s.k0 + wave * kStep;
+        held = look_up(a, s, lane, base);
+        start(a, s, lane, wave, n);
+        bad = __ballot(held.bad);
+        at = 0;
+        take(held, 0, tile);
+        pass(std::true_type{});
       }
     }
     // The next segment's first loads are under way while this one is joined and written.
@@ -1457,151 +1468,153 @@ struct ManyRows {
 
     float m = -INFINITY, l = 0.0f;
     f32x16 acc[DB] = {};
-    bool careful = false;
-  again:
-    int buf = 0;
-    for (int base = s.k0; base < hi; base += kUnit, buf ^= 1) {
-      const uint32_t bad_now = (uint32_t)(bad >> (at * kTilesUnit)) & ((1u << kTilesUnit) - 1);
-      const int64_t tiles_now = held.index;
-      const int at_now = at;
-      uint8_t* stage = smem + buf * kStage;
-      wait_for_loads();  // this wave's loads of the stage
-      __syncthreads();   // everyone's; and the other stage's readers are done
-      const bool more = base + kUnit < hi;
-      if (more) {
-        if (++at == 64 / kTilesUnit) look_up(base + kUnit);
-        issue(a, tid, held.index, at * kTilesUnit, smem + (buf ^ 1) * kStage, staged);
-      }
-      bool odd = false;
-      if (!kBytes<T> && (careful || base < s.span.lo || base + kUnit > s.span.hi || bad_now != 0))
-        odd = any_of(clear_v(s, tid, base, bad_now, careful, stage), wave, smem + kFlags);
+    // Twice in the code, so that the first pass has nothing of what only the second does.
+    auto pass = [&](auto second) __attribute__((always_inline)) {
+      constexpr bool careful = decltype(second)::value;
+      int buf = 0;
+      for (int base = s.k0; base < hi; base += kUnit, buf ^= 1) {
+        const uint32_t bad_now = (uint32_t)(bad >> (at * kTilesUnit)) & ((1u << kTilesUnit) - 1);
+        const int64_t tiles_now = held.index;
+        const int at_now = at;
+        uint8_t* stage = smem + buf * kStage;
+        wait_for_loads();  // this wave's loads of the stage
+        __syncthreads();   // everyone's; and the other stage's readers are done
+        const bool more = base + kUnit < hi;
+        if (more) {
+          if (++at == 64 / kTilesUnit) look_up(base + kUnit);
+          issue(a, tid, held.index, at * kTilesUnit, smem + (buf ^ 1) * kStage, staged);
+        }
+        bool odd = false;
+        if (!kBytes<T> && (careful || base < s.span.lo || base + kUnit > s.span.hi || bad_now != 0))
+          odd = any_of(clear_v(s, tid, base, bad_now, careful, stage), wave, smem + kFlags);
 
-      if (live && base < ours.hi && base + kUnit > ours.lo) {
+        if (live && base < ours.hi && base + kUnit > ours.lo) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {  // 32 keys: two tiles
-          const int from_key = base + u * 32;
-          if (from_key >= ours.hi || from_key + 32 <= ours.lo) continue;
-          const bool whole =
-              from_key >= ours.lo_all && from_key + 32 <= ours.hi_all && bad_now == 0;
-          f32x16 sc = {};
+          for (int u = 0; u < 2; ++u) {  // 32 keys: two tiles
+            const int from_key = base + u * 32;
+            if (from_key >= ours.hi || from_key + 32 <= ours.lo) continue;
+            const bool whole =
+                from_key >= ours.lo_all && from_key + 32 <= ours.hi_all && bad_now == 0;
+            f32x16 sc = {};
 #pragma unroll
-          for (int from = 0; from < KK; from += FB) {
-            read_k(stage, u, from);
+            for (int from = 0; from < KK; from += FB) {
+              read_k(stage, u, from);
 #pragma unroll
-            for (int n = 0; n < FB; ++n)
+              for (int n = 0; n < FB; ++n)
 #pragma unroll
-              for (int p = 0; p < kParts<T>; ++p) sc = mfma32<T>(f[n], qp[p][from + n], sc);
-          }
-          read_v(stage, u, 0);  // on its way during the softmax
-          const float* ks = reinterpret_cast<const float*>(smem + kScales) + buf * 3 * kUnit +
-                            u * 32 + half * 4;
-          if constexpr (kBytes<T>) {
-#pragma unroll
-            for (int b4 = 0; b4 < 4; ++b4) {
-              const f32x4 k4 = *reinterpret_cast<const f32x4*>(ks + b4 * 8);
-              const f32x4 l4 = *reinterpret_cast<const f32x4*>(ks + kUnit + b4 * 8);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
+                for (int p = 0; p < kParts<T>; ++p) sc = mfma32<T>(f[n], qp[p][from + n], sc);
             }
-          }
-          if (!kBytes<T> &&
-              __builtin_expect(careful && __any(any_nan(sc) & finite_q(qp)), false)) {
-            const AttentionArgs a = fresh_args();
-            const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
-            const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
-            const int token = (int)a.by_group.of(row);
-            const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                             (int64_t)(s.g * a.group + row - token * a.group) * D;
-#pragma unroll 1
-            for (int j = 0; j < 16; ++j) {
-              const int key = (j >> 2) * 8 + (me >> 3 & 4) + (j & 3);
-              const uint16_t* k = reinterpret_cast<const uint16_t*>(
-                                      stage + (2 * u + key / kKvTile) * kTileBytes) +
-                                  key % kKvTile * 8;
-              const float exact = product_of<T, D>(q, k);
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (i == j && sc[i] != sc[i]) sc[i] = exact * a.scale;
-            }
-          }
-          if (!whole) {
-            const int from = fresh(base + half * 4 - mine.lo);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const bool seen = (uint32_t)(from + u * 32 + (i >> 2) * 8 + (i & 3)) < width &&
-                                !(bad_now >> (2 * u + (i >> 3)) & 1);
-              sc[i] = seen ? sc[i] : -INFINITY;
-            }
-          }
-          const float to_log2 = kBytes<T> ? 1.0f : c;
-          float top = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
-          top *= to_log2;
-          if (__any(top - m > kSlack)) {
-            top = with_32(top, max_float);
-            const float to = fminf(fmaxf(m, top), kLargest);
-            const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
-            m = to;
-            l *= keep;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] *= keep;
-          }
-          const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
-          uint32_t w[kParts<T>][8];
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float p0 = exp2_of(__builtin_fmaf(sc[i], to_log2, -ref));
-            const float p1 = exp2_of(__builtin_fmaf(sc[i + 1], to_log2, -ref));
+            read_v(stage, u, 0);  // on its way during the softmax
+            const float* ks = reinterpret_cast<const float*>(smem + kScales) + buf * 3 * kUnit +
+                              u * 32 + half * 4;
             if constexpr (kBytes<T>) {
-              const f32x2 inv = *reinterpret_cast<const f32x2*>(ks + 2 * kUnit + (i >> 2) * 8 +
-                                                                (i & 3));
-              l = __builtin_fmaf(p0, inv.x, l);
-              l = __builtin_fmaf(p1, inv.y, l);
-            } else {
-              l += p0;
-              l += p1;
+#pragma unroll
+              for (int b4 = 0; b4 < 4; ++b4) {
+                const f32x4 k4 = *reinterpret_cast<const f32x4*>(ks + b4 * 8);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ks + kUnit + b4 * 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
+              }
             }
-            split2<T>(p0, p1, &w[0][i / 2], 8);
-          }
-#pragma unroll
-          for (int from = 0; from < KK; from += FB) {
-            if (from > 0) read_v(stage, u, from);
-#pragma unroll
-            for (int n = 0; n < FB; ++n) {
-              const int t = (from + n) / DB, db = (from + n) % DB;
-#pragma unroll
-              for (int p = 0; p < kParts<T>; ++p)
-                acc[db] = mfma32<T>(
-                    f[n], u32x4{w[p][4 * t], w[p][4 * t + 1], w[p][4 * t + 2], w[p][4 * t + 3]},
-                    acc[db]);
-            }
-          }
-        }
-        if constexpr (!kBytes<T>) {
-          if (odd) {  // values that are not finite, for the rows that see them
+            if (!kBytes<T> && careful && __any(any_nan(sc) & finite_q(qp))) {
+              const AttentionArgs a = fresh_args();
+              const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
+              const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
+              const int token = (int)a.by_group.of(row);
+              const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                               (int64_t)(s.g * a.group + row - token * a.group) * D;
 #pragma unroll 1
-            for (int j = 0; j < kUnit; ++j) {
-              const int tok = j % kKvTile, key = base + j;
-              const bool seen =
-                  (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
-              const int64_t ti = lane_of(tiles_now, at_now * kTilesUnit + j / kKvTile);
-              const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
-                                  (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
+              for (int j = 0; j < 16; ++j) {
+                const int key = (j >> 2) * 8 + (me >> 3 & 4) + (j & 3);
+                const uint16_t* k = reinterpret_cast<const uint16_t*>(
+                                        stage + (2 * u + key / kKvTile) * kTileBytes) +
+                                    key % kKvTile * 8;
+                const float exact = product_of<T, D>(q, k);
 #pragma unroll
-              for (int db = 0; db < DB; ++db)
+                for (int i = 0; i < 16; ++i)
+                  if (i == j && sc[i] != sc[i]) sc[i] = exact * a.scale;
+              }
+            }
+            if (!whole) {
+              const int from = fresh(base + half * 4 - mine.lo);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const uint32_t v = p[(db * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * 8];
-                  if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
-                }
+              for (int i = 0; i < 16; ++i) {
+                const bool seen = (uint32_t)(from + u * 32 + (i >> 2) * 8 + (i & 3)) < width &&
+                                  !(bad_now >> (2 * u + (i >> 3)) & 1);
+                sc[i] = seen ? sc[i] : -INFINITY;
+              }
+            }
+            const float to_log2 = kBytes<T> ? 1.0f : c;
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
+            top *= to_log2;
+            if (__any(top - m > kSlack)) {
+              top = with_32(top, max_float);
+              const float to = fminf(fmaxf(m, top), kLargest);
+              const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
+              m = to;
+              l *= keep;
+#pragma unroll
+              for (int db = 0; db < DB; ++db) acc[db] *= keep;
+            }
+            const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
+            uint32_t w[kParts<T>][8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float p0 = exp2_of(__builtin_fmaf(sc[i], to_log2, -ref));
+              const float p1 = exp2_of(__builtin_fmaf(sc[i + 1], to_log2, -ref));
+              if constexpr (kBytes<T>) {
+                const f32x2 inv = *reinterpret_cast<const f32x2*>(ks + 2 * kUnit + (i >> 2) * 8 +
+                                                                  (i & 3));
+                l = __builtin_fmaf(p0, inv.x, l);
+                l = __builtin_fmaf(p1, inv.y, l);
+              } else {
+                l += p0;
+                l += p1;
+              }
+              split2<T>(p0, p1, &w[0][i / 2], 8);
+            }
+#pragma unroll
+            for (int from = 0; from < KK; from += FB) {
+              if (from > 0) read_v(stage, u, from);
+#pragma unroll
+              for (int n = 0; n < FB; ++n) {
+                const int t = (from + n) / DB, db = (from + n) % DB;
+#pragma unroll
+                for (int p = 0; p < kParts<T>; ++p)
+                  acc[db] = mfma32<T>(
+                      f[n], u32x4{w[p][4 * t], w[p][4 * t + 1], w[p][4 * t + 2], w[p][4 * t + 3]},
+                      acc[db]);
+              }
+            }
+          }
+          if constexpr (!kBytes<T>) {
+            if (odd) {  // values that are not finite, for the rows that see them
+#pragma unroll 1
+              for (int j = 0; j < kUnit; ++j) {
+                const int tok = j % kKvTile, key = base + j;
+                const bool seen =
+                    (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
+                const int64_t ti = lane_of(tiles_now, at_now * kTilesUnit + j / kKvTile);
+                const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
+                                    (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const uint32_t v = p[(db * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * 8];
+                    if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
+                  }
+              }
             }
           }
         }
+        if (more) commit(tid, smem, buf ^ 1, staged);
       }
-      if (more) commit(tid, smem, buf ^ 1, staged);
-    }
+    };
+    pass(std::false_type{});
     if constexpr (!kBytes<T>) {
       float zero = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
@@ -1611,8 +1624,7 @@ struct ManyRows {
       // A row of q that is not finite is NaN either way.
       bool odd = false;
       if (__any(zero != zero)) odd = (zero != zero) & finite_q(qp);
-      if (!careful && any_of(odd, wave, smem + kFlags + 16)) {
-        careful = true;
+      if (any_of(odd, wave, smem + kFlags + 16)) {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
@@ -1620,7 +1632,7 @@ struct ManyRows {
         look_up(s.k0);
         __syncthreads();
         if (s.k0 < hi) issue(a, tid, held.index, 0, smem, staged);
-        goto again;
+        pass(std::true_type{});
       }
     }
     l = with_32(l, sum_float);
