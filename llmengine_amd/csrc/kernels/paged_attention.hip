@@ -570,6 +570,11 @@ __device__ __forceinline__ uint32_t slot_at(const Shared& sh, const Segment& s, 
   return (uint32_t)((s.first + part) * 2 + (part == 0)) * (uint32_t)sh.slot_floats * 4u;
 }
 
+// The same in every lane, and told so: an access goes lane by lane otherwise.
+__device__ __forceinline__ uint32_t same_slot_at(const Shared& sh, const Segment& s, int part) {
+  return (uint32_t)uniform((int)slot_at(sh, s, part));
+}
+
 __device__ __forceinline__ bool last_to_arrive(const Shared& sh, const Segment& s, int* shared) {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_waitcnt(0);  // this wave's part has reached the coherence point
@@ -1160,7 +1165,7 @@ struct FewRows {
 
     if (s.parts > 1) {
       const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
-      const uint32_t to = slot_at(sh, s, s.part);
+      const uint32_t to = same_slot_at(sh, s, s.part);
       if (r < s.rows) {
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
@@ -1184,7 +1189,7 @@ struct FewRows {
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) {
           // Past the last part: that one again, not used.
-          const uint32_t from = slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
+          const uint32_t from = same_slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
           ml[p] = load_part2(rs, r * 8, from + kMl);
 #pragma unroll
           for (int i = 0; i < NQ; ++i)
@@ -1382,8 +1387,13 @@ struct ManyRows {
     return found;
   }
 
-  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh,
-                                             uint8_t* smem) {
+  // The segment's keys for the tile's rows: their maxima m, sums l (a share of it a lane) and
+  // products acc.  Says whether a sum is not finite; the second pass, a function of its own so
+  // that the first has none of what only it needs, then does the same with values that are not
+  // finite row by row.
+  template <bool kSecond>
+  static __device__ __forceinline__ bool attend(const Segment& s, uint8_t* smem, float& m,
+                                                float& l, f32x16 (&acc)[DB]) {
     const AttentionArgs a = fresh_args();
     const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
     const int half = lane >> 5;
@@ -1466,156 +1476,157 @@ struct ManyRows {
             stage + v_at + (2 * u + (from + n) / DB) * kTileBytes + (from + n) % DB * 512);
     };
 
-    float m = -INFINITY, l = 0.0f;
-    f32x16 acc[DB] = {};
-    // Twice in the code, so that the first pass has nothing of what only the second does.
-    auto pass = [&](auto second) __attribute__((always_inline)) {
-      constexpr bool careful = decltype(second)::value;
-      int buf = 0;
-      for (int base = s.k0; base < hi; base += kUnit, buf ^= 1) {
-        const uint32_t bad_now = (uint32_t)(bad >> (at * kTilesUnit)) & ((1u << kTilesUnit) - 1);
-        const int64_t tiles_now = held.index;
-        const int at_now = at;
-        uint8_t* stage = smem + buf * kStage;
-        wait_for_loads();  // this wave's loads of the stage
-        __syncthreads();   // everyone's; and the other stage's readers are done
-        const bool more = base + kUnit < hi;
-        if (more) {
-          if (++at == 64 / kTilesUnit) look_up(base + kUnit);
-          issue(a, tid, held.index, at * kTilesUnit, smem + (buf ^ 1) * kStage, staged);
-        }
-        bool odd = false;
-        if (!kBytes<T> && (careful || base < s.span.lo || base + kUnit > s.span.hi || bad_now != 0))
-          odd = any_of(clear_v(s, tid, base, bad_now, careful, stage), wave, smem + kFlags);
-
-        if (live && base < ours.hi && base + kUnit > ours.lo) {
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {  // 32 keys: two tiles
-            const int from_key = base + u * 32;
-            if (from_key >= ours.hi || from_key + 32 <= ours.lo) continue;
-            const bool whole =
-                from_key >= ours.lo_all && from_key + 32 <= ours.hi_all && bad_now == 0;
-            f32x16 sc = {};
-#pragma unroll
-            for (int from = 0; from < KK; from += FB) {
-              read_k(stage, u, from);
-#pragma unroll
-              for (int n = 0; n < FB; ++n)
-#pragma unroll
-                for (int p = 0; p < kParts<T>; ++p) sc = mfma32<T>(f[n], qp[p][from + n], sc);
-            }
-            read_v(stage, u, 0);  // on its way during the softmax
-            const float* ks = reinterpret_cast<const float*>(smem + kScales) + buf * 3 * kUnit +
-                              u * 32 + half * 4;
-            if constexpr (kBytes<T>) {
-#pragma unroll
-              for (int b4 = 0; b4 < 4; ++b4) {
-                const f32x4 k4 = *reinterpret_cast<const f32x4*>(ks + b4 * 8);
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ks + kUnit + b4 * 8);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
-              }
-            }
-            if (!kBytes<T> && careful && __any(any_nan(sc) & finite_q(qp))) {
-              const AttentionArgs a = fresh_args();
-              const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
-              const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
-              const int token = (int)a.by_group.of(row);
-              const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                               (int64_t)(s.g * a.group + row - token * a.group) * D;
-#pragma unroll 1
-              for (int j = 0; j < 16; ++j) {
-                const int key = (j >> 2) * 8 + (me >> 3 & 4) + (j & 3);
-                const uint16_t* k = reinterpret_cast<const uint16_t*>(
-                                        stage + (2 * u + key / kKvTile) * kTileBytes) +
-                                    key % kKvTile * 8;
-                const float exact = product_of<T, D>(q, k);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  if (i == j && sc[i] != sc[i]) sc[i] = exact * a.scale;
-              }
-            }
-            if (!whole) {
-              const int from = fresh(base + half * 4 - mine.lo);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const bool seen = (uint32_t)(from + u * 32 + (i >> 2) * 8 + (i & 3)) < width &&
-                                  !(bad_now >> (2 * u + (i >> 3)) & 1);
-                sc[i] = seen ? sc[i] : -INFINITY;
-              }
-            }
-            const float to_log2 = kBytes<T> ? 1.0f : c;
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
-            top *= to_log2;
-            if (__any(top - m > kSlack)) {
-              top = with_32(top, max_float);
-              const float to = fminf(fmaxf(m, top), kLargest);
-              const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
-              m = to;
-              l *= keep;
-#pragma unroll
-              for (int db = 0; db < DB; ++db) acc[db] *= keep;
-            }
-            const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
-            uint32_t w[kParts<T>][8];
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float p0 = exp2_of(__builtin_fmaf(sc[i], to_log2, -ref));
-              const float p1 = exp2_of(__builtin_fmaf(sc[i + 1], to_log2, -ref));
-              if constexpr (kBytes<T>) {
-                const f32x2 inv = *reinterpret_cast<const f32x2*>(ks + 2 * kUnit + (i >> 2) * 8 +
-                                                                  (i & 3));
-                l = __builtin_fmaf(p0, inv.x, l);
-                l = __builtin_fmaf(p1, inv.y, l);
-              } else {
-                l += p0;
-                l += p1;
-              }
-              split2<T>(p0, p1, &w[0][i / 2], 8);
-            }
-#pragma unroll
-            for (int from = 0; from < KK; from += FB) {
-              if (from > 0) read_v(stage, u, from);
-#pragma unroll
-              for (int n = 0; n < FB; ++n) {
-                const int t = (from + n) / DB, db = (from + n) % DB;
-#pragma unroll
-                for (int p = 0; p < kParts<T>; ++p)
-                  acc[db] = mfma32<T>(
-                      f[n], u32x4{w[p][4 * t], w[p][4 * t + 1], w[p][4 * t + 2], w[p][4 * t + 3]},
-                      acc[db]);
-              }
-            }
-          }
-          if constexpr (!kBytes<T>) {
-            if (odd) {  // values that are not finite, for the rows that see them
-#pragma unroll 1
-              for (int j = 0; j < kUnit; ++j) {
-                const int tok = j % kKvTile, key = base + j;
-                const bool seen =
-                    (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
-                const int64_t ti = lane_of(tiles_now, at_now * kTilesUnit + j / kKvTile);
-                const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
-                                    (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
-#pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const uint32_t v = p[(db * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * 8];
-                    if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
-                  }
-              }
-            }
-          }
-        }
-        if (more) commit(tid, smem, buf ^ 1, staged);
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+    int buf = 0;
+    for (int base = s.k0; base < hi; base += kUnit, buf ^= 1) {
+      const uint32_t bad_now = (uint32_t)(bad >> (at * kTilesUnit)) & ((1u << kTilesUnit) - 1);
+      const int64_t tiles_now = held.index;
+      const int at_now = at;
+      uint8_t* stage = smem + buf * kStage;
+      wait_for_loads();  // this wave's loads of the stage
+      __syncthreads();   // everyone's; and the other stage's readers are done
+      const bool more = base + kUnit < hi;
+      if (more) {
+        if (++at == 64 / kTilesUnit) look_up(base + kUnit);
+        issue(a, tid, held.index, at * kTilesUnit, smem + (buf ^ 1) * kStage, staged);
       }
-    };
-    pass(std::false_type{});
-    if constexpr (!kBytes<T>) {
+      bool odd = false;
+      if (!kBytes<T> && (kSecond || base < s.span.lo || base + kUnit > s.span.hi || bad_now != 0))
+      {
+        const bool found = clear_v(s, tid, base, bad_now, kSecond, stage);
+        if constexpr (kSecond) odd = any_of(found, wave, smem + kFlags);
+        else __syncthreads();
+      }
+
+      if (live && base < ours.hi && base + kUnit > ours.lo) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // 32 keys: two tiles
+          const int from_key = base + u * 32;
+          if (from_key >= ours.hi || from_key + 32 <= ours.lo) continue;
+          const bool whole =
+              from_key >= ours.lo_all && from_key + 32 <= ours.hi_all && bad_now == 0;
+          f32x16 sc = {};
+#pragma unroll
+          for (int from = 0; from < KK; from += FB) {
+            read_k(stage, u, from);
+#pragma unroll
+            for (int n = 0; n < FB; ++n)
+#pragma unroll
+              for (int p = 0; p < kParts<T>; ++p) sc = mfma32<T>(f[n], qp[p][from + n], sc);
+          }
+          read_v(stage, u, 0);  // on its way during the softmax
+          const float* ks = reinterpret_cast<const float*>(smem + kScales) + buf * 3 * kUnit +
+                            u * 32 + half * 4;
+          if constexpr (kBytes<T>) {
+#pragma unroll
+            for (int b4 = 0; b4 < 4; ++b4) {
+              const f32x4 k4 = *reinterpret_cast<const f32x4*>(ks + b4 * 8);
+              const f32x4 l4 = *reinterpret_cast<const f32x4*>(ks + kUnit + b4 * 8);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
+            }
+          }
+          if (!kBytes<T> && kSecond && __any(any_nan(sc) & finite_q(qp))) {
+            const AttentionArgs a = fresh_args();
+            const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
+            const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
+            const int token = (int)a.by_group.of(row);
+            const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                             (int64_t)(s.g * a.group + row - token * a.group) * D;
+#pragma unroll 1
+            for (int j = 0; j < 16; ++j) {
+              const int key = (j >> 2) * 8 + (me >> 3 & 4) + (j & 3);
+              const uint16_t* k = reinterpret_cast<const uint16_t*>(
+                                      stage + (2 * u + key / kKvTile) * kTileBytes) +
+                                  key % kKvTile * 8;
+              const float exact = product_of<T, D>(q, k);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (i == j && sc[i] != sc[i]) sc[i] = exact * a.scale;
+            }
+          }
+          if (!whole) {
+            const int from = fresh(base + half * 4 - mine.lo);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const bool seen = (uint32_t)(from + u * 32 + (i >> 2) * 8 + (i & 3)) < width &&
+                                !(bad_now >> (2 * u + (i >> 3)) & 1);
+              sc[i] = seen ? sc[i] : -INFINITY;
+            }
+          }
+          const float to_log2 = kBytes<T> ? 1.0f : c;
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
+          top *= to_log2;
+          if (__any(top - m > kSlack)) {
+            top = with_32(top, max_float);
+            const float to = fminf(fmaxf(m, top), kLargest);
+            const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
+            m = to;
+            l *= keep;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= keep;
+          }
+          const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
+          uint32_t w[kParts<T>][8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float p0 = exp2_of(__builtin_fmaf(sc[i], to_log2, -ref));
+            const float p1 = exp2_of(__builtin_fmaf(sc[i + 1], to_log2, -ref));
+            if constexpr (kBytes<T>) {
+              const f32x2 inv = *reinterpret_cast<const f32x2*>(ks + 2 * kUnit + (i >> 2) * 8 +
+                                                                (i & 3));
+              l = __builtin_fmaf(p0, inv.x, l);
+              l = __builtin_fmaf(p1, inv.y, l);
+            } else {
+              l += p0;
+              l += p1;
+            }
+            split2<T>(p0, p1, &w[0][i / 2], 8);
+          }
+#pragma unroll
+          for (int from = 0; from < KK; from += FB) {
+            if (from > 0) read_v(stage, u, from);
+#pragma unroll
+            for (int n = 0; n < FB; ++n) {
+              const int t = (from + n) / DB, db = (from + n) % DB;
+#pragma unroll
+              for (int p = 0; p < kParts<T>; ++p)
+                acc[db] = mfma32<T>(
+                    f[n], u32x4{w[p][4 * t], w[p][4 * t + 1], w[p][4 * t + 2], w[p][4 * t + 3]},
+                    acc[db]);
+            }
+          }
+        }
+        if constexpr (!kBytes<T>) {
+          if (odd) {  // values that are not finite, for the rows that see them
+#pragma unroll 1
+            for (int j = 0; j < kUnit; ++j) {
+              const int tok = j % kKvTile, key = base + j;
+              const bool seen =
+                  (uint32_t)(key - mine.lo) < width && !(bad_now >> (j / kKvTile) & 1);
+              const int64_t ti = lane_of(tiles_now, at_now * kTilesUnit + j / kKvTile);
+              const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
+                                  (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
+#pragma unroll
+              for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const uint32_t v = p[(db * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * 8];
+                  if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
+                }
+            }
+          }
+        }
+      }
+      if (more) commit(tid, smem, buf ^ 1, staged);
+    }
+    if constexpr (!kBytes<T> && !kSecond) {
       float zero = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -1624,24 +1635,28 @@ struct ManyRows {
       // A row of q that is not finite is NaN either way.
       bool odd = false;
       if (__any(zero != zero)) odd = (zero != zero) & finite_q(qp);
-      if (any_of(odd, wave, smem + kFlags + 16)) {
-        m = -INFINITY;
-        l = 0.0f;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
-        look_up(s.k0);
-        __syncthreads();
-        if (s.k0 < hi) issue(a, tid, held.index, 0, smem, staged);
-        pass(std::true_type{});
-      }
+      return any_of(odd, wave, smem + kFlags + 16);
     }
+    return false;
+  }
+
+  static __device__ __forceinline__ void run(const Segment& s, const Shared& sh,
+                                             uint8_t* smem) {
+    float m, l;
+    f32x16 acc[DB];
+    if (attend<false>(s, smem, m, l, acc)) attend<true>(s, smem, m, l, acc);
     l = with_32(l, sum_float);
+    const AttentionArgs a = fresh_args();
+    const int tid = fresh_tid(), half = tid >> 5 & 1;
+    const int wrow = (tid >> 6) * 32 + (tid & 31);
+    const int row = s.r0 + (wrow < s.rows ? wrow : s.rows - 1);
+    const int token = (int)a.by_group.of(row);
 
     if (s.parts > 1) {
       constexpr uint32_t kMl = kTileRows * D * 4;
       const int at = fresh(tid);
       const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
-      const uint32_t to = slot_at(sh, s, s.part);
+      const uint32_t to = same_slot_at(sh, s, s.part);
       if (wrow < s.rows) {
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -1667,7 +1682,7 @@ struct ManyRows {
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) {
           // Past the last part: that one again, with no weight.
-          const uint32_t from = slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
+          const uint32_t from = same_slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
           ml[p] = load_part2(rs, at * 8, from + kMl);
 #pragma unroll
           for (int q = 0; q < kQuads; ++q)
