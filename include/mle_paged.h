@@ -30,8 +30,8 @@ extern "C" {
  * with one fp32 scale s = amax * (1/127) per token and KV head (over its head_dim
  * values, for K after the rotation); the value is q * s.  A row that holds a NaN or an
  * infinity gets such a scale, so it reads back as NaN, not as finite numbers.  A V row
- * whose s is at or below 2^-64 is stored as zeros with s = 0: the attention takes no
- * smaller V scales but 0, and V scales up to 2^40 beside that. */
+ * whose s is at or below 2^-64 is stored as zeros with s = 0; the attention reads V scales
+ * above 2^-64 and 0.  Rows of zeros have their weights beside V scales up to 2^40. */
 #define MLE_KV_F16 0
 #define MLE_KV_BF16 1
 #define MLE_KV_INT8 2
@@ -89,8 +89,8 @@ typedef struct mle_paged_cache {
  * a counter of the per-stream workspace (before a graph is captured: 256 bytes and 32
  * counters, or what mle_paged_attention_workspace_size says for as many rows).
  * Errors: NULL pointers, sequences or sizes <= 0, tokens < 0 -> InvalidArgument;
- * sequences * max_pages or num_pages * page_size above 2^31 - 1 -> Unsupported.
- * tokens == 0: positions and slots may be NULL.
+ * sequences * max_pages or num_pages * page_size above 2^31 - 1, num_pages, max_pages or
+ * tokens of 2^30 or more -> Unsupported.  tokens == 0: positions and slots may be NULL.
  */
 int mle_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int sequences,
                    int32_t* block_table, int max_pages, int page_size, int num_pages,
@@ -118,10 +118,10 @@ int mle_rope_table(float* table, int positions, int rope_dim, double theta,
  * of q [heads][head_dim], k and v [kv_heads][head_dim] starts at r * its stride (floats;
  * a multiple of 4, at least the row's size), so q, k and v may lie in one buffer of a
  * fused Linear.  With (c, s) = rope[positions[r]][i], elements (a, b) of a pair become
- * (a c - b s, a s + b c), each formed exactly and rounded once to fp32; elements from
- * rope_dim on stay.  rope NULL: no rotation, positions may be NULL.  Rotated q goes to
- * q_out (may be q with the same stride); k and v, in the cache's type, to slots[r].
- * A slot outside the cache (-1) writes none; two rows of one slot race.  A position
+ * (a c - b s, a s + b c): exact products, their sum in 64 bits, then rounded to fp32;
+ * elements from rope_dim on stay.  rope NULL: no rotation, positions may be NULL.  Rotated
+ * q goes to q_out (may be q with the same stride); k and v, in the cache's type, to
+ * slots[r].  A slot outside the cache (-1) writes none; two rows of one slot race.  A position
  * outside [0, rope_positions) has no rotation: its q_out row is zero and nothing of it
  * is cached.
  * Errors: NULL pointers, tokens < 0, sizes <= 0, misalignment -> InvalidArgument;
@@ -147,12 +147,12 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
  * in fp32 accuracy: q and the probabilities go to the matrix cores as sums of 16-bit
  * parts (two of f16, 22 bits, three of bf16 over a bf16 cache), the cache's values are
  * taken as they are, sums are fp32: a logit of 2^127 or more makes its row NaN, and sums
- * of more than 256 values within 2^8 of the largest bf16 may overflow.  A row that sees no
- * key is zero; a key in a page
- * outside [0, num_pages) counts as hidden, hidden keys and values may hold anything, NaN
- * included; a NaN or an infinity that a row sees reaches that row alone, where a logit of
- * minus infinity is a weight of 0.  Rows outside every sequence are not written.  Long sequences with few rows are split over the keys and joined in a fixed
- * order: deterministic run to run.
+ * of more than 256 values within 2^8 of the largest bf16 may overflow.
+ * A row that sees no key is zero.  A key in a page outside [0, num_pages) counts as hidden;
+ * hidden keys and values may hold anything, NaN included.  A NaN or an infinity that a row
+ * sees reaches that row alone, where a logit of minus infinity is a weight of 0.  Rows
+ * outside every sequence are not written.  Long sequences with few rows are split over the
+ * keys and joined in a fixed order: deterministic run to run.
  * Row strides in floats, multiples of 4; out must not overlap q unless it is q with the
  * same stride.  `sequences` may include some without new rows.
  * Errors: NULL pointers, sizes <= 0, tokens < 0, heads not a multiple of kv_heads, a

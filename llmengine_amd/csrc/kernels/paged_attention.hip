@@ -21,9 +21,14 @@
 // registers: with them kept the 128-wide kernels spilled.
 //
 // A value of V that is not finite must reach the rows that see it and no others, and 0 times
-// it, or the parts of P times it, are NaN.  Where a sum comes out non-finite, the keys are gone
-// through again, with such values taken out of the product and added to the rows that see
-// them.  Places that no row sees, which may hold anything, always count as zero.
+// it, or the parts of P times it, are NaN; so are the parts of q times an infinity in K, whose
+// product may be minus infinity, a weight of 0.  Where a sum comes out non-finite, the keys are
+// gone through again, with such values of V taken out of the product and added to the rows that
+// see them, and with products that came out NaN made again one by one.  Places that no row
+// sees, which may hold anything, always count as zero.  The second pass is code of its own,
+// which the first keeps nothing for: together in one loop, the 128-wide kernels spilled and 4
+// prompts of 512 took 39.7 us instead of 38.7.  With infinities in two of three pages of V the
+// 2048 tokens over 10240 below take 5.8 ms, with one in K of every token 33.
 //
 // The maximum moves only when a logit passes it by 2^8 (P and l stay far from their limits),
 // so that the rescaling of O is rare.  It stays finite, so that a logit past 2^128 makes NaN of
@@ -35,16 +40,21 @@
 // of short and long sequences, decoding and prompts.  A tile cut by a run's end is joined,
 // in order, by the workgroup that finishes last.
 //
-// What bounds it (MI355X; a large copy reaches 4.9 TB/s, a large f16 product 1.15 PFLOP/s):
-//   decoding: HBM.  32 sequences of up to 4096 tokens, 32 heads of 128, 181 us = 5.3 TB/s;
+// What bounds it (MI355X; 2 GiB are read at 6.1 TB/s, a large f16 product reaches 1.32
+// PFLOP/s in a row of calls):
+//   decoding: HBM.  32 sequences of up to 4096 tokens, 32 heads of 128, 182 us = 5.3 TB/s;
 //     8 of up to 32768 of 8 bits, 8 KV heads, 64 us = 4.1 TB/s, of which about 10 are the
 //     beginning and 5 the joins.
-//   prompts: the matrix cores at the clock they leave.  2048 tokens over 10240, 32 heads over
-//     8, 546-585 us = 1.06-1.13 PFLOP/s of parts; 55% of 1.07 million cycles.  Priorities
-//     of the waves, a second accumulator for the low parts, and loads issued between the
-//     matrix instructions changed nothing.
+//   prompts: power, and the softmax beside the products.  2048 tokens over 10240, 32 heads
+//     over 8, 555-575 us = 1.08-1.11 PFLOP/s of parts in a row of calls; the first 40 after a
+//     rest 600-780, while the card settles its clock (a library product of 8192^3 likewise,
+//     0.83 and 0.85-1.07 ms).  The matrix cores are busy in 56% of 1.06 million cycles (in 69%
+//     of the library's), with 4.2 vector instructions to each of theirs; of the two waves of a
+//     SIMD 1.65 are there on average, which wait for it 43% of their time, for memory and
+//     barriers 19%.  Priorities of the waves, a second accumulator for the low parts, and loads
+//     issued between the matrix instructions changed nothing.
 //   short calls: a chain of latencies (lengths, run, page table, keys) of 6 us for few rows
-//     and 12 for many: 129 tokens of 14 heads 8.9 us.
+//     and 12 for many: 129 tokens of 14 heads 8.7 us.
 #include "../launch.hpp"
 #include "../paged.hpp"
 #include "../q8_0_device.hpp"

@@ -1,9 +1,9 @@
 // paged_write.hip -- rotary embedding of a step's q and k rows, and the write of k and v
 // into the paged cache.
 //
-// A pair (x, y) turns to (x c - y s, x s + y c).  Both products are exact in 64 bits, so
-// one fma each gives the exact result rounded once: the same bits whatever the order, and
-// with them the same 8-bit quants, which a last-bit difference could move by a whole step.
+// A pair (x, y) turns to (x c - y s, x s + y c).  Both products are exact in 64 bits; their
+// sum is rounded to 64 bits (an fma each) and then to 32: the same bits whatever the order,
+// and with them the same 8-bit quants, which a last-bit difference could move by a whole step.
 // The 64-bit work hides behind memory: the kernel is bound by HBM (q in and out above
 // all).  MI355X: 8192 tokens of 32 heads of 128 over 8 KV heads into 8 bits 84 us, 4.25 TB/s
 // of the 4.9 that a large copy reaches; 1531 tokens of 14 heads of 64 6.4 us and 32 tokens of
