@@ -34,7 +34,7 @@ EXPORTED = ("mle_q8_0_abi_version", "mle_q8_0_linear", "mle_q8_0_linear_ex",
             "mle_paged_attention_workspace_size")
 
 KV_TYPES = {"f16": 0, "bf16": 1, "int8": 2}
-ROPE_MODES = {"pairs": 0, "halves": 1, "none": 0}
+ROPE_MODES = {"pairs": 0, "halves": 1, "none": -1}  # none: without a table, refused with one
 
 OP_LINEAR, OP_LINEAR_SWIGLU, OP_LINEAR_MULTI, OP_MATMUL = 0, 1, 2, 3
 

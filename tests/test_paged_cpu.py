@@ -172,6 +172,13 @@ def test_workspace_size():
             capi.paged_attention_workspace_size(cache(), **a)
 
 
+def test_rotation_table_without_a_mode():
+    """rope_mode "none" says that nothing turns: with a table it is refused, not taken for pairs."""
+    got, msg = write(rope_mode="none")
+    assert got == INVALID and "rope_mode" in msg, (got, msg)
+    assert write(rope=None, rope_mode="none", tokens=0)[0] == 0
+
+
 @pytest.mark.parametrize("head_dim,heads,kv_heads,tokens", [
     (64, 4, 2, (1 << 32) // (8 * 6)), (96, 2, 1, (1 << 32) // (16 * 3) + 1),
     (128, 8, 8, (1 << 32) // (16 * 20) + 1), (256, 8, 8, 1 << 23), (256, 1, 1, 1 << 26)])
