@@ -138,6 +138,23 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
                        const int32_t* slots, int tokens, hipStream_t stream);
 
 /*
+ * mle_paged_kv_write with a norm of every head of q and k in the same pass (the norms that
+ * models have between the q/k/v Linear and the rotation): a head's row x becomes
+ *   x w / sqrt(mean(x^2) + eps), w = q_norm or k_norm [head_dim] fp32, 16-byte aligned,
+ * over all of its head_dim elements, and is then rotated; in 64 bits throughout, rounded to
+ * fp32 once.  v has no norm.
+ * Errors: those of mle_paged_kv_write; NULL or misaligned norms, an eps that is negative or
+ * not finite -> InvalidArgument.
+ */
+int mle_paged_kv_write_normed(const mle_paged_cache* cache, const float* q, int q_stride,
+                              float* q_out, int q_out_stride, int heads, const float* k,
+                              int k_stride, const float* v, int v_stride, const float* q_norm,
+                              const float* k_norm, float eps, const float* rope,
+                              int rope_positions, int rope_dim, int rope_mode,
+                              const int32_t* positions, const int32_t* slots, int tokens,
+                              hipStream_t stream);
+
+/*
  * Attention of the new tokens over the cache.  Rows cu_tokens[b] .. cu_tokens[b+1] of q
  * [tokens][heads][head_dim] are the last new_b of the kv_lens[b] tokens of sequence b, so
  * row i stands at position p = kv_lens[b] - new_b + i and sees the keys j <= p, with
@@ -173,6 +190,72 @@ int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stri
                         hipStream_t stream);
 int mle_paged_attention_workspace_size(const mle_paged_cache* cache, int heads, int sequences,
                                        int tokens, size_t* bytes, size_t* counters);
+
+/*
+ * Speculative decoding: the new rows of a request are a tree of drafted tokens, which one
+ * step checks together.  The plan gives them slots one after the other, as ever; a step is
+ *
+ *   mle_paged_plan              new_lens[b] = nodes of the tree
+ *   mle_paged_kv_write(_normed) with the nodes' own positions: cached tokens + depth
+ *   mle_paged_tree_attention    a node sees the cached tokens, its ancestors and itself
+ *   mle_token_logprobs_f32      the drafted tokens under the model's logits
+ *   mle_paged_kv_keep           the accepted path's tokens move behind the cached ones
+ */
+
+/* Words of 64 nodes that a row's mask has at most. */
+#define MLE_TREE_MAX_WORDS 64
+
+/*
+ * mle_paged_attention for trees.  tree_mask is [tokens][mask_words] 64-bit words, 8-byte
+ * aligned: bit j of row r says that the row sees the j-th new row of its request (in a tree
+ * its ancestors and itself).  Nodes past 64 mask_words are seen by none, bits past the
+ * request's rows do not count.  The cached tokens before the new ones are seen by every row;
+ * with window > 0 only the keys j > p - window, p = row_positions[r] (held to the positions
+ * of the request's new rows, which a node's are); among the new rows the mask alone decides.
+ * trees [sequences]: requests with 0 there are not trees, their rows see as in
+ * mle_paged_attention and their masks are not read; NULL: all are trees.  row_positions may
+ * be NULL where window is 0.
+ * All else, accuracy, hidden keys, strides, workspace (mle_paged_attention_workspace_size)
+ * and errors, is mle_paged_attention's; a NULL or misaligned tree_mask, mask_words <= 0, a
+ * window without row_positions -> InvalidArgument, mask_words above MLE_TREE_MAX_WORDS
+ * -> Unsupported.
+ */
+int mle_paged_tree_attention(const mle_paged_cache* cache, const float* q, int q_stride,
+                             float* out, int out_stride, int heads, float scale, int window,
+                             const int32_t* block_table, int max_pages, const int32_t* kv_lens,
+                             const int32_t* cu_tokens, int sequences, int tokens,
+                             const uint64_t* tree_mask, int mask_words,
+                             const int32_t* row_positions, const int32_t* trees,
+                             hipStream_t stream);
+
+/*
+ * After a step of trees: of the n new rows of request b (cu_tokens, behind its
+ * base = kv_lens[b] - n cached tokens) the rows keep[b][0] < keep[b][1] < ..., keep_counts[b]
+ * of them, stay, as the tokens base, base + 1, ...: their K and V (and scales) move there in
+ * the caches of all `layers`, host array `caches`, which share type and sizes.  keep is
+ * [sequences][keep_stride]; keep_counts[b] < 0 keeps every row (a prompt's chunk).  A path
+ * ends before an entry that is not above the one before it or not a row of the request, and at
+ * keep_stride entries.  What the cache holds past the kept tokens is left as it was.
+ *   kept_lens[b] = base + the rows kept (may be the cached_lens that the plan read, not
+ *     kv_lens).  Of a request that the plan refused (granted[b] == 0) it is not written; one
+ *     with kv_lens[b] < n keeps kv_lens[b] and nothing moves.
+ *   The pages that held only rows which did not stay go on top of the free stack, in the order
+ *   of the requests and of the table row, which is left as it was; free_count_out (may be
+ *   free_count) = the pages then free, at most num_pages.  free_pages NULL: no pages go
+ *   back, the counts may be NULL (a second group of layers).
+ * A token in a page outside [0, num_pages) neither moves nor is written over.  One launch for
+ * up to 64 layers; no workspace.  Deterministic.
+ * Errors: NULL or misaligned pointers, sizes <= 0, kept_lens == kv_lens -> InvalidArgument;
+ * caches of different type or sizes -> ShapeMismatch; more than 31 bits of max_pages *
+ * page_size or sequences * max_pages, or as many threads as a launch does not hold (64 for
+ * each layer, request and KV head) -> Unsupported.
+ */
+int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* block_table,
+                      int max_pages, const int32_t* kv_lens, const int32_t* cu_tokens,
+                      const int32_t* granted, int sequences, const int32_t* keep,
+                      int keep_stride, const int32_t* keep_counts, int32_t* kept_lens,
+                      int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
+                      hipStream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -240,6 +240,31 @@ int mle_top_tokens_f32(const float* logits, int rows, int n, int top_n, float te
                        int32_t* ids, float* probs, hipStream_t stream);
 
 /*
+ * Log probabilities of given tokens under logits rows, with the rows' entropies and top
+ * alternatives, in one pass over the logits.  With x = logits * (1 / temperature) where
+ * temperature > 0 and != 1, else x = logits:
+ *   logprobs[r][j] = log p_r(tokens[r][j]) = x_t - log sum_i e^(x_i), j < tokens_per_row;
+ *     a token outside [0, n) has no probability: -Inf;
+ *   entropy[r] = -sum_i p_i log p_i (natural logarithms; a logit of -Inf adds nothing);
+ *   top_ids, top_logprobs[r][j], j < min(top_n, n): the tokens of largest probability and
+ *     their log probabilities, largest first, ties to the lower id.
+ * A row whose maximum is not finite or that holds a NaN is the uniform distribution 1 / n,
+ * as mle_top_tokens_f32 has it.  Sums are of 64 bits: log p is good to fp32 rounding also
+ * where it is near 0.  tokens_per_row 0, entropy NULL and top_n 0 leave a part out.
+ * Takes the per-stream workspace; mle_token_logprobs_workspace_size says how much any call of
+ * up to these sizes takes (mle_workspace_reserve, before a graph is captured).
+ * Errors: NULL pointers of a part asked for, rows or n <= 0, tokens_per_row or top_n < 0
+ * -> InvalidArgument; rows above 65535, top_n above 128, an n that mle_top_tokens_f32 does
+ * not take for this top_n -> Unsupported.
+ */
+int mle_token_logprobs_f32(const float* logits, int rows, int n, float temperature,
+                           const int32_t* tokens, int tokens_per_row, int top_n,
+                           float* logprobs, float* entropy, int32_t* top_ids,
+                           float* top_logprobs, hipStream_t stream);
+int mle_token_logprobs_workspace_size(int rows, int n, int top_n, size_t* bytes,
+                                      size_t* counters);
+
+/*
  * Q8_0 16-row tiles: the bytes of a raw Q8_0 weight [N,K] reordered once, at
  * weight-load time, for the MI355X matrix cores.  No counterpart in the
  * reference: its loader copies GGUF bytes to the device as they are

@@ -31,7 +31,9 @@ EXPORTED = ("mle_q8_0_abi_version", "mle_q8_0_linear", "mle_q8_0_linear_ex",
             "mle_q8_0_dequantize", "mle_q8_0_linear_bias_bf16",
             "mle_q8_0_linear_tiled_bias_bf16", "mle_probe_stream_read",
             "mle_paged_plan", "mle_rope_table", "mle_paged_kv_write", "mle_paged_attention",
-            "mle_paged_attention_workspace_size")
+            "mle_paged_attention_workspace_size", "mle_token_logprobs_f32",
+            "mle_token_logprobs_workspace_size", "mle_paged_kv_write_normed",
+            "mle_paged_tree_attention", "mle_paged_kv_keep")
 
 KV_TYPES = {"f16": 0, "bf16": 1, "int8": 2}
 ROPE_MODES = {"pairs": 0, "halves": 1, "none": -1}  # none: without a table, refused with one
@@ -134,6 +136,21 @@ def load() -> ctypes.CDLL:
                                         _vp, _vp, _i, _i, _vp]
     lib.mle_paged_attention_workspace_size.restype = _i
     lib.mle_paged_attention_workspace_size.argtypes = [_vp, _i, _i, _i, _vp, _vp]
+    lib.mle_token_logprobs_f32.restype = _i
+    lib.mle_token_logprobs_f32.argtypes = [_vp, _i, _i, ctypes.c_float, _vp, _i, _i, _vp, _vp,
+                                           _vp, _vp, _vp]
+    lib.mle_token_logprobs_workspace_size.restype = _i
+    lib.mle_token_logprobs_workspace_size.argtypes = [_i, _i, _i, _vp, _vp]
+    lib.mle_paged_kv_write_normed.restype = _i
+    lib.mle_paged_kv_write_normed.argtypes = [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp,
+                                              _vp, ctypes.c_float, _vp, _i, _i, _i, _vp, _vp,
+                                              _i, _vp]
+    lib.mle_paged_tree_attention.restype = _i
+    lib.mle_paged_tree_attention.argtypes = [_vp, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp,
+                                             _i, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp]
+    lib.mle_paged_kv_keep.restype = _i
+    lib.mle_paged_kv_keep.argtypes = [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp,
+                                      _vp, _vp, _vp, _vp]
     _lib = lib
     return lib
 
@@ -336,6 +353,31 @@ def top_tokens(logits, rows, n, top_n, ids, probs, temperature=1.0, stream=None)
     """ids/probs [rows, min(top_n, n)]: the top tokens of each logits row by softmax
     probability (after 1/temperature), largest first (Sampler::get_top_tokens)."""
     _raise(top_tokens_status(logits, rows, n, top_n, ids, probs, temperature, stream)[0])
+
+
+def token_logprobs_status(logits, rows, n, tokens, tokens_per_row, top_n, logprobs, entropy,
+                          top_ids, top_logprobs, temperature=1.0, stream=None):
+    rc = load().mle_token_logprobs_f32(_addr(logits), rows, n, float(temperature),
+                                       _addr(tokens), tokens_per_row, top_n, _addr(logprobs),
+                                       _addr(entropy), _addr(top_ids), _addr(top_logprobs),
+                                       _stream(stream))
+    return _status(rc)
+
+
+def token_logprobs(logits, rows, n, tokens, tokens_per_row, top_n, logprobs, entropy, top_ids,
+                   top_logprobs, temperature=1.0, stream=None) -> None:
+    """logprobs [rows, tokens_per_row] of the given tokens, entropy [rows], and the top_n
+    alternatives of each logits row with their log probabilities (None: left out)."""
+    _raise(token_logprobs_status(logits, rows, n, tokens, tokens_per_row, top_n, logprobs,
+                                 entropy, top_ids, top_logprobs, temperature, stream)[0])
+
+
+def token_logprobs_workspace_size(rows, n, top_n):
+    """(bytes, counters) that hold any token_logprobs call of up to these sizes."""
+    b, c = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _raise(load().mle_token_logprobs_workspace_size(rows, n, top_n, ctypes.byref(b),
+                                                    ctypes.byref(c)))
+    return b.value, c.value
 
 
 def dequantize_status(src, dst, n, stream=None):
@@ -541,6 +583,34 @@ def paged_kv_write(cache, q, q_out, heads, k, v, rope, rope_positions, rope_dim,
                                  k_stride, v_stride, stream)[0])
 
 
+def paged_kv_write_normed_status(cache, q, q_out, heads, k, v, q_norm, k_norm, eps, rope,
+                                 rope_positions, rope_dim, rope_mode, positions, slots, tokens,
+                                 q_stride=None, q_out_stride=None, k_stride=None, v_stride=None,
+                                 stream=None):
+    dim = cache.struct.head_dim
+    row, kv_row = heads * dim, cache.struct.kv_heads * dim
+    rc = load().mle_paged_kv_write_normed(
+        cache, _addr(q), _row_stride(q, q_stride, row), _addr(q_out),
+        _row_stride(q_out, q_out_stride, row), heads, _addr(k),
+        _row_stride(k, k_stride, kv_row), _addr(v), _row_stride(v, v_stride, kv_row),
+        _addr(q_norm), _addr(k_norm), eps, _addr(rope), rope_positions, rope_dim,
+        ROPE_MODES.get(rope_mode, rope_mode), _addr(positions), _addr(slots), tokens,
+        _stream(stream))
+    return _status(rc)
+
+
+def paged_kv_write_normed(cache, q, q_out, heads, k, v, q_norm, k_norm, eps, rope,
+                          rope_positions, rope_dim, rope_mode, positions, slots, tokens,
+                          q_stride=None, q_out_stride=None, k_stride=None, v_stride=None,
+                          stream=None) -> None:
+    """paged_kv_write with every head of q and k over its root mean square, times q_norm and
+    k_norm [head_dim], before the rotation."""
+    _raise(paged_kv_write_normed_status(cache, q, q_out, heads, k, v, q_norm, k_norm, eps, rope,
+                                        rope_positions, rope_dim, rope_mode, positions, slots,
+                                        tokens, q_stride, q_out_stride, k_stride, v_stride,
+                                        stream)[0])
+
+
 def paged_attention_status(cache, q, out, heads, scale, window, block_table, max_pages, kv_lens,
                            cu_tokens, sequences, tokens, q_stride=None, out_stride=None,
                            stream=None):
@@ -567,3 +637,63 @@ def paged_attention_workspace_size(cache, heads, sequences, tokens):
     _raise(load().mle_paged_attention_workspace_size(cache, heads, sequences, tokens,
                                                      ctypes.byref(b), ctypes.byref(c)))
     return b.value, c.value
+
+
+# Trees of drafted tokens over the paged cache.
+
+def paged_tree_attention_status(cache, q, out, heads, scale, window, block_table, max_pages,
+                                kv_lens, cu_tokens, sequences, tokens, tree_mask, mask_words,
+                                row_positions=None, trees=None, q_stride=None, out_stride=None,
+                                stream=None):
+    row = heads * cache.struct.head_dim
+    rc = load().mle_paged_tree_attention(
+        cache, _addr(q), _row_stride(q, q_stride, row), _addr(out),
+        _row_stride(out, out_stride, row), heads, scale, window, _addr(block_table), max_pages,
+        _addr(kv_lens), _addr(cu_tokens), sequences, tokens, _addr(tree_mask), mask_words,
+        _addr(row_positions), _addr(trees), _stream(stream))
+    return _status(rc)
+
+
+def paged_tree_attention(cache, q, out, heads, scale, window, block_table, max_pages, kv_lens,
+                         cu_tokens, sequences, tokens, tree_mask, mask_words,
+                         row_positions=None, trees=None, q_stride=None, out_stride=None,
+                         stream=None) -> None:
+    """paged_attention where a row sees, of its request's new rows, those of its mask
+    (tree_mask [tokens, mask_words] int64, a bit a row); trees[b] == 0: request b is a run."""
+    _raise(paged_tree_attention_status(cache, q, out, heads, scale, window, block_table,
+                                       max_pages, kv_lens, cu_tokens, sequences, tokens,
+                                       tree_mask, mask_words, row_positions, trees, q_stride,
+                                       out_stride, stream)[0])
+
+
+class PagedCaches:
+    """The PagedCache objects of a model's layers, as calls take them that work on all."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        self.structs = (_CacheStruct * max(len(self.caches), 1))(*(c.struct for c in self.caches))
+        self._as_parameter_ = ctypes.addressof(self.structs)
+
+    def __len__(self):
+        return len(self.caches)
+
+
+def paged_kv_keep_status(caches, block_table, max_pages, kv_lens, cu_tokens, granted, sequences,
+                         keep, keep_stride, keep_counts, kept_lens, free_pages, free_count,
+                         free_count_out, stream=None):
+    rc = load().mle_paged_kv_keep(caches, len(caches), _addr(block_table), max_pages,
+                                  _addr(kv_lens), _addr(cu_tokens), _addr(granted), sequences,
+                                  _addr(keep), keep_stride, _addr(keep_counts),
+                                  _addr(kept_lens), _addr(free_pages), _addr(free_count),
+                                  _addr(free_count_out), _stream(stream))
+    return _status(rc)
+
+
+def paged_kv_keep(caches, block_table, max_pages, kv_lens, cu_tokens, granted, sequences, keep,
+                  keep_stride, keep_counts, kept_lens, free_pages, free_count, free_count_out,
+                  stream=None) -> None:
+    """The rows keep[b, :keep_counts[b]] of each request become the tokens behind its cached
+    ones, in all layers' caches (PagedCaches); the pages past them go onto the free stack."""
+    _raise(paged_kv_keep_status(caches, block_table, max_pages, kv_lens, cu_tokens, granted,
+                                sequences, keep, keep_stride, keep_counts, kept_lens,
+                                free_pages, free_count, free_count_out, stream)[0])

@@ -743,6 +743,120 @@ void plan_matmul(int M, int N, int K, const Exec& ex) {
     (void)workspace_for(mle::gemm_mfma_workspace_up_to(M, gs, K), ex, &ws, &hold);
 }
 
+// The cache write of both entry points, `a` holding the norms.
+int kv_write(const char* ctx, mle::KvWriteArgs a, const mle_paged_cache* cache, const float* q,
+             int q_stride, float* q_out, int q_out_stride, int heads, const float* k,
+             int k_stride, const float* v, int v_stride, const float* rope, int rope_positions,
+             int rope_dim, int rope_mode, const int32_t* positions, const int32_t* slots,
+             int tokens, hipStream_t stream) {
+  MLE_TRY(check_cache(ctx, cache, &a.cache));
+  MLE_TRY(check_positive(ctx, heads, "heads"));
+  MLE_TRY(check_tokens(ctx, tokens));
+  MLE_TRY(check_ptrs(ctx, q, "q", q_out, "q_out", k, "k"));
+  MLE_TRY(check_ptrs(ctx, v, "v", slots, "slots", slots, "slots"));
+  const int64_t row = (int64_t)heads * cache->head_dim;
+  const int64_t kv_row = (int64_t)cache->kv_heads * cache->head_dim;
+  MLE_TRY(check_rows(ctx, q, q_stride, row, "q"));
+  MLE_TRY(check_rows(ctx, q_out, q_out_stride, row, "q_out"));
+  MLE_TRY(check_rows(ctx, k, k_stride, kv_row, "k"));
+  MLE_TRY(check_rows(ctx, v, v_stride, kv_row, "v"));
+  MLE_TRY(check_align(ctx, slots, 4, "slots"));
+  if (rope != nullptr) {
+    MLE_TRY(check_ptr(ctx, positions, "positions"));
+    MLE_TRY(check_align(ctx, positions, 4, "positions"));
+    MLE_TRY(check_align(ctx, rope, 16, "rope"));
+    MLE_TRY(check_positive(ctx, rope_positions, "rope_positions"));
+    MLE_TRY(check_positive(ctx, rope_dim, "rope_dim"));
+    if (rope_dim % 8 != 0 || rope_dim > cache->head_dim)
+      return fail(MLE_INVALID_ARGUMENT,
+                  std::string("hip ") + ctx +
+                      ": rope_dim must be a multiple of 8 and at most head_dim");
+    if (rope_mode != MLE_ROPE_PAIRS && rope_mode != MLE_ROPE_HALVES)
+      return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": unknown rope_mode " +
+                                            std::to_string(rope_mode));
+  }
+  if ((int64_t)tokens * (heads + 2LL * cache->kv_heads) > kPagedMax)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": tokens * (heads + 2 kv_heads) must fit 30 bits");
+  const mle::KvWriteBlocks blocks =
+      mle::paged_kv_write_blocks(tokens, heads, cache->kv_heads, cache->head_dim);
+  if (blocks.kv + blocks.q > mle::kMostBlocks)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": tokens * (2 kv_heads + heads / 2) rows of " +
+                                     std::to_string(cache->head_dim) +
+                                     " take more than 2^32 threads");
+  if (tokens == 0) return ok();
+  a.q = q;
+  a.q_out = q_out;
+  a.k = k;
+  a.v = v;
+  a.rope = rope;
+  a.positions = positions;
+  a.slots = slots;
+  a.q_stride = q_stride;
+  a.q_out_stride = q_out_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.heads = heads;
+  a.rope_positions = rope_positions;
+  a.rope_dim = rope != nullptr ? rope_dim : 0;
+  a.rope_halves = rope_mode == MLE_ROPE_HALVES;
+  a.tokens = tokens;
+  const hipError_t err = mle::launch_paged_kv_write(a, stream);
+  return check_launch(err, (std::string("hip ") + ctx + " launch failed").c_str());
+}
+
+// The attention of both entry points, `a` holding what only a tree's has.
+int attention(const char* ctx, mle::AttentionArgs a, bool trees, const mle_paged_cache* cache,
+              const float* q, int q_stride, float* out, int out_stride, int heads, float scale,
+              int window, const int32_t* block_table, int max_pages, const int32_t* kv_lens,
+              const int32_t* cu_tokens, int sequences, int tokens, hipStream_t stream) {
+  MLE_TRY(check_cache(ctx, cache, &a.cache));
+  MLE_TRY(check_attention_sizes(ctx, cache, heads, sequences, tokens));
+  MLE_TRY(check_ptrs(ctx, q, "q", out, "out", block_table, "block_table"));
+  MLE_TRY(check_ptrs(ctx, kv_lens, "kv_lens", cu_tokens, "cu_tokens", cu_tokens, "cu_tokens"));
+  const int64_t row = (int64_t)heads * cache->head_dim;
+  MLE_TRY(check_rows(ctx, q, q_stride, row, "q"));
+  MLE_TRY(check_rows(ctx, out, out_stride, row, "out"));
+  MLE_TRY(check_align(ctx, block_table, 4, "block_table"));
+  MLE_TRY(check_align(ctx, kv_lens, 4, "kv_lens"));
+  MLE_TRY(check_align(ctx, cu_tokens, 4, "cu_tokens"));
+  MLE_TRY(check_positive(ctx, max_pages, "max_pages"));
+  if (!std::isfinite(scale))
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": scale must be finite");
+  if (window < 0)
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": window must not be negative");
+  // The kernel's key numbers run a few steps past the last key.
+  if ((int64_t)max_pages * cache->page_size > INT32_MAX - 65536)
+    return fail(MLE_UNSUPPORTED,
+                std::string("hip ") + ctx + ": max_pages * page_size must fit 31 bits");
+  if (tokens == 0) return ok();
+  const int group = heads / cache->kv_heads;
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.heads = heads;
+  a.scale = scale;
+  a.window = window;
+  a.table = block_table;
+  a.max_pages = max_pages;
+  a.kv_lens = kv_lens;
+  a.cu = cu_tokens;
+  a.sequences = sequences;
+  a.tokens = tokens;
+  mle::SplitKWorkspace ws;
+  std::unique_lock<std::mutex> hold;
+  const int64_t rows = (int64_t)tokens * group;
+  MLE_TRY(get_workspace(trees ? mle::paged_tree_attention_workspace(cache->head_dim, rows)
+                              : mle::paged_attention_workspace(cache->head_dim, rows),
+                        stream, &ws, &hold));
+  return trees ? check_launch(mle::launch_paged_tree_attention(a, ws, stream),
+                              "hip paged_tree_attention launch failed")
+               : check_launch(mle::launch_paged_attention(a, ws, stream),
+                              "hip paged_attention launch failed");
+}
+
 }  // namespace
 
 extern "C" {
@@ -1120,6 +1234,67 @@ int mle_top_tokens_f32(const float* logits, int rows, int n, int top_n, float te
                       "hip top_tokens launch failed");
 }
 
+int mle_token_logprobs_f32(const float* logits, int rows, int n, float temperature,
+                           const int32_t* tokens, int tokens_per_row, int top_n,
+                           float* logprobs, float* entropy, int32_t* top_ids,
+                           float* top_logprobs, hipStream_t stream) {
+  const char* ctx = "token_logprobs_f32";
+  MLE_TRY(check_ptr(ctx, logits, "logits"));
+  MLE_TRY(check_positive(ctx, rows, "rows"));
+  MLE_TRY(check_positive(ctx, n, "n"));
+  if (tokens_per_row < 0 || top_n < 0)
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": tokens_per_row and top_n must not be negative");
+  if (tokens_per_row > 0)
+    MLE_TRY(check_ptrs(ctx, tokens, "tokens", logprobs, "logprobs", logprobs, "logprobs"));
+  if (top_n > 0)
+    MLE_TRY(check_ptrs(ctx, top_ids, "top_ids", top_logprobs, "top_logprobs", top_logprobs,
+                       "top_logprobs"));
+  if (tokens_per_row == 0 && top_n == 0 && entropy == nullptr) return ok();  // nothing asked for
+  if (rows > 65535)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": at most 65535 rows per call");
+  if (top_n > mle::kTopTokensMax)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": top_n must be at most " +
+                                     std::to_string(mle::kTopTokensMax) + ", got " +
+                                     std::to_string(top_n));
+  const int kk = top_n < n ? top_n : n;
+  if (kk > 0 && n > mle::topk_max_n(kk))
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": n must be at most " +
+                                     std::to_string(mle::topk_max_n(kk)) + " for top_n " +
+                                     std::to_string(kk));
+  MLE_TRY(check_align(ctx, logits, 4, "logits"));
+  MLE_TRY(check_align(ctx, tokens, 4, "tokens"));
+  MLE_TRY(check_align(ctx, logprobs, 4, "logprobs"));
+  MLE_TRY(check_align(ctx, entropy, 4, "entropy"));
+  MLE_TRY(check_align(ctx, top_ids, 4, "top_ids"));
+  MLE_TRY(check_align(ctx, top_logprobs, 4, "top_logprobs"));
+  mle::SplitKNeed need;
+  need.partial_floats = mle::token_logprobs_workspace_floats(rows, n, top_n);
+  mle::SplitKWorkspace ws;
+  std::unique_lock<std::mutex> hold;  // released after the launch is enqueued
+  MLE_TRY(get_workspace(need, stream, &ws, &hold));
+  return check_launch(
+      mle::launch_token_logprobs(logits, rows, n, temperature, tokens, tokens_per_row, top_n,
+                                 logprobs, entropy, top_ids, top_logprobs, ws.partials, stream),
+      "hip token_logprobs launch failed");
+}
+
+int mle_token_logprobs_workspace_size(int rows, int n, int top_n, size_t* bytes,
+                                      size_t* counters) {
+  const char* ctx = "token_logprobs_workspace_size";
+  MLE_TRY(check_ptrs(ctx, bytes, "bytes", counters, "counters", counters, "counters"));
+  MLE_TRY(check_positive(ctx, rows, "rows"));
+  MLE_TRY(check_positive(ctx, n, "n"));
+  if (top_n < 0 || top_n > mle::kTopTokensMax || rows > 65535)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": at most 65535 rows, top_n 0 to " +
+                                     std::to_string(mle::kTopTokensMax));
+  mle::SplitKNeed need;
+  need.partial_floats = mle::token_logprobs_workspace_floats(rows, n, top_n);
+  *bytes = need_bytes(need);
+  *counters = need.counters;
+  return ok();
+}
+
 int mle_q8_0_matmul(const float* a, const uint8_t* b_q8_0, float* c, int M, int N, int K,
                     hipStream_t stream) {
   const char* ctx = "sgemm_q8_0_weight";
@@ -1279,62 +1454,32 @@ int mle_paged_kv_write(const mle_paged_cache* cache, const float* q, int q_strid
                        const float* v, int v_stride, const float* rope, int rope_positions,
                        int rope_dim, int rope_mode, const int32_t* positions,
                        const int32_t* slots, int tokens, hipStream_t stream) {
-  const char* ctx = "paged_kv_write";
+  return kv_write("paged_kv_write", mle::KvWriteArgs{}, cache, q, q_stride, q_out, q_out_stride,
+                  heads, k, k_stride, v, v_stride, rope, rope_positions, rope_dim, rope_mode,
+                  positions, slots, tokens, stream);
+}
+
+int mle_paged_kv_write_normed(const mle_paged_cache* cache, const float* q, int q_stride,
+                              float* q_out, int q_out_stride, int heads, const float* k,
+                              int k_stride, const float* v, int v_stride, const float* q_norm,
+                              const float* k_norm, float eps, const float* rope,
+                              int rope_positions, int rope_dim, int rope_mode,
+                              const int32_t* positions, const int32_t* slots, int tokens,
+                              hipStream_t stream) {
+  const char* ctx = "paged_kv_write_normed";
+  MLE_TRY(check_ptrs(ctx, q_norm, "q_norm", k_norm, "k_norm", k_norm, "k_norm"));
+  MLE_TRY(check_align(ctx, q_norm, 16, "q_norm"));
+  MLE_TRY(check_align(ctx, k_norm, 16, "k_norm"));
+  if (!(eps >= 0.0f) || !std::isfinite(eps))
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": eps must be finite and not negative");
   mle::KvWriteArgs a{};
-  MLE_TRY(check_cache(ctx, cache, &a.cache));
-  MLE_TRY(check_positive(ctx, heads, "heads"));
-  MLE_TRY(check_tokens(ctx, tokens));
-  MLE_TRY(check_ptrs(ctx, q, "q", q_out, "q_out", k, "k"));
-  MLE_TRY(check_ptrs(ctx, v, "v", slots, "slots", slots, "slots"));
-  const int64_t row = (int64_t)heads * cache->head_dim;
-  const int64_t kv_row = (int64_t)cache->kv_heads * cache->head_dim;
-  MLE_TRY(check_rows(ctx, q, q_stride, row, "q"));
-  MLE_TRY(check_rows(ctx, q_out, q_out_stride, row, "q_out"));
-  MLE_TRY(check_rows(ctx, k, k_stride, kv_row, "k"));
-  MLE_TRY(check_rows(ctx, v, v_stride, kv_row, "v"));
-  MLE_TRY(check_align(ctx, slots, 4, "slots"));
-  if (rope != nullptr) {
-    MLE_TRY(check_ptr(ctx, positions, "positions"));
-    MLE_TRY(check_align(ctx, positions, 4, "positions"));
-    MLE_TRY(check_align(ctx, rope, 16, "rope"));
-    MLE_TRY(check_positive(ctx, rope_positions, "rope_positions"));
-    MLE_TRY(check_positive(ctx, rope_dim, "rope_dim"));
-    if (rope_dim % 8 != 0 || rope_dim > cache->head_dim)
-      return fail(MLE_INVALID_ARGUMENT,
-                  std::string("hip ") + ctx +
-                      ": rope_dim must be a multiple of 8 and at most head_dim");
-    if (rope_mode != MLE_ROPE_PAIRS && rope_mode != MLE_ROPE_HALVES)
-      return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": unknown rope_mode " +
-                                            std::to_string(rope_mode));
-  }
-  if ((int64_t)tokens * (heads + 2LL * cache->kv_heads) > kPagedMax)
-    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
-                                     ": tokens * (heads + 2 kv_heads) must fit 30 bits");
-  const mle::KvWriteBlocks blocks =
-      mle::paged_kv_write_blocks(tokens, heads, cache->kv_heads, cache->head_dim);
-  if (blocks.kv + blocks.q > mle::kMostBlocks)
-    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
-                                     ": tokens * (2 kv_heads + heads / 2) rows of " +
-                                     std::to_string(cache->head_dim) +
-                                     " take more than 2^32 threads");
-  if (tokens == 0) return ok();
-  a.q = q;
-  a.q_out = q_out;
-  a.k = k;
-  a.v = v;
-  a.rope = rope;
-  a.positions = positions;
-  a.slots = slots;
-  a.q_stride = q_stride;
-  a.q_out_stride = q_out_stride;
-  a.k_stride = k_stride;
-  a.v_stride = v_stride;
-  a.heads = heads;
-  a.rope_positions = rope_positions;
-  a.rope_dim = rope != nullptr ? rope_dim : 0;
-  a.rope_halves = rope_mode == MLE_ROPE_HALVES;
-  a.tokens = tokens;
-  return check_launch(mle::launch_paged_kv_write(a, stream), "hip paged_kv_write launch failed");
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
+  return kv_write(ctx, a, cache, q, q_stride, q_out, q_out_stride, heads, k, k_stride, v,
+                  v_stride, rope, rope_positions, rope_dim, rope_mode, positions, slots, tokens,
+                  stream);
 }
 
 int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stride, float* out,
@@ -1342,48 +1487,35 @@ int mle_paged_attention(const mle_paged_cache* cache, const float* q, int q_stri
                         const int32_t* block_table, int max_pages, const int32_t* kv_lens,
                         const int32_t* cu_tokens, int sequences, int tokens,
                         hipStream_t stream) {
-  const char* ctx = "paged_attention";
+  return attention("paged_attention", mle::AttentionArgs{}, false, cache, q, q_stride, out,
+                   out_stride, heads, scale, window, block_table, max_pages, kv_lens, cu_tokens,
+                   sequences, tokens, stream);
+}
+
+int mle_paged_tree_attention(const mle_paged_cache* cache, const float* q, int q_stride,
+                             float* out, int out_stride, int heads, float scale, int window,
+                             const int32_t* block_table, int max_pages, const int32_t* kv_lens,
+                             const int32_t* cu_tokens, int sequences, int tokens,
+                             const uint64_t* tree_mask, int mask_words,
+                             const int32_t* row_positions, const int32_t* trees,
+                             hipStream_t stream) {
+  const char* ctx = "paged_tree_attention";
+  MLE_TRY(check_ptr(ctx, tree_mask, "tree_mask"));
+  MLE_TRY(check_align(ctx, tree_mask, 8, "tree_mask"));
+  MLE_TRY(check_positive(ctx, mask_words, "mask_words"));
+  if (mask_words > MLE_TREE_MAX_WORDS)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": mask_words must be at most " +
+                                     std::to_string(MLE_TREE_MAX_WORDS));
+  if (window > 0) MLE_TRY(check_ptr(ctx, row_positions, "row_positions"));
+  MLE_TRY(check_align(ctx, row_positions, 4, "row_positions"));
+  MLE_TRY(check_align(ctx, trees, 4, "trees"));
   mle::AttentionArgs a{};
-  MLE_TRY(check_cache(ctx, cache, &a.cache));
-  MLE_TRY(check_attention_sizes(ctx, cache, heads, sequences, tokens));
-  MLE_TRY(check_ptrs(ctx, q, "q", out, "out", block_table, "block_table"));
-  MLE_TRY(check_ptrs(ctx, kv_lens, "kv_lens", cu_tokens, "cu_tokens", cu_tokens, "cu_tokens"));
-  const int64_t row = (int64_t)heads * cache->head_dim;
-  MLE_TRY(check_rows(ctx, q, q_stride, row, "q"));
-  MLE_TRY(check_rows(ctx, out, out_stride, row, "out"));
-  MLE_TRY(check_align(ctx, block_table, 4, "block_table"));
-  MLE_TRY(check_align(ctx, kv_lens, 4, "kv_lens"));
-  MLE_TRY(check_align(ctx, cu_tokens, 4, "cu_tokens"));
-  MLE_TRY(check_positive(ctx, max_pages, "max_pages"));
-  if (!std::isfinite(scale))
-    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": scale must be finite");
-  if (window < 0)
-    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": window must not be negative");
-  // The kernel's key numbers run a few steps past the last key.
-  if ((int64_t)max_pages * cache->page_size > INT32_MAX - 65536)
-    return fail(MLE_UNSUPPORTED,
-                std::string("hip ") + ctx + ": max_pages * page_size must fit 31 bits");
-  if (tokens == 0) return ok();
-  const int group = heads / cache->kv_heads;
-  a.q = q;
-  a.out = out;
-  a.q_stride = q_stride;
-  a.out_stride = out_stride;
-  a.heads = heads;
-  a.scale = scale;
-  a.window = window;
-  a.table = block_table;
-  a.max_pages = max_pages;
-  a.kv_lens = kv_lens;
-  a.cu = cu_tokens;
-  a.sequences = sequences;
-  a.tokens = tokens;
-  mle::SplitKWorkspace ws;
-  std::unique_lock<std::mutex> hold;
-  MLE_TRY(get_workspace(mle::paged_attention_workspace(cache->head_dim, (int64_t)tokens * group),
-                        stream, &ws, &hold));
-  return check_launch(mle::launch_paged_attention(a, ws, stream),
-                      "hip paged_attention launch failed");
+  a.mask = reinterpret_cast<const uint32_t*>(tree_mask);
+  a.mask_words = mask_words;
+  a.row_positions = row_positions;
+  a.trees = trees;
+  return attention(ctx, a, true, cache, q, q_stride, out, out_stride, heads, scale, window,
+                   block_table, max_pages, kv_lens, cu_tokens, sequences, tokens, stream);
 }
 
 int mle_paged_attention_workspace_size(const mle_paged_cache* cache, int heads, int sequences,
@@ -1396,6 +1528,83 @@ int mle_paged_attention_workspace_size(const mle_paged_cache* cache, int heads, 
       cache->head_dim, (int64_t)tokens * (heads / cache->kv_heads));
   *bytes = tokens > 0 ? need_bytes(need) : 0;
   *counters = tokens > 0 ? need.counters : 0;
+  return ok();
+}
+
+int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* block_table,
+                      int max_pages, const int32_t* kv_lens, const int32_t* cu_tokens,
+                      const int32_t* granted, int sequences, const int32_t* keep,
+                      int keep_stride, const int32_t* keep_counts, int32_t* kept_lens,
+                      int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
+                      hipStream_t stream) {
+  const char* ctx = "paged_kv_keep";
+  MLE_TRY(check_ptr(ctx, caches, "caches"));
+  MLE_TRY(check_positive(ctx, layers, "layers"));
+  for (int i = 0; i < layers; ++i) {
+    mle::PagedCache c;
+    MLE_TRY(check_cache(ctx, caches + i, &c));
+    if (c.type != (mle::KvType)caches->type || c.num_pages != caches->num_pages ||
+        c.page_size != caches->page_size || c.kv_heads != caches->kv_heads ||
+        c.head_dim != caches->head_dim)
+      return fail(MLE_SHAPE_MISMATCH, std::string("hip ") + ctx + ": cache " +
+                                          std::to_string(i) +
+                                          " differs from cache 0 in type or sizes");
+  }
+  const struct { const void* p; const char* name; bool need; } bufs[] = {
+      {block_table, "block_table", true}, {kv_lens, "kv_lens", true},
+      {cu_tokens, "cu_tokens", true},     {granted, "granted", true},
+      {keep, "keep", true},               {keep_counts, "keep_counts", true},
+      {kept_lens, "kept_lens", true},     {free_pages, "free_pages", false},
+      {free_count, "free_count", free_pages != nullptr},
+      {free_count_out, "free_count_out", free_pages != nullptr}};
+  for (const auto& b : bufs) {
+    if (b.need) MLE_TRY(check_ptr(ctx, b.p, b.name));
+    MLE_TRY(check_align(ctx, b.p, 4, b.name));
+  }
+  MLE_TRY(check_positive(ctx, sequences, "sequences"));
+  MLE_TRY(check_positive(ctx, max_pages, "max_pages"));
+  MLE_TRY(check_positive(ctx, keep_stride, "keep_stride"));
+  if (kept_lens == kv_lens)
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": kept_lens must not be kv_lens, which the move reads");
+  if ((int64_t)max_pages * caches->page_size > INT32_MAX - 65536 ||
+      (int64_t)sequences * max_pages > INT32_MAX)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": max_pages * page_size and sequences * max_pages must "
+                                     "fit 31 bits");
+  const int most = layers < mle::kKeepLayers ? layers : mle::kKeepLayers;
+  if (mle::paged_keep_blocks(most, sequences, caches->kv_heads) >= mle::kMostBlocks)
+    return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
+                                     ": layers * sequences * kv_heads take more than 2^32 threads");
+  mle::KeepArgs a{};
+  a.num_pages = caches->num_pages;
+  a.page_size = caches->page_size;
+  a.kv_heads = caches->kv_heads;
+  a.table = block_table;
+  a.max_pages = max_pages;
+  a.kv_lens = kv_lens;
+  a.cu = cu_tokens;
+  a.granted = granted;
+  a.sequences = sequences;
+  a.keep = keep;
+  a.keep_stride = keep_stride;
+  a.counts = keep_counts;
+  a.kept_lens = kept_lens;
+  a.stack = free_pages;
+  a.count = free_count;
+  a.count_out = free_count_out;
+  for (int first = 0; first < layers; first += mle::kKeepLayers) {
+    a.layers = layers - first < mle::kKeepLayers ? layers - first : mle::kKeepLayers;
+    for (int i = 0; i < a.layers; ++i) {
+      const mle_paged_cache& c = caches[first + i];
+      a.layer[i] = {c.k, c.v, c.k_scale, c.v_scale};
+    }
+    MLE_TRY(check_launch(mle::launch_paged_keep(a, (mle::KvType)caches->type, caches->head_dim,
+                                                stream),
+                         "hip paged_kv_keep launch failed"));
+    a.kept_lens = nullptr;  // once
+    a.stack = nullptr;
+  }
   return ok();
 }
 

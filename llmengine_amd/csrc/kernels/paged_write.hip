@@ -19,6 +19,11 @@
 // the rows r .. r + 3 fill such a place, the group of the first writes all four, 8 bytes
 // at a time, and the others' groups leave it to that one; any other row writes its
 // elements one by one.
+//
+// With weights, q and k are first normed, row by row of a head: x w / sqrt(mean x^2 + eps),
+// then rotated.  All of it in 64 bits, rounded once, so that 8-bit quants do not depend on the
+// order of the sum either; the sum is a few lane exchanges, and the lanes of a row past its
+// head_dim take part in them with zeros.
 #include "../paged.hpp"
 #include "../q8_0_device.hpp"
 
@@ -63,6 +68,46 @@ __device__ __forceinline__ void rotate8(Row8& r, const float* rope_row, int s, b
     if (halves) turn(r.x[i], r.x[4 + i], c[i], n[i]);
     else turn(r.x[2 * i], r.x[2 * i + 1], c[i], n[i]);
   }
+}
+
+__device__ __forceinline__ double from_lane_xor(double v, int off) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, off);
+  const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(u >> 32), off);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// 1 / sqrt(mean x^2 + eps) of a head's row held by LPR lanes.
+template <int LPR>
+__device__ __forceinline__ double inverse_rms(const Row8& r, int head_dim, double eps) {
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)r.x[i], (double)r.x[i], sum);
+#pragma unroll
+  for (int off = LPR / 2; off > 0; off >>= 1) sum += from_lane_xor(sum, off);
+  return 1.0 / __builtin_sqrt(sum / head_dim + eps);
+}
+
+// x w inv of a lane's 8 elements, turned as rotate8 turns them where `turns`.
+__device__ __forceinline__ void norm8(Row8& r, const Row8& w, double inv, const float* rope_row,
+                                      int s, bool halves, bool turns) {
+  double x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (double)r.x[i] * inv * (double)w.x[i];
+  if (turns) {
+    const f32x4 t0 = *reinterpret_cast<const f32x4*>(rope_row + 8 * s);
+    const f32x4 t1 = *reinterpret_cast<const f32x4*>(rope_row + 8 * s + 4);
+    const double c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = halves ? i : 2 * i, q = halves ? 4 + i : 2 * i + 1;
+      const double a = x[p], b = x[q];
+      x[p] = __builtin_fma(a, c[i], -(b * n[i]));
+      x[q] = __builtin_fma(a, n[i], b * c[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.x[i] = (float)x[i];
 }
 
 // Largest magnitude over a group of LPR lanes as a bit pattern: the order of the patterns
@@ -120,7 +165,7 @@ __device__ __forceinline__ void put1(void* base, int64_t at, uint32_t c) {
 constexpr int kQHeads = 2;
 
 // LPR lanes (a power of two, at least head_dim / 8) take one head's row of one token.
-template <KvType T, int LPR>
+template <KvType T, int LPR, bool kNorm>
 __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const int G = a.cache.kv_heads, D = a.cache.head_dim, P = a.cache.page_size;
   // The first workgroups take k and v, head by head, the others q, token by token.
@@ -144,19 +189,33 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const bool turns = a.rope != nullptr && placed && s * 8 < a.rope_dim;
 
   if (is_q) {
-    if (!live) return;
+    if (!kNorm && !live) return;
     const Span sp = span_of(s, a.rope_dim, halves);
     const float* q = a.q + t * a.q_stride + (int64_t)h * kQHeads * D;
     float* o = a.q_out + t * a.q_out_stride + (int64_t)h * kQHeads * D;
     const int n = a.heads - h * kQHeads;  // heads from here on
     Row8 r[kQHeads];
+    if constexpr (kNorm) {
+      Row8 w = {};
+      if (live) w = load8(a.q_norm, sp);
 #pragma unroll
-    for (int i = 0; i < kQHeads; ++i)
-      if (i < n) r[i] = load8(q + i * D, sp);
+      for (int i = 0; i < kQHeads; ++i) {
+        r[i] = {};
+        if (i < n && live) r[i] = load8(q + i * D, sp);
+      }
+#pragma unroll
+      for (int i = 0; i < kQHeads; ++i)
+        norm8(r[i], w, inverse_rms<LPR>(r[i], D, a.eps), rope_row, s, halves, turns);
+      if (!live) return;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kQHeads; ++i)
+        if (i < n) r[i] = load8(q + i * D, sp);
+    }
 #pragma unroll
     for (int i = 0; i < kQHeads; ++i) {
       if (i >= n) continue;
-      if (turns) rotate8(r[i], rope_row, s, halves);
+      if (!kNorm && turns) rotate8(r[i], rope_row, s, halves);
       if (!placed) r[i] = {};
       float* to = o + i * D;
       *reinterpret_cast<f32x4*>(to + sp.a) =
@@ -177,7 +236,14 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
     const Span sp = span_of(s, a.rope_dim, halves);
     Row8 r = {};
     if (live) r = load8(a.k + t * a.k_stride + (int64_t)g * D, sp);
-    if (turns && live) rotate8(r, rope_row, s, halves);
+    if constexpr (kNorm) {
+      Row8 w = {};
+      if (live) w = load8(a.k_norm, sp);
+      norm8(r, w, inverse_rms<LPR>(r, D, a.eps), rope_row, s, halves, turns && live);
+      if (!live) r = {};  // 0 times an infinity
+    } else if (turns && live) {
+      rotate8(r, rope_row, s, halves);
+    }
     const int64_t cell = ((int64_t)page * G + g) * P + off;
     float scale = 1.0f;
     if constexpr (T == KvType::kInt8) {
@@ -252,12 +318,17 @@ hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
       paged_kv_write_blocks(a.tokens, a.heads, a.cache.kv_heads, a.cache.head_dim);
   b.kv_blocks = (uint32_t)n.kv;
   const dim3 grid((unsigned)(n.kv + n.q)), block(256);
-  if (lpr == 8)
-    hipLaunchKernelGGL((paged_kv_write_kernel<T, 8>), grid, block, 0, stream, b);
-  else if (lpr == 16)
-    hipLaunchKernelGGL((paged_kv_write_kernel<T, 16>), grid, block, 0, stream, b);
-  else
-    hipLaunchKernelGGL((paged_kv_write_kernel<T, 32>), grid, block, 0, stream, b);
+  auto launch = [&](auto norm) {
+    constexpr bool kNorm = decltype(norm)::value;
+    if (lpr == 8)
+      hipLaunchKernelGGL((paged_kv_write_kernel<T, 8, kNorm>), grid, block, 0, stream, b);
+    else if (lpr == 16)
+      hipLaunchKernelGGL((paged_kv_write_kernel<T, 16, kNorm>), grid, block, 0, stream, b);
+    else
+      hipLaunchKernelGGL((paged_kv_write_kernel<T, 32, kNorm>), grid, block, 0, stream, b);
+  };
+  if (a.q_norm != nullptr) launch(std::true_type{});
+  else launch(std::false_type{});
   return hipGetLastError();
 }
 

@@ -217,6 +217,15 @@ size_t top_tokens_workspace_floats(int rows, int64_t n, int top_n);
 hipError_t launch_top_tokens(const float* x, int rows, int64_t n, int top_n, float temperature,
                              int32_t* ids, float* probs, float* workspace, hipStream_t stream);
 
+// Log probabilities of `given` tokens a row, the row's entropy (null: not asked for) and its
+// top_n alternatives (0: none), with the scaling, rows without a distribution and limits of
+// launch_top_tokens.  `workspace` holds token_logprobs_workspace_floats() floats.
+size_t token_logprobs_workspace_floats(int rows, int64_t n, int top_n);
+hipError_t launch_token_logprobs(const float* x, int rows, int64_t n, float temperature,
+                                 const int32_t* tokens, int given, int top_n, float* logprobs,
+                                 float* entropy, int32_t* top_ids, float* top_logprobs,
+                                 float* workspace, hipStream_t stream);
+
 // p[i] = v for i < n (clears workspace counters: a kernel, so that a captured
 // call records no memset node).
 hipError_t launch_fill_u32(uint32_t* p, size_t n, uint32_t v, hipStream_t stream);

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "launch.hpp"
 
 namespace mle {
@@ -85,6 +87,9 @@ struct KvWriteArgs {
   int rope_dim;
   int rope_halves;
   int tokens;
+  const float* q_norm;  // weights of the norms of q's and k's heads, both or (null) none
+  const float* k_norm;
+  double eps;
   uint32_t kv_blocks;  // set by the launcher
 };
 // Workgroups of the write: for k and v, then for q.
@@ -112,6 +117,12 @@ struct AttentionArgs {
   int group;
   int most;
   Divisor by_group, by_page;
+  // Of calls with trees: a row's mask in words of 32 bits, 2 mask_words a row; positions of
+  // the rows, read where there is a window; which requests are trees (null: all).
+  const uint32_t* mask;
+  int mask_words;
+  const int32_t* row_positions;
+  const int32_t* trees;
 };
 constexpr int kAttentionThreads = 256;
 constexpr int kFewRows = 16;  // up to this many rows of a tile the waves split the keys
@@ -143,5 +154,38 @@ struct FewPart {
 SplitKNeed paged_attention_workspace(int head_dim, int64_t rows);
 hipError_t launch_paged_attention(const AttentionArgs& a, const SplitKWorkspace& ws,
                                   hipStream_t stream);
+SplitKNeed paged_tree_attention_workspace(int head_dim, int64_t rows);
+hipError_t launch_paged_tree_attention(const AttentionArgs& a, const SplitKWorkspace& ws,
+                                       hipStream_t stream);
+
+// Layers whose caches one launch of the move takes.
+constexpr int kKeepLayers = 64;
+struct KeepArgs {
+  struct {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+  } layer[kKeepLayers];
+  int layers;
+  int num_pages, page_size, kv_heads;
+  const int32_t* table;
+  int max_pages;
+  const int32_t* kv_lens;
+  const int32_t* cu;
+  const int32_t* granted;
+  int sequences;
+  const int32_t* keep;
+  int keep_stride;
+  const int32_t* counts;
+  int32_t* kept_lens;  // null: only the move
+  int32_t* stack;      // null: no pages go back
+  const int32_t* count;
+  int32_t* count_out;
+  Divisor by_page;     // set by the launcher
+};
+// Workgroups of a launch, besides one for the lengths.
+int64_t paged_keep_blocks(int layers, int sequences, int kv_heads);
+hipError_t launch_paged_keep(const KeepArgs& a, KvType type, int head_dim, hipStream_t stream);
 
 }  // namespace mle
