@@ -107,7 +107,12 @@ __device__ __forceinline__ void norm8(Row8& r, const Row8& w, double inv, const 
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.x[i] = (float)x[i];
+  for (int i = 0; i < 8; ++i) {
+    r.x[i] = (float)x[i];
+    // The fp32 value is what the cache's type rounds: the compiler would otherwise go from 64
+    // bits to 16 at once, in a dozen instructions.
+    asm("" : "+v"(r.x[i]));
+  }
 }
 
 // Largest magnitude over a group of LPR lanes as a bit pattern: the order of the patterns
