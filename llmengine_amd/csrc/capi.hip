@@ -1268,14 +1268,12 @@ int mle_token_logprobs_f32(const float* logits, int rows, int n, float temperatu
   MLE_TRY(check_align(ctx, entropy, 4, "entropy"));
   MLE_TRY(check_align(ctx, top_ids, 4, "top_ids"));
   MLE_TRY(check_align(ctx, top_logprobs, 4, "top_logprobs"));
-  mle::SplitKNeed need;
-  need.partial_floats = mle::token_logprobs_workspace_floats(rows, n, top_n);
   mle::SplitKWorkspace ws;
   std::unique_lock<std::mutex> hold;  // released after the launch is enqueued
-  MLE_TRY(get_workspace(need, stream, &ws, &hold));
+  MLE_TRY(get_workspace(mle::token_logprobs_workspace(rows, n, top_n), stream, &ws, &hold));
   return check_launch(
       mle::launch_token_logprobs(logits, rows, n, temperature, tokens, tokens_per_row, top_n,
-                                 logprobs, entropy, top_ids, top_logprobs, ws.partials, stream),
+                                 logprobs, entropy, top_ids, top_logprobs, ws, stream),
       "hip token_logprobs launch failed");
 }
 
@@ -1288,8 +1286,7 @@ int mle_token_logprobs_workspace_size(int rows, int n, int top_n, size_t* bytes,
   if (top_n < 0 || top_n > mle::kTopTokensMax || rows > 65535)
     return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": at most 65535 rows, top_n 0 to " +
                                      std::to_string(mle::kTopTokensMax));
-  mle::SplitKNeed need;
-  need.partial_floats = mle::token_logprobs_workspace_floats(rows, n, top_n);
+  const mle::SplitKNeed need = mle::token_logprobs_workspace(rows, n, top_n);
   *bytes = need_bytes(need);
   *counters = need.counters;
   return ok();

@@ -42,6 +42,7 @@
 // issues all its loads of a stage before it uses one, and a NaN travels as an infinite
 // maximum instead of through a reduction of its own (13.7 us otherwise).
 #include "../launch.hpp"
+#include "../select.hpp"
 
 namespace mle {
 namespace {
@@ -61,99 +62,13 @@ __host__ __device__ constexpr int chunk_groups(int k) {
   return c;
 }
 
-__device__ __forceinline__ uint64_t topk_key(float v, uint32_t i) {
-  if (v != v) return 0;      // NaN (the row becomes uniform anyway)
-  if (v == 0.0f) v = 0.0f;   // -0 -> +0
-  uint32_t u = __builtin_bit_cast(uint32_t, v);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((uint64_t)u << 32) | (uint32_t)~i;
-}
-
-__device__ __forceinline__ float key_value(uint64_t k) {
-  uint32_t u = (uint32_t)(k >> 32);
-  u = (u & 0x80000000u) ? (u & 0x7fffffffu) : ~u;
-  return __builtin_bit_cast(float, u);
-}
-
-template <int NT, typename T, typename Op>
-__device__ T block_reduce(T v, Op op, T* part) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = op(v, __shfl_xor(v, off, 64));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __syncthreads();  // part[] may still be read from an earlier reduction
-  if (lane == 0) part[wave] = v;
-  __syncthreads();
-  T r = part[0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; ++i) r = op(r, part[i]);
-  return r;
-}
-
-struct SelectLds {
-  uint32_t hist[256];
-  uint64_t cand[256];
-  uint32_t digit, above, eq, total, ncand;
-};
-
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, m, 64);
-  const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), m, 64);
-  return ((uint64_t)hi << 32) | lo;
-}
-
-// Descending bitonic sort of 256 keys held by one wave, 4 per lane (element
-// 4 lane + j), in registers.
-__device__ void wave_sort256_desc(uint64_t (&v)[4]) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int size = 2; size <= 256; size <<= 1)
-#pragma unroll
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      if (stride >= 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = 4 * lane + j;
-          const uint64_t o = shfl_xor64(v[j], stride >> 2);
-          const bool lower = (e & stride) == 0;
-          const bool keep_max = lower == ((e & size) == 0);
-          v[j] = keep_max ? (o > v[j] ? o : v[j]) : (o < v[j] ? o : v[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j & stride) continue;  // handle each in-lane pair once, from its lower element
-          const int e = 4 * lane + j;
-          const bool desc = (e & size) == 0;
-          const uint64_t a = v[j], c = v[j + stride];
-          const bool swap = desc ? a < c : a > c;
-          v[j] = swap ? c : a;
-          v[j + stride] = swap ? a : c;
-        }
-      }
-    }
-}
-
-// hist[bin] += 1 for every lane with `in`.  Lanes that all name one bin (ties, the leading
-// digits) add once: 16384 single adds to one LDS word took 7 us a digit (MI355X).
-__device__ __forceinline__ void count_bin(uint32_t* hist, uint32_t bin, bool in) {
-  const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
-  if (lanes == 0) return;  // uniform
-  const int first = __builtin_ctzll(lanes);
-  const uint32_t one = (uint32_t)__builtin_amdgcn_readlane((int)bin, first);
-  if (__builtin_amdgcn_ballot_w64(in && bin == one) == lanes) {
-    if ((int)(threadIdx.x & 63) == first) atomicAdd(&hist[one], (uint32_t)__builtin_popcountll(lanes));
-  } else if (in) {
-    atomicAdd(&hist[bin], 1u);
-  }
-}
-
 // Top k (k <= kTopTokensMax) of the distinct keys held E per thread by NT threads
 // (0 = no key), written sorted descending to out[0, k) (zeros past the number
 // of keys).
 template <int NT, int E>
 __device__ void select_top(const uint64_t (&key)[E], int k, uint64_t* __restrict__ out,
                            SelectLds& sm) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, wave = tid >> 6;
   uint64_t prefix = 0, mask = 0;
   int need = k;
   bool all = false;  // fewer keys than k: every key is a candidate
@@ -167,31 +82,7 @@ __device__ void select_top(const uint64_t (&key)[E], int k, uint64_t* __restrict
       count_bin(sm.hist, (uint32_t)(key[e] >> shift) & 255u,
                 key[e] != 0 && (key[e] & mask) == prefix);
     __syncthreads();
-    if (wave == 0) {
-      uint32_t h[4], local = 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        h[t] = sm.hist[255 - (4 * lane + t)];
-        local += h[t];
-      }
-      uint32_t incl = local;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)incl, off, 64);
-        if (lane >= off) incl += o;
-      }
-      uint32_t run = incl - local;  // keys in the bins above this lane's first bin
-      if (lane == 63) sm.total = incl;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (run < (uint32_t)need && (uint32_t)need <= run + h[t]) {
-          sm.digit = 255u - (uint32_t)(4 * lane + t);
-          sm.above = run;
-          sm.eq = h[t];
-        }
-        run += h[t];
-      }
-    }
+    if (wave == 0) find_digit(sm, need);
     __syncthreads();
     if (shift == 56 && sm.total <= (uint32_t)k) {
       all = true;
@@ -211,23 +102,8 @@ __device__ void select_top(const uint64_t (&key)[E], int k, uint64_t* __restrict
   for (int e = 0; e < E; ++e)
     if (key[e] != 0 && (all || key[e] >= prefix)) sm.cand[atomicAdd(&sm.ncand, 1u)] = key[e];
   __syncthreads();
-  if (wave == 0) {
-    uint64_t v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = sm.cand[4 * lane + j];
-    wave_sort256_desc(v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * lane + j < k) out[4 * lane + j] = v[j];
-  }
+  if (wave == 0) sort_candidates(sm, k, out);
   __syncthreads();
-}
-
-// A logit under the temperature, rounded once.  Never contracted with what uses it: both
-// passes have to see the same value, or a row's own maximum could lie above its maximum.
-__device__ __forceinline__ float scaled_logit(float v, float inv_temp) {
-#pragma clang fp contract(off)
-  return v * inv_temp;
 }
 
 // Distance bin of a value not above the row's finite maximum (0: at it, +Inf: 8160).  The
@@ -239,8 +115,6 @@ __device__ __forceinline__ uint32_t dist_bin(float mx, float v) {
 // Pass 1: workgroup (c, r) over logits[r, c * kChunk : (c + 1) * kChunk).
 // maxima: [row][chunk][gpc] group maxima; stats: [row][chunk] x {max (+Inf beside a
 // NaN), sum, rest of the sum, 0}.
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows are 4-byte aligned
-
 __global__ __launch_bounds__(kP1Threads) void topk_chunks_kernel(
     const float* __restrict__ x, int64_t n, int gpc, float inv_temp, int scale,
     float* __restrict__ maxima, float* __restrict__ stats) {
@@ -303,205 +177,13 @@ __global__ __launch_bounds__(kP1Threads) void topk_chunks_kernel(
   }
 }
 
-// ---- log probabilities ----
-//
-// log p(t) = x_t - m - log S and the entropy log S - W / S, with S = sum e^(x - m) and
-// W = sum (x - m) e^(x - m), m the row's maximum.  One pass over the logits: a thread keeps its
-// own maximum and sums, brought to a new maximum when one comes, S <- f S and
-// W <- f (W + (m - m') S) with f = e^(m - m').  Sums are of 64 bits (their additions cost no
-// more than those of 32): log p of a likely token is near 0, and S near 1, whose
-// difference from 1 is what counts.  exp2 of a product rounded once more is off by
-// 2^-23 |x - m|, of terms that are the smaller the larger that is.
-
-// Statistics of a piece of a row: the maximum (+Inf beside a NaN), S in two parts, W.
-struct LogStats {
-  float max, sum, rest, weighted;
-};
-
-constexpr float kLog2E = 1.44269504088896340736f;
-constexpr float kFarBelow = -1e30f;  // stands for distances of -Inf, whose terms are 0
-
-struct LogSums {
-  float m = -__builtin_inff();
-  double s = 0.0, w = 0.0;
-
-  __device__ __forceinline__ void to(float top) {  // a maximum at or above m
-    if (!(top > m)) return;
-    const double low = fmaxf(m - top, kFarBelow);  // m may be -Inf: s and w are 0 then
-    const double f = __builtin_amdgcn_exp2f((float)low * kLog2E);
-    w = f * (w + low * s);
-    s *= f;
-    m = top;
-  }
-  __device__ __forceinline__ void add(float x) {
-    const float low = fmaxf(x - m, kFarBelow);  // of -Inf too, and of -Inf - -Inf
-    const float e = __builtin_amdgcn_exp2f(low * kLog2E);
-    s += (double)e;
-    w = __builtin_fma((double)low, (double)e, w);
-  }
-};
-
-// f of 16 lanes' values, in all of them.
-__device__ __forceinline__ float max_of_16(float g) {
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) g = fmaxf(g, __shfl_xor(g, off, 64));
-  return g;
-}
-
-// Workgroup (p, r) takes the row's `span` chunks from p * span on.  maxima (kGroups): [row][n /
-// 64 rounded up to chunks] group maxima; stats: [row][piece].
-template <bool kGroups>
-__global__ __launch_bounds__(kP1Threads) void logprob_chunks_kernel(
-    const float* __restrict__ x, int64_t n, int chunks, int span, float inv_temp, int scale,
-    float* __restrict__ maxima, LogStats* __restrict__ stats) {
-  __shared__ float fpart[kP1Threads / 64];
-  __shared__ double dpart[kP1Threads / 64];
-  const int64_t r = blockIdx.y;
-  const int tid = threadIdx.x;
-  const float* row = x + r * n;
-  const int first = blockIdx.x * span;
-  const int past = first + span < chunks ? first + span : chunks;
-  constexpr int Q = kChunk / kP1Threads / 4;
-  LogSums sums;
-  bool nan = false;
-  for (int c = first; c < past; ++c) {
-    const int64_t b = (int64_t)c * kChunk;
-    f4 t[Q];
-#pragma unroll
-    for (int j = 0; j < Q; ++j) {
-      const int64_t i = b + 4 * (tid + kP1Threads * j);
-      t[j] = f4{-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
-      if (i + 4 <= n) {
-        t[j] = *reinterpret_cast<const f4*>(row + i);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e < n) t[j][e] = row[i + e];
-      }
-      if (scale)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e < n) t[j][e] = scaled_logit(t[j][e], inv_temp);
-    }
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int j = 0; j < Q; ++j) {
-      float g = -__builtin_inff();
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        nan |= t[j][e] != t[j][e];
-        g = fmaxf(g, t[j][e]);  // ignores NaN
-      }
-      top = fmaxf(top, g);
-      if constexpr (kGroups) {
-        g = max_of_16(g);
-        if ((tid & 15) == 0)
-          maxima[(r * chunks + c) * (kChunk / kGroup) + tid / 16 + kP1Threads / 16 * j] = g;
-      }
-    }
-    sums.to(top);
-#pragma unroll
-    for (int j = 0; j < Q; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sums.add(t[j][e]);
-  }
-  const float mx = block_reduce<kP1Threads>(
-      nan ? __builtin_inff() : sums.m, [](float a, float c) { return fmaxf(a, c); }, fpart);
-  if (mx < __builtin_inff()) sums.to(mx);
-  auto plus = [](double a, double c) { return a + c; };
-  const double s = block_reduce<kP1Threads>(sums.s, plus, dpart);
-  const double w = block_reduce<kP1Threads>(sums.w, plus, dpart);
-  if (tid == 0)
-    stats[r * gridDim.x + blockIdx.x] =
-        LogStats{mx, (float)s, (float)(s - (double)(float)s), (float)w};
-}
-
-// What a row's log probabilities need of it.
-struct RowLog {
-  float max;
-  double log_sum, entropy;
-  bool uniform;  // a row without a finite maximum or with a NaN: every token 1 / n
-};
-
-// From the statistics of a row's pieces, in every thread.
-template <int NT>
-__device__ RowLog row_log(const LogStats* st, int pieces, int64_t n, float* fpart,
-                          double* dpart) {
-  const int tid = threadIdx.x;
-  RowLog row;
-  float mx = -__builtin_inff();
-  for (int c = tid; c < pieces; c += NT) mx = fmaxf(mx, st[c].max);
-  row.max = block_reduce<NT>(mx, [](float a, float c) { return fmaxf(a, c); }, fpart);
-  row.uniform = !(row.max > -__builtin_inff() && row.max < __builtin_inff());
-  double s = 0.0, w = 0.0;
-  if (!row.uniform) {
-    for (int c = tid; c < pieces; c += NT) {
-      const LogStats p = st[c];
-      if (!(p.max > -__builtin_inff())) continue;
-      const double low = (double)p.max - (double)row.max, f = exp(low);
-      const double sum = (double)p.sum + p.rest;
-      s += f * sum;
-      w += f * (p.weighted + low * sum);
-    }
-  }
-  auto plus = [](double a, double c) { return a + c; };
-  s = block_reduce<NT>(s, plus, dpart);
-  w = block_reduce<NT>(w, plus, dpart);
-  row.log_sum = row.uniform ? log((double)n) : log(s);
-  row.entropy = row.uniform ? row.log_sum : row.log_sum - w / s;
-  return row;
-}
-
-// A finite or lower value's log probability.
-__device__ __forceinline__ float log_prob(const RowLog& row, float x) {
-  return (float)((row.uniform ? 0.0 : (double)x - (double)row.max) - row.log_sum);
-}
-
-struct LogOut {
-  const int32_t* tokens;  // `given` of a row
-  int given;
-  float* logprobs;
-  float* entropy;  // may be null
-  const LogStats* stats;
-  int pieces;
-};
-
-// The entropy and the given tokens of row r; an id outside the vocabulary has no probability.
-template <int NT>
-__device__ void write_row(const RowLog& row, const LogOut& o, const float* x, int64_t r,
-                          int64_t n, float inv_temp, int scale) {
-  if (threadIdx.x == 0 && o.entropy != nullptr) o.entropy[r] = (float)row.entropy;
-  for (int j = threadIdx.x; j < o.given; j += NT) {
-    const int32_t t = o.tokens[r * o.given + j];
-    float p = -__builtin_inff();
-    if (t >= 0 && t < n) {
-      const float v = x[r * n + t];
-      p = log_prob(row, scale ? scaled_logit(v, inv_temp) : v);
-    }
-    o.logprobs[r * o.given + j] = p;
-  }
-}
-
-// Where no alternatives are asked for.
-__global__ __launch_bounds__(kP1Threads) void logprob_rows_kernel(const float* __restrict__ x,
-                                                                  int64_t n, float inv_temp,
-                                                                  int scale, LogOut o) {
-  __shared__ float fpart[kP1Threads / 64];
-  __shared__ double dpart[kP1Threads / 64];
-  const int64_t r = blockIdx.x;
-  const RowLog row = row_log<kP1Threads>(o.stats + r * o.pieces, o.pieces, n, fpart, dpart);
-  write_row<kP1Threads>(row, o, x, r, n, inv_temp, scale);
-}
-
 // Pass 2: one workgroup per row over its chunks' statistics and group maxima.  A group
 // here is `gm` consecutive written maxima (a power of two; 1 up to kP2Groups maxima),
-// 2^gshift values; the kk groups' values fit kP2Keys for every accepted n.  kLog: log
-// probabilities, from statistics of their own, in place of probabilities.
-template <bool kLog>
+// 2^gshift values; the kk groups' values fit kP2Keys for every accepted n.
 __global__ __launch_bounds__(kP2Threads) void topk_final_kernel(
     const float* __restrict__ x, const float* __restrict__ maxima,
     const float* __restrict__ stats, int chunks, int gpc, int gm, int gshift, int64_t n, int kk,
-    float inv_temp, int scale, int32_t* __restrict__ ids, float* __restrict__ probs, LogOut o) {
+    float inv_temp, int scale, int32_t* __restrict__ ids, float* __restrict__ probs) {
   __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
   __shared__ SelectLds sm;
   __shared__ uint64_t top[kTopTokensMax];
@@ -532,13 +214,9 @@ __global__ __launch_bounds__(kP2Threads) void topk_final_kernel(
       gv[e] = g;
     }
   }
-  f4 st0 = {};
-  float mx = 0.0f;
-  if constexpr (!kLog) {
-    st0 = *reinterpret_cast<const f4*>(st + 4 * min(tid, chunks - 1));
-    mx = st0.x;
-    for (int c = tid + kP2Threads; c < chunks; c += kP2Threads) mx = fmaxf(mx, st[c * 4]);
-  }
+  const f4 st0 = *reinterpret_cast<const f4*>(st + 4 * min(tid, chunks - 1));
+  float mx = st0.x;
+  for (int c = tid + kP2Threads; c < chunks; c += kP2Threads) mx = fmaxf(mx, st[c * 4]);
   for (int i = tid; i < kBins / 4; i += kP2Threads)
     reinterpret_cast<uint4*>(hist)[i] = uint4{0u, 0u, 0u, 0u};
   if (tid == 0) {
@@ -547,14 +225,7 @@ __global__ __launch_bounds__(kP2Threads) void topk_final_kernel(
     nlist = 0;
     sm.ncand = 0;
   }
-  RowLog row_stats{};
-  if constexpr (kLog) {
-    row_stats = row_log<kP2Threads>(o.stats + r * o.pieces, o.pieces, n, fpart, dpart);
-    mx = row_stats.max;
-    write_row<kP2Threads>(row_stats, o, x, r, n, inv_temp, scale);
-  } else {
-    mx = block_reduce<kP2Threads>(mx, [](float a, float c) { return fmaxf(a, c); }, fpart);
-  }
+  mx = block_reduce<kP2Threads>(mx, [](float a, float c) { return fmaxf(a, c); }, fpart);
   double sum = 0.0;
   const bool finite_max = mx > -__builtin_inff() && mx < __builtin_inff();
   if (finite_max) {
@@ -562,26 +233,19 @@ __global__ __launch_bounds__(kP2Threads) void topk_final_kernel(
 #pragma unroll
     for (int e = 0; e < GPT; ++e)
       count_bin(hist, dist_bin(mx, gv[e]), tid + kP2Threads * e < groups);
-    if constexpr (!kLog) {
-      auto add = [&](const f4 c) {
-        if (c.x > -__builtin_inff()) sum += ((double)c.y + c.z) * exp((double)c.x - (double)mx);
-      };
-      if (tid < chunks) add(st0);
-      for (int c = tid + kP2Threads; c < chunks; c += kP2Threads)
-        add(*reinterpret_cast<const f4*>(st + c * 4));
-    }
+    auto add = [&](const f4 c) {
+      if (c.x > -__builtin_inff()) sum += ((double)c.y + c.z) * exp((double)c.x - (double)mx);
+    };
+    if (tid < chunks) add(st0);
+    for (int c = tid + kP2Threads; c < chunks; c += kP2Threads)
+      add(*reinterpret_cast<const f4*>(st + c * 4));
   }
-  bool uniform = row_stats.uniform;
-  if constexpr (kLog) {
-    __syncthreads();  // the counts
-  } else {
-    sum = block_reduce<kP2Threads>(sum, [](double a, double c) { return a + c; }, dpart);
-    uniform = !finite_max || !(sum > 0.0) || !(sum < __builtin_inf());
-  }
+  sum = block_reduce<kP2Threads>(sum, [](double a, double c) { return a + c; }, dpart);
+  const bool uniform = !finite_max || !(sum > 0.0) || !(sum < __builtin_inf());
   int32_t* oid = ids + r * kk;
   float* opr = probs + r * kk;
   if (uniform) {
-    const float u = kLog ? (float)-row_stats.log_sum : 1.0f / (float)n;
+    const float u = 1.0f / (float)n;
     for (int j = tid; j < kk; j += kP2Threads) {
       oid[j] = j;
       opr[j] = u;
@@ -687,8 +351,7 @@ __global__ __launch_bounds__(kP2Threads) void topk_final_kernel(
   for (int j = tid; j < kk; j += kP2Threads) {
     const uint64_t kv = top[j];
     oid[j] = (int32_t)~(uint32_t)kv;
-    if constexpr (kLog) opr[j] = log_prob(row_stats, key_value(kv));
-    else opr[j] = (float)(exp((double)key_value(kv) - (double)mx) / sum);
+    opr[j] = (float)(exp((double)key_value(kv) - (double)mx) / sum);
   }
 }
 
@@ -723,68 +386,9 @@ hipError_t launch_top_tokens(const float* x, int rows, int64_t n, int top_n, flo
                      0, stream, x, n, gpc, inv_temp, scale ? 1 : 0, maxima, stats);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL(topk_final_kernel<false>, dim3((unsigned)rows), dim3(kP2Threads), 0, stream,
-                     x, maxima, stats, chunks, gpc, gm, gshift, n, kk, inv_temp, scale ? 1 : 0,
-                     ids, probs, LogOut{});
-  return hipGetLastError();
-}
-
-namespace {
-
-// Chunks of a piece of a row: as many workgroups in all as keep the card busy.
-constexpr int64_t kLogPieces = 2048;
-int log_span(int rows, int chunks) {
-  const int64_t span = ((int64_t)rows * chunks + kLogPieces - 1) / kLogPieces;
-  return (int)(span < chunks ? span : chunks);
-}
-
-}  // namespace
-
-size_t token_logprobs_workspace_floats(int rows, int64_t n, int top_n) {
-  // No more pieces than this for these or smaller sizes.
-  const int64_t chunks = topk_chunks(n), all = rows * chunks, most = kLogPieces + rows;
-  return (size_t)(all < most ? all : most) * 4 +
-         (top_n > 0 ? (size_t)all * (kChunk / kGroup) : 0);
-}
-
-hipError_t launch_token_logprobs(const float* x, int rows, int64_t n, float temperature,
-                                 const int32_t* tokens, int given, int top_n, float* logprobs,
-                                 float* entropy, int32_t* top_ids, float* top_logprobs,
-                                 float* workspace, hipStream_t stream) {
-  const int kk = (int)(top_n < n ? top_n : n);
-  if (rows <= 0 || rows > 65535 || n <= 0 || given < 0 || kk < 0 || kk > kTopTokensMax ||
-      (kk > 0 && n > topk_max_n(kk)))
-    return hipErrorInvalidValue;
-  const int chunks = topk_chunks(n), span = log_span(rows, chunks);
-  const int pieces = (chunks + span - 1) / span;
-  LogStats* stats = reinterpret_cast<LogStats*>(workspace);
-  float* maxima = workspace + (size_t)rows * pieces * 4;
-  const bool scale = temperature > 0.0f && temperature != 1.0f;
-  const float inv_temp = scale ? 1.0f / temperature : 1.0f;
-  const LogOut o{tokens, given, logprobs, entropy, stats, pieces};
-  const dim3 grid((unsigned)pieces, (unsigned)rows), block(kP1Threads);
-  if (kk == 0) {
-    hipLaunchKernelGGL(logprob_chunks_kernel<false>, grid, block, 0, stream, x, n, chunks, span,
-                       inv_temp, scale ? 1 : 0, maxima, stats);
-    hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(logprob_rows_kernel, dim3((unsigned)rows), block, 0, stream, x, n,
-                       inv_temp, scale ? 1 : 0, o);
-    return hipGetLastError();
-  }
-  hipLaunchKernelGGL(logprob_chunks_kernel<true>, grid, block, 0, stream, x, n, chunks, span,
-                     inv_temp, scale ? 1 : 0, maxima, stats);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  // Pass 2 groups of gm maxima, as launch_top_tokens has them.
-  constexpr int gpc = kChunk / kGroup;
-  int gm = 1, gshift = 0;
-  while ((int64_t)chunks * gpc > (int64_t)gm * kP2Groups) gm <<= 1;
-  while ((1 << gshift) < kGroup * gm) ++gshift;
-  if (((int64_t)kk << gshift) > kP2Keys) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(topk_final_kernel<true>, dim3((unsigned)rows), dim3(kP2Threads), 0, stream,
-                     x, maxima, nullptr, chunks, gpc, gm, gshift, n, kk, inv_temp, scale ? 1 : 0,
-                     top_ids, top_logprobs, o);
+  hipLaunchKernelGGL(topk_final_kernel, dim3((unsigned)rows), dim3(kP2Threads), 0, stream, x,
+                     maxima, stats, chunks, gpc, gm, gshift, n, kk, inv_temp, scale ? 1 : 0, ids,
+                     probs);
   return hipGetLastError();
 }
 

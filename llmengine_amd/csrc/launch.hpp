@@ -219,12 +219,12 @@ hipError_t launch_top_tokens(const float* x, int rows, int64_t n, int top_n, flo
 
 // Log probabilities of `given` tokens a row, the row's entropy (null: not asked for) and its
 // top_n alternatives (0: none), with the scaling, rows without a distribution and limits of
-// launch_top_tokens.  `workspace` holds token_logprobs_workspace_floats() floats.
-size_t token_logprobs_workspace_floats(int rows, int64_t n, int top_n);
+// launch_top_tokens.  The workspace holds any call of up to these sizes.
+SplitKNeed token_logprobs_workspace(int rows, int64_t n, int top_n);
 hipError_t launch_token_logprobs(const float* x, int rows, int64_t n, float temperature,
                                  const int32_t* tokens, int given, int top_n, float* logprobs,
                                  float* entropy, int32_t* top_ids, float* top_logprobs,
-                                 float* workspace, hipStream_t stream);
+                                 const SplitKWorkspace& ws, hipStream_t stream);
 
 // p[i] = v for i < n (clears workspace counters: a kernel, so that a captured
 // call records no memset node).

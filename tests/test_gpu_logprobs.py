@@ -97,7 +97,9 @@ def check(x, tokens, top_n, temperature, dev, **kw):
     (2, 2049, 9, 128, 1.0), (1, 151936, 1, 0, 1.0), (4, 151936, 4, 20, 0.8),
     (2, 100000, 0, 1, 0.0), (2, 32000, 300, 0, 1.5), (5, 63, 1, 0, 1.0), (3, 65, 2, 64, 2.5),
     (300, 5003, 2, 5, 1.0), (700, 12001, 1, 0, 0.6), (2, 600000, 1, 9, 1.0),
-    (1, 2500000, 2, 2, 1.0), (1, 3000001, 1, 0, 1.0)])
+    (1, 2500000, 2, 2, 1.0), (1, 3000001, 1, 0, 1.0), (520, 40011, 1, 7, 1.0),
+    (60, 400001, 2, 33, 1.0), (530, 3333, 1, 50, 1.1), (9, 33000, 0, 128, 1.0),
+    (17, 8191, 1, 64, 1.0)])
 def test_logprobs(dev, rows, n, given, top_n, temperature):
     note(f"logprobs rows={rows} n={n} given={given} top_n={top_n} t={temperature}")
     rng = np.random.default_rng(n + rows)
