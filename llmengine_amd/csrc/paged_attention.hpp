@@ -75,6 +75,9 @@ constexpr int kUnit = 64;         // keys of a unit of work, and of a stage in L
 // KV heads of 128) that form takes 37 us against 42 with the tiles of many rows, at 7 over
 // 32768 of 8 bits (2 heads of 64) 22 against 148, and nowhere longer.
 constexpr int kTileRows = 128;    // above kFewRows: four waves of 32 rows share the keys in LDS
+// Between: rows of trees, of which a request seldom has more, in tiles of kSomeRows, whose keys
+// the waves split as those of few rows.
+constexpr int kSomeRows = 2 * kFewRows;
 constexpr float kLargest = 0x1.fffffep127f;
 constexpr float kSlack = 8.0f;    // log2 of what a logit may pass the kept maximum by
 constexpr int kDeviceScope = 16;  // cache policy of loads and stores
@@ -96,6 +99,14 @@ constexpr bool kBytes = T == KvType::kInt8;
 // 65536 where the maximum does not lag).
 template <KvType T>
 constexpr float kHeadroom = T == KvType::kBF16 ? -16.0f : 6.0f;
+
+// So far the tiles of kSomeRows go: with the 64 keys of a tile of kTileRows read once instead of
+// twice, f16 caches are faster from 33 rows on (64 rows over 16 requests of 8192: 61 us against
+// 72), the others, whose steps have more to compute, from 65 (8 bits 60 against 66, bf16 73
+// against 77).  Head size 256 leaves no registers for them.
+template <KvType T, int D>
+constexpr int kMostSome =
+    !kTrees || D > 128 ? 0 : T == KvType::kF16 ? kSomeRows : 2 * kSomeRows;
 
 // Two fp32 values as pairs of 16-bit parts that add up to them.
 template <KvType T>
@@ -456,31 +467,39 @@ template <KvType T>
 struct Weights {
   static constexpr int kMany = kParts<T> * 16;
   static constexpr int kFew = kBytes<T> ? 8 : 11;
+  static constexpr int kSome = kFew + 2;
   static constexpr int kTileMany = 80, kTileFew = 40;
   // The least piece of a tile worth a workgroup of its own.
   static constexpr int kLeastMany = kTileMany + kMany, kLeastFew = kTileFew + 20;
 };
 
-template <KvType T>
+template <KvType T, int D>
 __device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Seq& s) {
   constexpr int kMax = 1 << 29;
   const int rows = s.n * a.group;
-  const bool few = rows <= kFewRows;
-  const int unit = few ? Weights<T>::kFew : Weights<T>::kMany;
-  const int fixed = few ? Weights<T>::kTileFew : Weights<T>::kTileMany;
+  const bool few = rows <= kFewRows, some = !few && rows <= kMostSome<T, D>;
+  const int tile_rows = some ? kSomeRows : kTileRows;
+  int unit = few ? Weights<T>::kFew : some ? Weights<T>::kSome : Weights<T>::kMany;
+  // Waves without rows take no time.
+  if (kTrees && !few && !some && rows < kTileRows)
+    unit = Weights<T>::kSome + (unit - Weights<T>::kSome) * ((rows + 31) / 32 - 1) / 3;
+  const int fixed = few || some ? Weights<T>::kTileFew : Weights<T>::kTileMany;
   auto units = [&](int64_t keys) {  // at least a partial one
     const int64_t v = (keys > 0 ? (keys * unit) / kUnit : 0) + unit / 2 + fixed;
     return (int)(v < kMax ? v : kMax);
   };
   Cost c;
-  c.tiles = few ? rows > 0 : (rows + kTileRows - 1) / kTileRows;
-  const int tokens = c.tiles > 1 ? (int)a.by_group.of(kTileRows + a.group - 1) : s.n;
+  c.tiles = few ? rows > 0 : (rows + tile_rows - 1) / tile_rows;
+  const int tokens = c.tiles > 1 ? (int)a.by_group.of(tile_rows + a.group - 1) : s.n;
   const int reach = is_tree(s) ? s.n : tokens;
   c.cap = a.window > 0 ? units((int64_t)a.window + reach) : kMax;
   c.first = units((int64_t)s.pos0 + reach);
-  c.slope = is_tree(s) ? 0 : (int)a.by_group.of(2 * Weights<T>::kMany);  // kTileRows / group keys
+  // From tile to tile tile_rows / group keys more.
+  c.slope = is_tree(s) ? 0
+            : some     ? (int)a.by_group.of(Weights<T>::kSome / 2)
+                       : (int)a.by_group.of(2 * Weights<T>::kMany);
   c.fixed = fixed;
-  c.least = few ? Weights<T>::kLeastFew : Weights<T>::kLeastMany;
+  c.least = few || some ? Weights<T>::kLeastFew : Weights<T>::kLeastMany;
   return c;
 }
 
@@ -535,7 +554,7 @@ struct Schedule {
 // A workgroup's way through its run of the work.  The whole work, `total`, is cut at
 // multiples of `run`; a cut that leaves less than cost.least of a tile before or behind it moves to
 // the tile's begin or end.
-template <KvType T>
+template <KvType T, int D>
 struct Cursor {
   int b, g, t;
   Seq seq;
@@ -553,7 +572,7 @@ struct Cursor {
       seq = uniform(seq);
       if (seq.n > 0) break;
     }
-    cost = cost_of<T>(a, seq);
+    cost = cost_of<T, D>(a, seq);
   }
 
   __device__ __forceinline__ void advance(const AttentionArgs& a, const Schedule& sch,
@@ -642,7 +661,7 @@ struct Cursor {
     s.g = g;
     s.seq = seq;
     const int rows = seq.n * a.group;
-    const int tr = rows <= kFewRows ? kFewRows : kTileRows;
+    const int tr = rows <= kFewRows ? kFewRows : rows <= kMostSome<T, D> ? kSomeRows : kTileRows;
     s.r0 = t * tr;
     s.rows = rows - s.r0 < tr ? rows - s.r0 : tr;
     s.span = span_of(a, seq, s.r0, s.r0 + s.rows);
@@ -753,10 +772,14 @@ __device__ __forceinline__ Tiles find_tile(const AttentionArgs& a, const Segment
 // makes each load one run of memory.  16 columns of q are 16 rows or copies of the last one:
 // the matrix cores are idle for most of the time anyway.  The next tile's first loads go out
 // before the present one is joined and written (32 x <= 4096: 200 -> 182 us).
+//
+// R times 16 rows: a step's keys are multiplied by R operands of q, which then lie in LDS, read
+// anew for each step: in registers beside the loads, the sums of 32 rows of 128 spilled.
 
-template <KvType T, int D>
+template <KvType T, int D, int R>
 struct FewRows {
-  static constexpr int kTiles = kBytes<T> ? 4 : 2;    // cache tiles of a wave's step
+  // Cache tiles of a wave's step.
+  static constexpr int kTiles = kBytes<T> && R == 1 ? 4 : 2;
   static constexpr int kStep = kTiles * kKvTile;
   static constexpr int KK = D / 32, DB = D / 16;
   static constexpr int NQ = (4 * D + kThreads - 1) / kThreads;  // quads of the result a thread
@@ -872,6 +895,7 @@ struct FewRows {
 
   static __device__ __forceinline__ float* out_row(const AttentionArgs& a, const Segment& s,
                                                    int r) {
+    if constexpr (R > 1) r += s.r0;
     const int tok = (int)a.by_group.of(r);
     return a.out + (int64_t)(s.seq.row0 + tok) * a.out_stride +
            (int64_t)(s.g * a.group + r - tok * a.group) * D;
@@ -967,23 +991,36 @@ struct FewRows {
     forget();
     const int tid = fresh_tid(), lane = tid & 63, wave = uniform(tid >> 6);
     const int quad = lane >> 4;
-    const int row = (lane & 15) < s.rows ? lane & 15 : s.rows - 1;
-    const int token = (int)a.by_group.of(row);
-    const Sight mine = sight_of(a, s.seq, row);
+    // The rows of q as operands, of R > 1 in LDS, with their factors and whether they are finite.
+    constexpr int kC = R * kParts<T> * KK * 1024;
+    float* s_c = reinterpret_cast<float*>(smem + kC);
+    uint32_t* s_odd = reinterpret_cast<uint32_t*>(smem + kC + R * 64);
+    // The lane's rows among the request's, or copies of the last one.
+    auto row_of = [&](int r) {
+      const int in = r * 16 + (lane & 15);
+      return (R > 1 ? s.r0 : 0) + (in < s.rows ? in : s.rows - 1);
+    };
+    Sight mine[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) mine[r] = sight_of(a, s.seq, row_of(r));
 
     // Steps of this wave: s.k0 + (wave + 4 i) kStep.
     const int hi = last_key(s);
     Loads& x = n.x;
     Tiles& held = n.held;
-    // Ahead of the first keys, which wait for the table.
-    const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
-                     (int64_t)(s.g * a.group + row - token * a.group) * D + quad * 8;
     f32x4 qv[KK][2];
+    auto load_q = [&](int row) {
+      const int token = (int)a.by_group.of(row);
+      const float* q = a.q + (int64_t)(s.seq.row0 + token) * a.q_stride +
+                       (int64_t)(s.g * a.group + row - token * a.group) * D + quad * 8;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        qv[kk][h] = *reinterpret_cast<const f32x4*>(q + kk * 32 + h * 4);
+        for (int h = 0; h < 2; ++h)
+          qv[kk][h] = *reinterpret_cast<const f32x4*>(q + kk * 32 + h * 4);
+    };
+    // Ahead of the first keys, which wait for the table.
+    if (R == 1 || wave < R) load_q(row_of(R == 1 ? 0 : wave));
     int base = s.k0 + wave * kStep;
     if (!n.started) {
       held = look_up(a, s, lane, base);
@@ -1002,8 +1039,8 @@ struct FewRows {
 
     // q as the right operand: element 8 (l / 16) + e of each run of 32.
     u32x4 qp[kParts<T>][KK];
-    float c;  // logits in units of log2 are S * c
-    {
+    float c[R];  // logits in units of log2 are S * c
+    auto convert = [&](float* c) {
       uint32_t amax = 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
@@ -1011,7 +1048,7 @@ struct FewRows {
         for (int h = 0; h < 2; ++h) amax = max_bits(amax, magnitude(qv[kk][h]));
       amax = with_32(with_16(amax, max_bits), max_bits);
       float up;
-      row_scale<T>(amax, a.scale, &up, &c);
+      row_scale<T>(amax, a.scale, &up, c);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[kParts<T>][4];
@@ -1020,12 +1057,50 @@ struct FewRows {
           split2<T>(qv[kk][i >> 1][(i & 1) * 2] * up, qv[kk][i >> 1][(i & 1) * 2 + 1] * up,
                     &w[0][i], 4);
 #pragma unroll
-        for (int p = 0; p < kParts<T>; ++p) qp[p][kk] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+        for (int p = 0; p < kParts<T>; ++p)
+          qp[p][kk] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
       }
+    };
+    if constexpr (R == 1) {
+      convert(&c[0]);
+    } else {
+      __syncthreads();  // the memory's earlier readers
+      if (wave < R) {   // a block of 16 rows each
+        float mine;
+        convert(&mine);
+        const bool finite = finite_q(qp);
+#pragma unroll
+        for (int p = 0; p < kParts<T>; ++p)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+            reinterpret_cast<u32x4*>(smem)[((wave * kParts<T> + p) * KK + kk) * 64 + lane] =
+                qp[p][kk];
+        if (lane < 16) {
+          s_c[wave * 16 + lane] = mine;
+          s_odd[wave * 16 + lane] = !finite;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < R; ++r) c[r] = s_c[r * 16 + (lane & 15)];
     }
+    auto finite = [&](int r) {
+      if constexpr (R == 1) return finite_q(qp);
+      else return s_odd[r * 16 + (fresh(lane) & 15)] == 0;
+    };
 
-    float m = -INFINITY, l = 0.0f;
-    f32x4 acc[DB] = {};
+    float m[R], l[R];
+    f32x4 acc[R][DB];
+    auto begin = [&] {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[r][db] = f32x4{};
+      }
+    };
+    begin();
     // Twice in the code, so that the first pass has nothing of what only the second does.
     auto pass = [&](auto second) __attribute__((always_inline)) {
       constexpr bool careful = decltype(second)::value;
@@ -1034,41 +1109,75 @@ struct FewRows {
         const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
         const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0;
 
-        float sc[kTiles][4];
+        float sc[R][kTiles][4];
+        if constexpr (R == 1) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          f32x4 r = {};
+          for (int t = 0; t < kTiles; ++t) {
+            f32x4 sum = {};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+              const u32x4 kf = operand(x.k[t][kk]);
+#pragma unroll
+              for (int p = 0; p < kParts<T>; ++p) sum = mfma16<T>(kf, qp[p][kk], sum);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[0][t][i] = sum[i];
+          }
+        } else {
+          const u32x4* s_q = reinterpret_cast<const u32x4*>(smem) + fresh(lane);
+          f32x4 sum[R][kTiles] = {};
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
-            const u32x4 kf = operand(x.k[t][kk]);
+            u32x4 kf[kTiles];
 #pragma unroll
-            for (int p = 0; p < kParts<T>; ++p) r = mfma16<T>(kf, qp[p][kk], r);
+            for (int t = 0; t < kTiles; ++t) kf[t] = operand(x.k[t][kk]);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+              for (int p = 0; p < kParts<T>; ++p) {
+                const u32x4 qf = s_q[((r * kParts<T> + p) * KK + kk) * 64];
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) sum[r][t] = mfma16<T>(kf[t], qf, sum[r][t]);
+              }
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[t][i] = r[i];
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sc[r][t][i] = sum[r][t][i];
         }
         if constexpr (kBytes<T>) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sc[t][i] = __builtin_fmaf(sc[t][i] * c, x.ks[t][i], scale_log2(x.vs[t][i]));
-        } else if (careful && __any(any_nan(sc) & finite_q(qp))) {
-          const AttentionArgs a = fresh_args();
-          const int me = fresh(lane), in = (me & 15) < s.rows ? me & 15 : s.rows - 1;
-          const int tok = (int)a.by_group.of(in);
-          const float* q = a.q + (int64_t)(s.seq.row0 + tok) * a.q_stride +
-                           (int64_t)(s.g * a.group + in - tok * a.group) * D;
-#pragma unroll 1
-          for (int j = 0; j < kTiles * 4; ++j) {
-            const uint16_t* k = static_cast<const uint16_t*>(a.cache.k) +
-                                (j < 4 ? tile[0] : tile[1]) * (kKvTile * D) +
-                                ((me >> 4) * 4 + j % 4) * 8;
-            const float exact = product_of<T, D>(q, k);
+            for (int i = 0; i < 4; ++i) {
+              const float log2_scale = scale_log2(x.vs[t][i]);
 #pragma unroll
-            for (int i = 0; i < kTiles * 4; ++i)
-              if (i == j && sc[i / 4][i % 4] != sc[i / 4][i % 4])
-                sc[i / 4][i % 4] = exact * a.scale;
+              for (int r = 0; r < R; ++r)
+                sc[r][t][i] = __builtin_fmaf(sc[r][t][i] * c[r], x.ks[t][i], log2_scale);
+            }
+        } else if (careful) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (!__any(any_nan(sc[r]) & finite(r))) continue;
+            const AttentionArgs a = fresh_args();
+            const int me = fresh(lane), place = r * 16 + (me & 15);
+            const int in = (R > 1 ? s.r0 : 0) + (place < s.rows ? place : s.rows - 1);
+            const int tok = (int)a.by_group.of(in);
+            const float* q = a.q + (int64_t)(s.seq.row0 + tok) * a.q_stride +
+                             (int64_t)(s.g * a.group + in - tok * a.group) * D;
+#pragma unroll 1
+            for (int j = 0; j < kTiles * 4; ++j) {
+              const uint16_t* k = static_cast<const uint16_t*>(a.cache.k) +
+                                  (j < 4 ? tile[0] : tile[1]) * (kKvTile * D) +
+                                  ((me >> 4) * 4 + j % 4) * 8;
+              const float exact = product_of<T, D>(q, k);
+#pragma unroll
+              for (int i = 0; i < kTiles * 4; ++i)
+                if (i == j && sc[r][i / 4][i % 4] != sc[r][i / 4][i % 4])
+                  sc[r][i / 4][i % 4] = exact * a.scale;
+            }
           }
         }
 
@@ -1086,46 +1195,52 @@ struct FewRows {
         }
 
         if (!whole) {
-          const int from = fresh(base + quad * 4 - (kTrees ? 0 : mine.lo));
-          uint32_t bits = 0;
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            if (kTrees && t % 2 == 0) bits = mine.of(from + t * kKvTile);
+          for (int r = 0; r < R; ++r) {
+            const int from = fresh(base + quad * 4 - (kTrees ? 0 : mine[r].lo));
+            uint32_t bits = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool in = kTrees ? bits >> (t % 2 * kKvTile + i) & 1
-                                     : (uint32_t)(from + t * kKvTile + i) < mine.width;
-              const bool seen = in && !(bad_now >> t & 1);
-              sc[t][i] = seen ? sc[t][i] : -INFINITY;
+            for (int t = 0; t < kTiles; ++t) {
+              if (kTrees && t % 2 == 0) bits = mine[r].of(from + t * kKvTile);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const bool in = kTrees ? bits >> (t % 2 * kKvTile + i) & 1
+                                       : (uint32_t)(from + t * kKvTile + i) < mine[r].width;
+                const bool seen = in && !(bad_now >> t & 1);
+                sc[r][t][i] = seen ? sc[r][t][i] : -INFINITY;
+              }
             }
           }
         }
-        const float to_log2 = kBytes<T> ? 1.0f : c;
-        float top = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
+        for (int r = 0; r < R; ++r) {
+          const float to_log2 = kBytes<T> ? 1.0f : c[r];
+          float top = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
-        top *= to_log2;
-        if (__any(top - m > kSlack)) {
-          top = with_32(with_16(top, max_float), max_float);
-          const float to = fminf(fmaxf(m, top), kLargest);
-          const float keep = to == -INFINITY ? 1.0f : exp2_of(m - to);
-          m = to;
-          l *= keep;
+          for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-          for (int db = 0; db < DB; ++db) acc[db] *= keep;
-        }
-        const float ref = (m == -INFINITY ? 0.0f : m) - kHeadroom<T>;
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[r][t][i]);
+          top *= to_log2;
+          if (__any(top - m[r] > kSlack)) {
+            top = with_32(with_16(top, max_float), max_float);
+            const float to = fminf(fmaxf(m[r], top), kLargest);
+            const float keep = to == -INFINITY ? 1.0f : exp2_of(m[r] - to);
+            m[r] = to;
+            l[r] *= keep;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = exp2_of(__builtin_fmaf(sc[t][i], to_log2, -ref));
-            if constexpr (kBytes<T>) l = __builtin_fmaf(p, scale_inverse(x.vs[t][i]), l);
-            else l += p;
-            sc[t][i] = p;
+            for (int db = 0; db < DB; ++db) acc[r][db] *= keep;
           }
+          const float ref = (m[r] == -INFINITY ? 0.0f : m[r]) - kHeadroom<T>;
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = exp2_of(__builtin_fmaf(sc[r][t][i], to_log2, -ref));
+              if constexpr (kBytes<T>) l[r] = __builtin_fmaf(p, scale_inverse(x.vs[t][i]), l[r]);
+              else l[r] += p;
+              sc[r][t][i] = p;
+            }
+        }
 
         bool odd = false;  // a value of V that is not finite
         if constexpr (!kBytes<T>) {
@@ -1166,24 +1281,32 @@ struct FewRows {
         // wave's halves.
 #pragma unroll
         for (int u = 0; u < kTiles / 2; ++u) {
-          uint32_t w[2][2][kParts<T>];  // [tile][pair][part]
+          u32x4 pp[R][kParts<T>];
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int r = 0; r < R; ++r) {
+            uint32_t w[2][2][kParts<T>];  // [tile][pair][part]
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              split2<T>(sc[2 * u + t][2 * h], sc[2 * u + t][2 * h + 1], &w[t][h][0], 1);
-          u32x4 pp[kParts<T>];
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int p = 0; p < kParts<T>; ++p) {
-            const auto e0 = __builtin_amdgcn_permlane32_swap(w[0][0][p], w[1][0][p], false, false);
-            const auto e1 = __builtin_amdgcn_permlane32_swap(w[0][1][p], w[1][1][p], false, false);
-            pp[p] = u32x4{(uint32_t)e0[0], (uint32_t)e1[0], (uint32_t)e0[1], (uint32_t)e1[1]};
+              for (int h = 0; h < 2; ++h)
+                split2<T>(sc[r][2 * u + t][2 * h], sc[r][2 * u + t][2 * h + 1], &w[t][h][0], 1);
+#pragma unroll
+            for (int p = 0; p < kParts<T>; ++p) {
+              const auto e0 =
+                  __builtin_amdgcn_permlane32_swap(w[0][0][p], w[1][0][p], false, false);
+              const auto e1 =
+                  __builtin_amdgcn_permlane32_swap(w[0][1][p], w[1][1][p], false, false);
+              pp[r][p] =
+                  u32x4{(uint32_t)e0[0], (uint32_t)e1[0], (uint32_t)e0[1], (uint32_t)e1[1]};
+            }
           }
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
             const u32x4 vf = operand(x.v[u][db]);
 #pragma unroll
-            for (int p = 0; p < kParts<T>; ++p) acc[db] = mfma16<T>(vf, pp[p], acc[db]);
+            for (int p = 0; p < kParts<T>; ++p)
+#pragma unroll
+              for (int r = 0; r < R; ++r) acc[r][db] = mfma16<T>(vf, pp[r][p], acc[r][db]);
           }
         }
         if constexpr (!kBytes<T>) {
@@ -1192,7 +1315,10 @@ struct FewRows {
             for (int j = 0; j < kStep; ++j) {
               const int64_t ti = j < kKvTile ? tile_now[0] : tile_now[1];
               const int tok = j % kKvTile, key = base + j;
-              const bool seen = mine.sees(key) && !(bad_now >> (j / kKvTile) & 1);
+              const bool there = !(bad_now >> (j / kKvTile) & 1);
+              bool seen[R];
+#pragma unroll
+              for (int r = 0; r < R; ++r) seen[r] = mine[r].sees(key) && there;
               const uint16_t* p = static_cast<const uint16_t*>(a.cache.v) + ti * (kKvTile * D) +
                                   (tok / 4 % 2) * (D * 8) + (tok / 8) * 4 + tok % 4;
 #pragma unroll
@@ -1200,7 +1326,9 @@ struct FewRows {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const uint32_t v = p[(db * 16 + quad * 4 + i) * 8];
-                  if (seen && is_non_finite<T>(v)) acc[db][i] += value_of<T>(v);
+#pragma unroll
+                  for (int r = 0; r < R; ++r)
+                    if (seen[r] && is_non_finite<T>(v)) acc[r][db][i] += value_of<T>(v);
                 }
             }
           }
@@ -1210,17 +1338,19 @@ struct FewRows {
     };
     pass(std::false_type{});
     if constexpr (!kBytes<T>) {
-      float zero = 0.0f;  // NaN where a sum is not finite
+      bool again = false;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+      for (int r = 0; r < R; ++r) {
+        float zero = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
-        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[db][i], 0.0f, zero);
-      // A row of q that is not finite is NaN either way.
-      if (__any(zero != zero) && __any((zero != zero) & finite_q(qp))) {
-        m = -INFINITY;
-        l = 0.0f;
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = f32x4{};
+          for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[r][db][i], 0.0f, zero);
+        // A row of q that is not finite is NaN either way.
+        if (__any(zero != zero) && __any((zero != zero) & finite(r))) again = true;
+      }
+      if (again) {
+        begin();
         base = s.k0 + wave * kStep;
         held = look_up(a, s, lane, base);
         start(a, s, lane, wave, n);
@@ -1238,64 +1368,82 @@ struct FewRows {
       held = tile_of(a, t, key_of(lane, t.k0 + wave * kStep), then_page);
       start(a, t, lane, wave, n);
     }
-    l = with_32(with_16(l, sum_float), sum_float);
-
-    // Join the four waves; thread tid has the quads tid + 256 i: row tid % 16.
     f32x4* s_acc = reinterpret_cast<f32x4*>(smem);                // [wave][4 D]
     f32x2* s_ml = reinterpret_cast<f32x2*>(smem + 4 * 4 * D * 16);  // [wave][16]
-    __syncthreads();  // the memory's earlier readers
-    const int here = fresh(tid);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-      s_acc[wave * 4 * D + db * 64 + (here & 63)] = acc[db];
-    if ((here & 63) < 16) s_ml[wave * 16 + (here & 15)] = f32x2{m, l};
-    __syncthreads();
-    // Thread tid has the quads tid + 256 i of the result: row tid % 16.
-    const int r = here & 15;
+    const int here = fresh(tid), row = here & 15;
     auto in_range = [&](int i) { return 4 * D % kThreads == 0 || here + i * kThreads < 4 * D; };
-    f32x4 out[NQ] = {};
-    float M = -INFINITY, L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_ml[w * 16 + r].x);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const f32x2 ml = s_ml[w * 16 + r];
-      const float f = weight(ml.x, M);
-      // A NaN row's sum is NaN whatever its weight.
-      L = __builtin_fmaf(ml.y, f, L);
-#pragma unroll
-      for (int i = 0; i < NQ; ++i)
-        if (in_range(i)) out[i] += s_acc[w * 4 * D + here + i * kThreads] * f;
-    }
-
-    if (s.parts > 1) {
-      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
-      const uint32_t to = same_slot_at(sh, s, s.part);
-      if (r < s.rows) {
+    auto write = [&](int r, const f32x4 (&out)[NQ], float L) {
+      if (r * 16 + row < s.rows) {
+        float* o = out_row(a, s, r * 16 + row);
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-          if (in_range(i)) store_part(out[i], rs, here * 16, to + i * kThreads * 16);
-        if (here < 16) store_part2(f32x2{M, L}, rs, here * 8, to + kMl);
+          if (in_range(i))
+            *reinterpret_cast<f32x4*>(o + (here + i * kThreads) / 16 * 4) =
+                L != 0.0f ? out[i] * inv : f32x4{};
       }
-      if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return go_on;
-      if (s.rows <= 8 && s.parts > 8) {
-        join_many(a, s, sh, here, smem);
-        return go_on;
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      l[r] = with_32(with_16(l[r], sum_float), sum_float);
+
+      // Join the four waves; thread tid has the quads tid + 256 i: row tid % 16.
+      __syncthreads();  // the memory's earlier readers
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        s_acc[wave * 4 * D + db * 64 + (here & 63)] = acc[r][db];
+      if ((here & 63) < 16) s_ml[wave * 16 + row] = f32x2{m[r], l[r]};
+      __syncthreads();
+      f32x4 out[NQ] = {};
+      float M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, s_ml[w * 16 + row].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const f32x2 ml = s_ml[w * 16 + row];
+        const float f = weight(ml.x, M);
+        // A NaN row's sum is NaN whatever its weight.
+        L = __builtin_fmaf(ml.y, f, L);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          if (in_range(i)) out[i] += s_acc[w * 4 * D + here + i * kThreads] * f;
       }
+      if (s.parts > 1) {
+        const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
+        const uint32_t to = same_slot_at(sh, s, s.part) + r * Part::kBytes;
+        if (r * 16 + row < s.rows) {
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if (in_range(i)) store_part(out[i], rs, here * 16, to + i * kThreads * 16);
+          if (here < 16) store_part2(f32x2{M, L}, rs, here * 8, to + kMl);
+        }
+      } else {
+        write(r, out, L);
+      }
+    }
+    if (s.parts == 1) return go_on;
+
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
+    if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return go_on;
+    if (R == 1 && s.rows <= 8 && s.parts > 8) {
+      join_many(a, s, sh, here, smem);
+      return go_on;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       // In order, some at a time, whose loads are in flight together.
       constexpr int kAtOnce = 12 / NQ;
-      M = -INFINITY;
-      L = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) out[i] = f32x4{};
+      float M = -INFINITY, L = 0.0f;
+      f32x4 out[NQ] = {};
       for (int p0 = 0; p0 < s.parts; p0 += kAtOnce) {
         f32x2 ml[kAtOnce];
         f32x4 v[kAtOnce][NQ];
 #pragma unroll
         for (int p = 0; p < kAtOnce; ++p) {
           // Past the last part: that one again, not used.
-          const uint32_t from = same_slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
-          ml[p] = load_part2(rs, r * 8, from + kMl);
+          const uint32_t from =
+              same_slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1) + r * Part::kBytes;
+          ml[p] = load_part2(rs, row * 8, from + kMl);
 #pragma unroll
           for (int i = 0; i < NQ; ++i)
             if (in_range(i)) v[p][i] = load_part(rs, here * 16, from + i * kThreads * 16);
@@ -1319,15 +1467,7 @@ struct FewRows {
           }
         }
       }
-    }
-    if (r < s.rows) {
-      float* o = out_row(a, s, r);
-      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-#pragma unroll
-      for (int i = 0; i < NQ; ++i)
-        if (in_range(i))
-          *reinterpret_cast<f32x4*>(o + (here + i * kThreads) / 16 * 4) =
-              L != 0.0f ? out[i] * inv : f32x4{};
+      write(r, out, L);
     }
     return go_on;
   }
@@ -1843,7 +1983,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   __shared__ __attribute__((aligned(16))) uint8_t smem[kLds<T, D>];
   __shared__ Schedule sch;
   // A wave's cursor and next segment, here rather than in registers that its loops need.
-  __shared__ Cursor<T> s_cursor[4];
+  __shared__ Cursor<T, D> s_cursor[4];
   __shared__ Segment s_then[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
 
@@ -1856,7 +1996,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     Seq s{0, 0, 0};
     if (b < a.sequences) s = seq_of(a, b);
     sch.seq[tid] = s;
-    const Cost c = cost_of<T>(a, s);
+    const Cost c = cost_of<T, D>(a, s);
     sum += c.before(c.tiles) * a.cache.kv_heads;
     // More than workgroups are no matter.
     const int64_t n = (int64_t)c.tiles * a.cache.kv_heads;
@@ -1881,7 +2021,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   __syncthreads();
 
   // Runs of equal cost; neighbours on one XCD, whose L2 they share.
-  Cursor<T> cur;
+  Cursor<T, D> cur;
   cur.total = uniform(sch.sum[kThreads - 1]);
   if (cur.total == 0) return;
   // One for each tile, or each least piece of the work if that is more, in eights.
@@ -1909,7 +2049,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     forget();
     const AttentionArgs args = fresh_args();
     const int mine = uniform(fresh_tid() >> 6);
-    Cursor<T> c = s_cursor[mine].uniform_copy();
+    Cursor<T, D> c = s_cursor[mine].uniform_copy();
     Segment then;
     if (!c.next(args, sch, (args.sequences + kThreads - 1) / kThreads, &then)) return false;
     s_cursor[mine] = c;
@@ -1921,26 +2061,38 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     forget();
     return uniform(s_then[uniform(fresh_tid() >> 6)]);
   };
-  auto few = [](const Segment& s) { return s.seq.n * fresh_args().group <= kFewRows; };
-  for (bool have = false;; ) {
+  // 0: few rows, 1: some, 2: many.
+  auto kind_of = [](const Segment& s) {
+    const int rows = s.seq.n * fresh_args().group;
+    return rows <= kFewRows ? 0 : rows <= kMostSome<T, D> ? 1 : 2;
+  };
+  // Segments of one kind, whose loads go out ahead; false at the run's end.
+  bool have = false;
+  auto go = [&]<class Rows>(Rows, int kind, Segment s) __attribute__((always_inline)) {
+    typename Rows::Ahead ahead;
+    Rows::none_ahead(ahead);
+    for (;;) {
+      const bool go_on = Rows::run(
+          s, sh, smem, &s_then[uniform(fresh_tid() >> 6)],
+          [&] {
+            have = next();
+            return have && kind_of(take()) == kind;
+          },
+          ahead);
+      if (!go_on) return have;
+      s = take();
+    }
+  };
+  for (;;) {
     if (!have && !next()) return;
     have = false;
-    Segment s = take();
-    if (few(s)) {
-      typename FewRows<T, D>::Ahead ahead;
-      FewRows<T, D>::none_ahead(ahead);
-      for (;;) {
-        const bool go_on = FewRows<T, D>::run(
-            s, sh, smem, &s_then[uniform(fresh_tid() >> 6)],
-            [&] {
-              have = next();
-              return have && few(take());
-            },
-            ahead);
-        if (!go_on) break;
-        s = take();
-      }
-      if (!have) return;
+    const Segment s = take();
+    const int kind = kind_of(s);
+    if (kind == 0) {
+      if (!go(FewRows<T, D, 1>{}, 0, s)) return;
+    } else if (kMostSome<T, D> > 0 && kind == 1) {
+      if constexpr (kMostSome<T, D> > 0)
+        if (!go(FewRows<T, D, 2>{}, 1, s)) return;
     } else {
       ManyRows<T, D>::run(s, sh, smem);
     }
