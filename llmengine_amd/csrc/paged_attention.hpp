@@ -100,14 +100,6 @@ constexpr bool kBytes = T == KvType::kInt8;
 template <KvType T>
 constexpr float kHeadroom = T == KvType::kBF16 ? -16.0f : 6.0f;
 
-// So far the tiles of kSomeRows go: with the 64 keys of a tile of kTileRows read once instead of
-// twice, f16 caches are faster from 33 rows on (64 rows over 16 requests of 8192: 61 us against
-// 72), the others, whose steps have more to compute, from 65 (8 bits 60 against 66, bf16 73
-// against 77).  Head size 256 leaves no registers for them.
-template <KvType T, int D>
-constexpr int kMostSome =
-    !kTrees || D > 128 ? 0 : T == KvType::kF16 ? kSomeRows : 2 * kSomeRows;
-
 // Two fp32 values as pairs of 16-bit parts that add up to them.
 template <KvType T>
 __device__ __forceinline__ void split2(float a, float b, uint32_t* part, int stride) {
@@ -351,6 +343,21 @@ __device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int b) {
   return s;
 }
 
+// Up to this many rows a request's tiles are of kSomeRows.  They begin and end sooner than those
+// of kTileRows, but two of them read the keys twice: of f16 caches, whose steps have the least to
+// compute, that costs more once the requests together read some 512 MB (as if all were as long as
+// this one).  64 rows of 8 requests, 8 KV heads of 128: up to 1024 keys 21 us against 29, 4096 30
+// against 41; of 16 requests up to 8192 72 against 61.  65 rows and more: of 8 requests of 8192
+// 103 against 66.  Head size 256 leaves no registers for these tiles.
+template <KvType T, int D>
+__device__ __forceinline__ int most_some_rows(const AttentionArgs& a, const Seq& s) {
+  if (!kTrees || D > 128) return 0;
+  if (T != KvType::kF16) return 2 * kSomeRows;
+  const int64_t keys = (int64_t)s.pos0 + s.n;
+  return keys * a.sequences * a.cache.kv_heads < (int64_t(1) << 29) / (4 * D) ? 2 * kSomeRows
+                                                                             : kSomeRows;
+}
+
 __device__ __forceinline__ int clamp_key(int64_t x, int most) {
   return (int)(x < 0 ? 0 : x < most ? x : most);
 }
@@ -477,7 +484,7 @@ template <KvType T, int D>
 __device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Seq& s) {
   constexpr int kMax = 1 << 29;
   const int rows = s.n * a.group;
-  const bool few = rows <= kFewRows, some = !few && rows <= kMostSome<T, D>;
+  const bool few = rows <= kFewRows, some = !few && rows <= most_some_rows<T, D>(a, s);
   const int tile_rows = some ? kSomeRows : kTileRows;
   int unit = few ? Weights<T>::kFew : some ? Weights<T>::kSome : Weights<T>::kMany;
   // Waves without rows take no time.
@@ -661,7 +668,9 @@ struct Cursor {
     s.g = g;
     s.seq = seq;
     const int rows = seq.n * a.group;
-    const int tr = rows <= kFewRows ? kFewRows : rows <= kMostSome<T, D> ? kSomeRows : kTileRows;
+    const int tr = rows <= kFewRows                        ? kFewRows
+                   : rows <= most_some_rows<T, D>(a, seq) ? kSomeRows
+                                                          : kTileRows;
     s.r0 = t * tr;
     s.rows = rows - s.r0 < tr ? rows - s.r0 : tr;
     s.span = span_of(a, seq, s.r0, s.r0 + s.rows);
@@ -2063,8 +2072,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   };
   // 0: few rows, 1: some, 2: many.
   auto kind_of = [](const Segment& s) {
-    const int rows = s.seq.n * fresh_args().group;
-    return rows <= kFewRows ? 0 : rows <= kMostSome<T, D> ? 1 : 2;
+    const AttentionArgs a = fresh_args();
+    const int rows = s.seq.n * a.group;
+    return rows <= kFewRows ? 0 : rows <= most_some_rows<T, D>(a, s.seq) ? 1 : 2;
   };
   // Segments of one kind, whose loads go out ahead; false at the run's end.
   bool have = false;
@@ -2090,8 +2100,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     const int kind = kind_of(s);
     if (kind == 0) {
       if (!go(FewRows<T, D, 1>{}, 0, s)) return;
-    } else if (kMostSome<T, D> > 0 && kind == 1) {
-      if constexpr (kMostSome<T, D> > 0)
+    } else if (kTrees && D <= 128 && kind == 1) {
+      if constexpr (kTrees && D <= 128)
         if (!go(FewRows<T, D, 2>{}, 1, s)) return;
     } else {
       ManyRows<T, D>::run(s, sh, smem);
