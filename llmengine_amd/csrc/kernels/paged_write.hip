@@ -22,8 +22,10 @@
 //
 // With weights, q and k are first normed, row by row of a head: x w / sqrt(mean x^2 + eps),
 // then rotated.  All of it in 64 bits, rounded once, so that 8-bit quants do not depend on the
-// order of the sum either; the sum is a few lane exchanges, and the lanes of a row past its
-// head_dim take part in them with zeros.
+// order of the sum either; the sum is a few lane exchanges, in which the lanes of a row past its
+// head_dim take part with zeros.  That takes the 8192 tokens above 95 us, 3.8 TB/s, 11 more
+// than without norms (86 registers, with nothing kept from one head to the next 76: 101 -> 95;
+// held to 64 they spill: 215), and 37 tokens of 14 heads of 64 6.6 us.
 #include "../paged.hpp"
 #include "../q8_0_device.hpp"
 
@@ -70,40 +72,70 @@ __device__ __forceinline__ void rotate8(Row8& r, const float* rope_row, int s, b
   }
 }
 
-__device__ __forceinline__ double from_lane_xor(double v, int off) {
+// The sum over a group of LPR lanes, the same bits in all of them: with the neighbour, the
+// other pair, and the lanes mirrored in 8 and 16.
+template <int kCtrl>
+__device__ __forceinline__ double in_row(double v) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, off);
-  const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(u >> 32), off);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, 0xf, 0xf,
+                                                            false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl,
+                                                            0xf, 0xf, false);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-
-// 1 / sqrt(mean x^2 + eps) of a head's row held by LPR lanes.
 template <int LPR>
-__device__ __forceinline__ double inverse_rms(const Row8& r, int head_dim, double eps) {
+__device__ __forceinline__ double sum_of(double v) {
+  v += in_row<0xb1>(v);
+  v += in_row<0x4e>(v);
+  v += in_row<0x141>(v);
+  if (LPR >= 16) v += in_row<0x140>(v);
+  if (LPR >= 32) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, 16);
+    const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(u >> 32), 16);
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  }
+  return v;
+}
+
+// 1 / sqrt(mean x^2 + eps) of a head's row held by LPR lanes: the instruction's estimate is good
+// to some 2^-24, and squared by each of two steps of Newton's method, which 0 and infinity are
+// kept from.
+template <int LPR>
+__device__ __forceinline__ double inverse_rms(const Row8& r, double inverse_dim, double eps) {
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)r.x[i], (double)r.x[i], sum);
+  const double a = __builtin_fma(sum_of<LPR>(sum), inverse_dim, eps);
+  const double y = __builtin_amdgcn_rsq(a);
+  double z = y;
 #pragma unroll
-  for (int off = LPR / 2; off > 0; off >>= 1) sum += from_lane_xor(sum, off);
-  return 1.0 / __builtin_sqrt(sum / head_dim + eps);
+  for (int i = 0; i < 2; ++i) z = z * __builtin_fma(-0.5 * a * z, z, 1.5);
+  return a > 0.0 && a < __builtin_inf() ? z : y;
 }
 
-// x w inv of a lane's 8 elements, turned as rotate8 turns them where `turns`.
-__device__ __forceinline__ void norm8(Row8& r, const Row8& w, double inv, const float* rope_row,
-                                      int s, bool halves, bool turns) {
+__device__ __forceinline__ void anew(Row8& r) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm("" : "+v"(r.x[i]));
+}
+
+// x w inv of a lane's 8 elements, turned by `t` as rotate8 turns them where `turns`.
+__device__ __forceinline__ void norm8(Row8& r, const Row8& w, double inv, const Row8& t,
+                                      bool halves, bool turns) {
   double x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (double)r.x[i] * inv * (double)w.x[i];
   if (turns) {
-    const f32x4 t0 = *reinterpret_cast<const f32x4*>(rope_row + 8 * s);
-    const f32x4 t1 = *reinterpret_cast<const f32x4*>(rope_row + 8 * s + 4);
-    const double c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
+    auto turn64 = [&](double& a, double& b, int i) {
+      const double c = t.x[2 * i], n = t.x[2 * i + 1];
+      const double to = __builtin_fma(a, c, -(b * n));
+      b = __builtin_fma(a, n, b * c);
+      a = to;
+    };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int p = halves ? i : 2 * i, q = halves ? 4 + i : 2 * i + 1;
-      const double a = x[p], b = x[q];
-      x[p] = __builtin_fma(a, c[i], -(b * n[i]));
-      x[q] = __builtin_fma(a, n[i], b * c[i]);
+      if (halves) turn64(x[i], x[4 + i], i);
+      else turn64(x[2 * i], x[2 * i + 1], i);
     }
   }
 #pragma unroll
@@ -170,7 +202,11 @@ __device__ __forceinline__ void put1(void* base, int64_t at, uint32_t c) {
 constexpr int kQHeads = 2;
 
 // LPR lanes (a power of two, at least head_dim / 8) take one head's row of one token.
-template <KvType T, int LPR, bool kNorm>
+// With norms, a kernel for each kind of rotation: 64-bit values chosen among at run time cost
+// moves and registers.
+enum Norm { kNoNorm, kNormPairs, kNormHalves };
+
+template <KvType T, int LPR, Norm kOf>
 __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const int G = a.cache.kv_heads, D = a.cache.head_dim, P = a.cache.page_size;
   // The first workgroups take k and v, head by head, the others q, token by token.
@@ -183,7 +219,8 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
   const int t = (int)(is_q ? item / q_items : item % (uint32_t)a.tokens);
   const int h = (int)(is_q ? item % q_items : item / (uint32_t)a.tokens);
   const bool live = s * 8 < D;
-  const bool halves = a.rope_halves != 0;
+  constexpr bool kNorm = kOf != kNoNorm;
+  const bool halves = kNorm ? kOf == kNormHalves : a.rope_halves != 0;
   int pos = 0;
   bool placed = true;
   if (a.rope != nullptr) {
@@ -201,16 +238,24 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
     const int n = a.heads - h * kQHeads;  // heads from here on
     Row8 r[kQHeads];
     if constexpr (kNorm) {
-      Row8 w = {};
-      if (live) w = load8(a.q_norm, sp);
+      Row8 w = {}, t = {};
 #pragma unroll
       for (int i = 0; i < kQHeads; ++i) {
         r[i] = {};
         if (i < n && live) r[i] = load8(q + i * D, sp);
       }
+      if (live) w = load8(a.q_norm, sp);
+      if (turns) t = load8(rope_row, {8 * s, 8 * s + 4});
 #pragma unroll
-      for (int i = 0; i < kQHeads; ++i)
-        norm8(r[i], w, inverse_rms<LPR>(r[i], D, a.eps), rope_row, s, halves, turns);
+      for (int i = 0; i < kQHeads; ++i) {
+        // One head after the other, nothing of 64 bits kept for the next: registers.
+        if (i > 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          anew(w);
+          anew(t);
+        }
+        norm8(r[i], w, inverse_rms<LPR>(r[i], a.inverse_dim, a.eps), t, halves, turns);
+      }
       if (!live) return;
     } else {
 #pragma unroll
@@ -242,9 +287,10 @@ __global__ __launch_bounds__(256) void paged_kv_write_kernel(KvWriteArgs a) {
     Row8 r = {};
     if (live) r = load8(a.k + t * a.k_stride + (int64_t)g * D, sp);
     if constexpr (kNorm) {
-      Row8 w = {};
+      Row8 w = {}, t = {};
       if (live) w = load8(a.k_norm, sp);
-      norm8(r, w, inverse_rms<LPR>(r, D, a.eps), rope_row, s, halves, turns && live);
+      if (turns && live) t = load8(rope_row, {8 * s, 8 * s + 4});
+      norm8(r, w, inverse_rms<LPR>(r, a.inverse_dim, a.eps), t, halves, turns && live);
       if (!live) r = {};  // 0 times an infinity
     } else if (turns && live) {
       rotate8(r, rope_row, s, halves);
@@ -322,18 +368,20 @@ hipError_t launch_typed(const KvWriteArgs& a, hipStream_t stream) {
   const KvWriteBlocks n =
       paged_kv_write_blocks(a.tokens, a.heads, a.cache.kv_heads, a.cache.head_dim);
   b.kv_blocks = (uint32_t)n.kv;
+  b.inverse_dim = 1.0 / a.cache.head_dim;
   const dim3 grid((unsigned)(n.kv + n.q)), block(256);
-  auto launch = [&](auto norm) {
-    constexpr bool kNorm = decltype(norm)::value;
+  auto launch = [&](auto of) {
+    constexpr Norm kOf = decltype(of)::value;
     if (lpr == 8)
-      hipLaunchKernelGGL((paged_kv_write_kernel<T, 8, kNorm>), grid, block, 0, stream, b);
+      hipLaunchKernelGGL((paged_kv_write_kernel<T, 8, kOf>), grid, block, 0, stream, b);
     else if (lpr == 16)
-      hipLaunchKernelGGL((paged_kv_write_kernel<T, 16, kNorm>), grid, block, 0, stream, b);
+      hipLaunchKernelGGL((paged_kv_write_kernel<T, 16, kOf>), grid, block, 0, stream, b);
     else
-      hipLaunchKernelGGL((paged_kv_write_kernel<T, 32, kNorm>), grid, block, 0, stream, b);
+      hipLaunchKernelGGL((paged_kv_write_kernel<T, 32, kOf>), grid, block, 0, stream, b);
   };
-  if (a.q_norm != nullptr) launch(std::true_type{});
-  else launch(std::false_type{});
+  if (a.q_norm == nullptr) launch(std::integral_constant<Norm, kNoNorm>{});
+  else if (a.rope_halves != 0) launch(std::integral_constant<Norm, kNormHalves>{});
+  else launch(std::integral_constant<Norm, kNormPairs>{});
   return hipGetLastError();
 }
 

@@ -90,7 +90,8 @@ struct KvWriteArgs {
   const float* q_norm;  // weights of the norms of q's and k's heads, both or (null) none
   const float* k_norm;
   double eps;
-  uint32_t kv_blocks;  // set by the launcher
+  uint32_t kv_blocks;  // set by the launcher, as is:
+  double inverse_dim;  // 1 / head_dim
 };
 // Workgroups of the write: for k and v, then for q.
 struct KvWriteBlocks {
