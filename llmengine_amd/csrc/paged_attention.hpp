@@ -705,21 +705,57 @@ __device__ __forceinline__ uint32_t same_slot_at(const Shared& sh, const Segment
   return (uint32_t)uniform((int)slot_at(sh, s, part));
 }
 
-__device__ __forceinline__ bool last_to_arrive(const Shared& sh, const Segment& s, int* shared) {
+// Whether this workgroup is the last of `all` at a counter.
+__device__ __forceinline__ bool last_to_arrive(uint32_t* c, int all, int* shared) {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_waitcnt(0);  // this wave's part has reached the coherence point
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __syncthreads();
   if (threadIdx.x == 0) {
-    uint32_t* c = sh.counters + s.first * kCounterStride;
     const int n = (int)__hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     *shared = n;
-    if (n == s.parts - 1)  // nobody else comes: zero again for the next launch
+    if (n == all - 1)  // nobody else comes: zero again for the next launch
       __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  return *shared == s.parts - 1;
+  return *shared == all - 1;
+}
+
+// Parts of a tile that are joined before all of them are.  One workgroup alone reads a part of
+// 128 rows of 256 in about a microsecond: 20 tokens of 8 heads over 8000 keys took 135 us, and 59
+// in groups; 64 of 14 heads of 64 over 20000 54 and 37.  Up to 12 parts a second wait for the
+// counter costs what it saves.
+__device__ __forceinline__ int parts_of_group(int parts) {
+  return !kTrees || parts <= 12 ? parts : parts <= 64 ? 8 : parts <= 144 ? 12 : 24;
+}
+
+// Joins a tile's parts, in order, whichever workgroup comes last: join(first, step, count) adds
+// up the parts first, first + step, .. into registers, keep(part) makes them that part.  Says
+// whether this workgroup has them all.  A group's counter lies beside that of a tile that would
+// begin with the group's first workgroup; a last part alone, whose workgroup may begin one, needs
+// none.
+template <class Join, class Keep>
+__device__ __forceinline__ bool join_parts(const Shared& sh, const Segment& s, int* shared,
+                                           Join join, Keep keep) {
+  uint32_t* tile = sh.counters + s.first * kCounterStride;
+  const int size = parts_of_group(s.parts);
+  if (!kTrees || size >= s.parts) {
+    if (!last_to_arrive(tile, s.parts, shared)) return false;
+    join(0, 1, s.parts);
+    return true;
+  }
+  const int first = s.part / size * size;
+  const int count = s.parts - first < size ? s.parts - first : size;
+  if (count > 1) {
+    if (!last_to_arrive(tile + first * kCounterStride + 1, count, shared)) return false;
+    join(first, 1, count);
+    keep(first);
+  }
+  const int groups = (s.parts + size - 1) / size;
+  if (!last_to_arrive(tile, groups, shared)) return false;
+  join(0, size, groups);
+  return true;
 }
 
 // Parts lie at `slot` + `at` bytes: what lanes share, and what they do not.
@@ -1392,6 +1428,17 @@ struct FewRows {
                 L != 0.0f ? out[i] * inv : f32x4{};
       }
     };
+    // A row's part, of which the rows past the tile's are not read.
+    auto store = [&](int r, int part, const f32x4 (&out)[NQ], float M, float L) {
+      const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
+      const uint32_t to = same_slot_at(sh, s, part) + r * Part::kBytes;
+      if (r * 16 + row < s.rows) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          if (in_range(i)) store_part(out[i], rs, here * 16, to + i * kThreads * 16);
+        if (here < 16) store_part2(f32x2{M, L}, rs, here * 8, to + kMl);
+      }
+    };
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l[r] = with_32(with_16(l[r], sum_float), sum_float);
@@ -1417,67 +1464,72 @@ struct FewRows {
         for (int i = 0; i < NQ; ++i)
           if (in_range(i)) out[i] += s_acc[w * 4 * D + here + i * kThreads] * f;
       }
-      if (s.parts > 1) {
-        const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
-        const uint32_t to = same_slot_at(sh, s, s.part) + r * Part::kBytes;
-        if (r * 16 + row < s.rows) {
-#pragma unroll
-          for (int i = 0; i < NQ; ++i)
-            if (in_range(i)) store_part(out[i], rs, here * 16, to + i * kThreads * 16);
-          if (here < 16) store_part2(f32x2{M, L}, rs, here * 8, to + kMl);
-        }
-      } else {
-        write(r, out, L);
-      }
+      if (s.parts > 1) store(r, s.part, out, M, L);
+      else write(r, out, L);
     }
     if (s.parts == 1) return go_on;
 
-    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
-    if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return go_on;
+    int* arrived = reinterpret_cast<int*>(smem);
     if (R == 1 && s.rows <= 8 && s.parts > 8) {
-      join_many(a, s, sh, here, smem);
+      if (last_to_arrive(sh.counters + s.first * kCounterStride, s.parts, arrived))
+        join_many(a, s, sh, here, smem);
       return go_on;
     }
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
+    float M[R], L[R];
+    f32x4 out[R][NQ];
+    const bool whole = join_parts(
+        sh, s, arrived,
+        [&](int first, int step, int count) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      // In order, some at a time, whose loads are in flight together.
-      constexpr int kAtOnce = 12 / NQ;
-      float M = -INFINITY, L = 0.0f;
-      f32x4 out[NQ] = {};
-      for (int p0 = 0; p0 < s.parts; p0 += kAtOnce) {
-        f32x2 ml[kAtOnce];
-        f32x4 v[kAtOnce][NQ];
+          for (int r = 0; r < R; ++r) {
+            // Some at a time, whose loads are in flight together.
+            constexpr int kAtOnce = 12 / NQ;
+            M[r] = -INFINITY;
+            L[r] = 0.0f;
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) {
-          // Past the last part: that one again, not used.
-          const uint32_t from =
-              same_slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1) + r * Part::kBytes;
-          ml[p] = load_part2(rs, row * 8, from + kMl);
+            for (int i = 0; i < NQ; ++i) out[r][i] = f32x4{};
+            for (int p0 = 0; p0 < count; p0 += kAtOnce) {
+              f32x2 ml[kAtOnce];
+              f32x4 v[kAtOnce][NQ];
 #pragma unroll
-          for (int i = 0; i < NQ; ++i)
-            if (in_range(i)) v[p][i] = load_part(rs, here * 16, from + i * kThreads * 16);
-        }
-        float top = M;
+              for (int p = 0; p < kAtOnce; ++p) {
+                // Past the last part: that one again, not used.
+                const int part = first + step * (p0 + p < count ? p0 + p : count - 1);
+                const uint32_t from = same_slot_at(sh, s, part) + r * Part::kBytes;
+                ml[p] = load_part2(rs, row * 8, from + kMl);
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) top = fmaxf(top, ml[p].x);
-        const float keep = weight(M, top);
-        M = top;
-        L *= keep;
+                for (int i = 0; i < NQ; ++i)
+                  if (in_range(i)) v[p][i] = load_part(rs, here * 16, from + i * kThreads * 16);
+              }
+              float top = M[r];
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) out[i] *= keep;
+              for (int p = 0; p < kAtOnce; ++p) top = fmaxf(top, ml[p].x);
+              const float keep = weight(M[r], top);
+              M[r] = top;
+              L[r] *= keep;
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) {
-          if (p0 + p < s.parts) {
-            const float f = weight(ml[p].x, M);
-            L = __builtin_fmaf(ml[p].y, f, L);
+              for (int i = 0; i < NQ; ++i) out[r][i] *= keep;
 #pragma unroll
-            for (int i = 0; i < NQ; ++i)
-              if (in_range(i)) out[i] += v[p][i] * f;
+              for (int p = 0; p < kAtOnce; ++p) {
+                if (p0 + p < count) {
+                  const float f = weight(ml[p].x, M[r]);
+                  L[r] = __builtin_fmaf(ml[p].y, f, L[r]);
+#pragma unroll
+                  for (int i = 0; i < NQ; ++i)
+                    if (in_range(i)) out[r][i] += v[p][i] * f;
+                }
+              }
+            }
           }
-        }
-      }
-      write(r, out, L);
-    }
+        },
+        [&](int part) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) store(r, part, out[r], M[r], L[r]);
+        });
+    if (whole)
+#pragma unroll
+      for (int r = 0; r < R; ++r) write(r, out[r], L[r]);
     return go_on;
   }
 };
@@ -1911,58 +1963,67 @@ struct ManyRows {
       constexpr uint32_t kMl = kTileRows * D * 4;
       const int at = fresh(tid);
       const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(sh.partials, sh.bytes);
-      const uint32_t to = same_slot_at(sh, s, s.part);
-      if (wrow < s.rows) {
+      auto store = [&](int part) {
+        const uint32_t to = same_slot_at(sh, s, part);
+        if (wrow < s.rows) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+          for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            store_part(f32x4{acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2],
-                             acc[db][4 * q + 3]},
-                       rs, at * 16, to + (db * 4 + q) * kThreads * 16);
-        store_part2(f32x2{m, l}, rs, at * 8, to + kMl);
-      }
-      if (!last_to_arrive(sh, s, reinterpret_cast<int*>(smem))) return;
-      if (wrow >= s.rows) return;
-      // In order, some at a time: their loads are in flight together.
-      constexpr int kAtOnce = D <= 64 ? 4 : D <= 128 ? 2 : 1, kQuads = D / 8;
-      m = -INFINITY;
-      l = 0.0f;
+            for (int q = 0; q < 4; ++q)
+              store_part(f32x4{acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2],
+                               acc[db][4 * q + 3]},
+                         rs, at * 16, to + (db * 4 + q) * kThreads * 16);
+          store_part2(f32x2{m, l}, rs, at * 8, to + kMl);
+        }
+      };
+      store(s.part);
+      const bool whole = join_parts(
+          sh, s, reinterpret_cast<int*>(smem),
+          [&](int first, int step, int count) {
+            if (wrow >= s.rows) return;
+            // Some at a time: their loads are in flight together.
+            constexpr int kAtOnce = D <= 64 ? 4 : D <= 128 ? 2 : 1, kQuads = D / 8;
+            m = -INFINITY;
+            l = 0.0f;
 #pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+            for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
 #pragma unroll 1
-      for (int p0 = 0; p0 < s.parts; p0 += kAtOnce) {
-        f32x2 ml[kAtOnce];
-        f32x4 v[kAtOnce][kQuads];
+            for (int p0 = 0; p0 < count; p0 += kAtOnce) {
+              f32x2 ml[kAtOnce];
+              f32x4 v[kAtOnce][kQuads];
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) {
-          // Past the last part: that one again, with no weight.
-          const uint32_t from = same_slot_at(sh, s, p0 + p < s.parts ? p0 + p : s.parts - 1);
-          ml[p] = load_part2(rs, at * 8, from + kMl);
+              for (int p = 0; p < kAtOnce; ++p) {
+                // Past the last part: that one again, with no weight.
+                const int part = first + step * (p0 + p < count ? p0 + p : count - 1);
+                const uint32_t from = same_slot_at(sh, s, part);
+                ml[p] = load_part2(rs, at * 8, from + kMl);
 #pragma unroll
-          for (int q = 0; q < kQuads; ++q)
-            v[p][q] = load_part(rs, at * 16, from + q * kThreads * 16);
-        }
-        float to = m;
+                for (int q = 0; q < kQuads; ++q)
+                  v[p][q] = load_part(rs, at * 16, from + q * kThreads * 16);
+              }
+              float to = m;
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) to = fmaxf(to, ml[p].x);
-        const float keep = weight(m, to);
-        m = to;
-        l *= keep;
+              for (int p = 0; p < kAtOnce; ++p) to = fmaxf(to, ml[p].x);
+              const float keep = weight(m, to);
+              m = to;
+              l *= keep;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] *= keep;
+              for (int db = 0; db < DB; ++db) acc[db] *= keep;
 #pragma unroll
-        for (int p = 0; p < kAtOnce; ++p) {
-          if (p0 + p < s.parts) {
-            const float f = weight(ml[p].x, m);
-            l = __builtin_fmaf(ml[p].y, f, l);
+              for (int p = 0; p < kAtOnce; ++p) {
+                if (p0 + p < count) {
+                  const float f = weight(ml[p].x, m);
+                  l = __builtin_fmaf(ml[p].y, f, l);
 #pragma unroll
-            for (int q = 0; q < kQuads; ++q)
+                  for (int q = 0; q < kQuads; ++q)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) acc[q / 4][q % 4 * 4 + i] += v[p][q][i] * f;
-          }
-        }
-      }
+                    for (int i = 0; i < 4; ++i) acc[q / 4][q % 4 * 4 + i] += v[p][q][i] * f;
+                }
+              }
+            }
+          },
+          store);
+      if (!whole || wrow >= s.rows) return;
     }
     if (wrow < s.rows) {
       const float inv = 1.0f / l;

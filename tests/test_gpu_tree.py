@@ -193,6 +193,22 @@ def test_tree_long_context(dev, kv_type):
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+def test_tree_tiles_in_many_parts(dev, kv_type, D):
+    """One tile, or two, of every height in so many parts that groups of them are joined
+    first; the sums do not depend on which workgroup comes last."""
+    for lens in ([(4, 12000, "tree")], [(7, 14001, "tree")], [(13, 9000, "tree")],
+                 [(50, 11000, "tree")], [(60, 5000, "tree"), (11, 7777, "run")],
+                 [(66, 9009, "tree")]):
+        note(f"tree many parts {kv_type} D={D} {lens}")
+        b = Trees(dev, kv_type, 2, 1, D, 64, lens, seed=D)
+        out = b.run().clone()
+        b.check(out)
+        for _ in range(4):
+            assert bool((b.run() == out).all())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
 @pytest.mark.parametrize("n", [3, 40, 150])
 def test_tree_rows_that_see_nothing(dev, kv_type, n):
     """Masks without a bit, over no cached token, are rows of zeros; over cached ones they see
