@@ -261,6 +261,13 @@ Status argmax(const float* logits, int rows, int n, int32_t* idx, float* val = n
 // [rows][min(top_n, n)] of each logits row, largest probability first.
 Status top_tokens(const float* logits, int rows, int n, int top_n, float temperature,
                   int32_t* ids, float* probs, hipStream_t stream = nullptr);
+// Log probabilities of given tokens [rows][tokens_per_row], entropies [rows] and the top_n
+// tokens with their log probabilities of each logits row (mle_token_logprobs_f32; no
+// counterpart in the reference).
+Status token_logprobs(const float* logits, int rows, int n, float temperature,
+                      const int32_t* tokens, int tokens_per_row, int top_n, float* logprobs,
+                      float* entropy = nullptr, int32_t* top_ids = nullptr,
+                      float* top_logprobs = nullptr, hipStream_t stream = nullptr);
 }  // namespace hip
 
 }  // namespace minillm

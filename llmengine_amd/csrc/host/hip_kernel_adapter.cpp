@@ -436,6 +436,15 @@ Status top_tokens(const float* logits, int rows, int n, int top_n, float tempera
   return from_capi(mle_top_tokens_f32(logits, rows, n, top_n, temperature, ids, probs, stream));
 }
 
+Status token_logprobs(const float* logits, int rows, int n, float temperature,
+                      const int32_t* tokens, int tokens_per_row, int top_n, float* logprobs,
+                      float* entropy, int32_t* top_ids, float* top_logprobs,
+                      hipStream_t stream) {
+  return from_capi(mle_token_logprobs_f32(logits, rows, n, temperature, tokens, tokens_per_row,
+                                          top_n, logprobs, entropy, top_ids, top_logprobs,
+                                          stream));
+}
+
 size_t q8_0_tiled_bytes(int N, int K) { return mle_q8_0_tiled_bytes(N, K); }
 
 Status tile_q8_0(const uint8_t* w_q8_0, uint8_t* w_tiled, int N, int K, hipStream_t stream) {

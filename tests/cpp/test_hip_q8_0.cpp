@@ -701,6 +701,62 @@ static void test_fused_launchers() {
   std::printf("  PASS test_fused_launchers\n");
 }
 
+static void test_token_logprobs_launcher() {
+  // Log probabilities, entropies and alternatives against 64-bit sums.
+  // A term e^-d is off by less than (d + 1) 2^-22 of itself: log p by the mean of that and its
+  // own rounding, the entropy by the mean weighted with |log p| + 2 and by W / S in 24 bits.
+  const int M = 3, N = 4100, top = 3, per = 2;
+  std::vector<float> g(M * N);
+  for (int i = 0; i < M * N; ++i) g[i] = float((i * 7919) % 10007 - 5003) * 0x1p-9f;
+  DevBuf<float> dy(M * N);
+  dy.put(g);
+  std::vector<int32_t> ask(M * per);
+  for (int i = 0; i < M * per; ++i) ask[i] = i % 5 == 4 ? N : (i * 7) % N;
+  DevBuf<int32_t> da(M * per), tid(M * top);
+  DevBuf<float> lp(M * per), en(M), tlp(M * top);
+  da.put(ask);
+  check_status(hip::token_logprobs(dy.p, M, N, 1.0f, da.p, per, top, lp.p, en.p, tid.p, tlp.p));
+  const auto l = lp.get(), e = en.get(), t = tlp.get();
+  const auto ti = tid.get();
+  for (int m = 0; m < M; ++m) {
+    const float* v = &g[m * N];
+    const double mx = *std::max_element(v, v + N);
+    double sum = 0, mean = 0, off = 0, off_h = 0;
+    for (int n = 0; n < N; ++n) sum += std::exp(v[n] - mx);
+    auto want = [&](int id) { return v[id] - mx - std::log(sum); };
+    for (int n = 0; n < N; ++n) {
+      const double d = mx - v[n], p = std::exp(-d) / sum;
+      mean += p * d;
+      if (d > 0) off += p * (d + 1) * 0x1p-22;
+      if (d > 0) off_h += p * (d + 1) * (2 - want(n)) * 0x1p-22;
+    }
+    off_h += mean * 0x1p-23;
+    auto close = [&](double got, double right, double tol) {
+      CHECK(std::fabs(got - right) <= tol + std::fabs(right) * 0x1p-24);
+    };
+    for (int j = 0; j < per; ++j) {
+      const int id = ask[m * per + j];
+      if (id == N) CHECK(std::isinf(l[m * per + j]) && l[m * per + j] < 0);
+      else close(l[m * per + j], want(id), off);
+    }
+    close(e[m], std::log(sum) + mean, off_h);
+    std::vector<int> order(N);
+    for (int n = 0; n < N; ++n) order[n] = n;
+    std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return v[a] > v[b]; });
+    for (int j = 0; j < top; ++j) {
+      CHECK(ti[m * top + j] == order[j]);
+      close(t[m * top + j], want(order[j]), off);
+    }
+  }
+  check_status(hip::token_logprobs(dy.p, M, N, 1.0f, da.p, per, 0, lp.p));
+  CHECK(lp.get() == l);
+  CHECK(hip::token_logprobs(dy.p, M, N, 1.0f, nullptr, per, 0, lp.p).code() ==
+        ErrorCode::InvalidArgument);
+  CHECK(hip::token_logprobs(dy.p, M, N, 1.0f, da.p, per, 129, lp.p, en.p, tid.p, tlp.p).code() ==
+        ErrorCode::Unsupported);
+  std::printf("  PASS test_token_logprobs_launcher\n");
+}
+
 static void test_executor_fusion_end_to_end() {
   // x -> {gate, up} -> SwiGLU -> down, plus q / k / v on x; the fused executor
   // against the unfused one (bitwise for M < 64, the same kernels' arithmetic;
@@ -1609,6 +1665,7 @@ int main() {
   test_executor_prefill_linear();
   test_gguf_model_end_to_end();
   test_fused_launchers();
+  test_token_logprobs_launcher();
   test_executor_fusion_end_to_end();
   test_executor_tiled_weights();
   test_executor_rows_decode();
