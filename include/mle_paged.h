@@ -236,8 +236,8 @@ int mle_paged_tree_attention(const mle_paged_cache* cache, const float* q, int q
  * [sequences][keep_stride]; keep_counts[b] < 0 keeps every row (a prompt's chunk).  A path
  * ends before an entry that is not above the one before it or not a row of the request, and at
  * keep_stride entries.  What the cache holds past the kept tokens is left as it was.
- *   kept_lens[b] = base + the rows kept (may be the cached_lens that the plan read, not
- *     kv_lens).  Of a request that the plan refused (granted[b] == 0) it is not written; one
+ *   kept_lens[b] = base + the rows kept (may be the cached_lens that the plan read, not what
+ *     this call reads).  Of a request that the plan refused (granted[b] == 0) it is not written; one
  *     with kv_lens[b] < n keeps kv_lens[b] and nothing moves.
  *   The pages that held only rows which did not stay go on top of the free stack, in the order
  *   of the requests and of the table row, which is left as it was; free_count_out (may be
@@ -245,7 +245,8 @@ int mle_paged_tree_attention(const mle_paged_cache* cache, const float* q, int q
  *   back, the counts may be NULL (a second group of layers).
  * A token in a page outside [0, num_pages) neither moves nor is written over.  One launch for
  * up to 64 layers; no workspace.  Deterministic.
- * Errors: NULL or misaligned pointers, sizes <= 0, kept_lens == kv_lens -> InvalidArgument;
+ * Errors: NULL or misaligned pointers, sizes <= 0, kept_lens over another argument's memory,
+ * the same cache twice -> InvalidArgument;
  * caches of different type or sizes -> ShapeMismatch; more than 31 bits of max_pages *
  * page_size or sequences * max_pages, or as many threads as a launch does not hold (64 for
  * each layer, request and KV head) -> Unsupported.

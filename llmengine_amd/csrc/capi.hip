@@ -1546,6 +1546,11 @@ int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* 
       return fail(MLE_SHAPE_MISMATCH, std::string("hip ") + ctx + ": cache " +
                                           std::to_string(i) +
                                           " differs from cache 0 in type or sizes");
+    for (int j = 0; j < i; ++j)
+      if (caches[i].k == caches[j].k || caches[i].v == caches[j].v)
+        return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": caches " +
+                                              std::to_string(j) + " and " + std::to_string(i) +
+                                              " are the same memory");
   }
   const struct { const void* p; const char* name; bool need; } bufs[] = {
       {block_table, "block_table", true}, {kv_lens, "kv_lens", true},
@@ -1561,9 +1566,6 @@ int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* 
   MLE_TRY(check_positive(ctx, sequences, "sequences"));
   MLE_TRY(check_positive(ctx, max_pages, "max_pages"));
   MLE_TRY(check_positive(ctx, keep_stride, "keep_stride"));
-  if (kept_lens == kv_lens)
-    return fail(MLE_INVALID_ARGUMENT,
-                std::string("hip ") + ctx + ": kept_lens must not be kv_lens, which the move reads");
   if ((int64_t)max_pages * caches->page_size > INT32_MAX - 65536 ||
       (int64_t)sequences * max_pages > INT32_MAX)
     return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
@@ -1573,6 +1575,18 @@ int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* 
   if (mle::paged_keep_blocks(most, sequences, caches->kv_heads) >= mle::kMostBlocks)
     return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
                                      ": layers * sequences * kv_heads take more than 2^32 threads");
+  // Other workgroups read these while the lengths are written.
+  const struct { const int32_t* p; const char* name; int64_t n; } read[] = {
+      {kv_lens, "kv_lens", sequences},
+      {cu_tokens, "cu_tokens", (int64_t)sequences + 1},
+      {granted, "granted", sequences},
+      {keep_counts, "keep_counts", sequences},
+      {keep, "keep", (int64_t)sequences * keep_stride},
+      {block_table, "block_table", (int64_t)sequences * max_pages}};
+  for (const auto& r : read)
+    if (kept_lens < r.p + r.n && r.p < kept_lens + sequences)
+      return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": kept_lens must not overlap " +
+                                            r.name + ", which the move reads");
   mle::KeepArgs a{};
   a.num_pages = caches->num_pages;
   a.page_size = caches->page_size;

@@ -63,10 +63,10 @@ __device__ __forceinline__ int64_t cell_of(const KeepArgs& a, int b, int pos, in
 
 // The kept lengths, and the pages past them onto the stack, by one workgroup.
 __device__ __forceinline__ void keep_lengths(const KeepArgs& a) {
-  __shared__ int wave_pages[kWaves];
+  __shared__ int64_t wave_pages[kWaves];  // up to 31 bits in all, and the stack's
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int most = a.max_pages * a.page_size;
-  int top = 0;
+  int64_t top = 0;
   if (a.stack != nullptr) {
     top = *a.count;
     top = top < 0 ? 0 : top < a.num_pages ? top : a.num_pages;
@@ -95,15 +95,15 @@ __device__ __forceinline__ void keep_lengths(const KeepArgs& a) {
     }
     if (a.stack == nullptr) continue;
     const int mine = past - first;
-    int upto = mine;
+    int64_t upto = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(upto, off);
+      const int64_t o = __shfl_up(upto, off);
       if (lane >= off) upto += o;
     }
     if (lane == 63) wave_pages[wave] = upto;
     __syncthreads();
-    int at = top + upto - mine;
+    int64_t at = top + upto - mine;
     for (int w = 0; w < kWaves; ++w) {
       if (w < wave) at += wave_pages[w];
       top += wave_pages[w];
@@ -113,7 +113,7 @@ __device__ __forceinline__ void keep_lengths(const KeepArgs& a) {
     top = top < a.num_pages ? top : a.num_pages;
     __syncthreads();  // wave_pages is written anew
   }
-  if (a.stack != nullptr && tid == 0) *a.count_out = top;
+  if (a.stack != nullptr && tid == 0) *a.count_out = (int)top;
 }
 
 // E bytes an element; a wave moves one head's path of one layer.  The first workgroup has the

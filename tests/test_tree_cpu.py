@@ -34,8 +34,12 @@ def attention(c=None, **kw):
     return capi.paged_tree_attention_status(**a)
 
 
+def layer(i, **kw):
+    return cache(k=(2 * i + 3) * FAKE, v=(2 * i + 4) * FAKE, **kw)
+
+
 def keep(caches=None, **kw):
-    a = dict(caches=capi.PagedCaches(caches if caches is not None else [cache(), cache()]),
+    a = dict(caches=capi.PagedCaches(caches if caches is not None else [layer(0), layer(1)]),
              block_table=FAKE, max_pages=4, kv_lens=FAKE, cu_tokens=FAKE, granted=FAKE,
              sequences=2, keep=FAKE, keep_stride=3, keep_counts=FAKE, kept_lens=2 * FAKE,
              free_pages=FAKE, free_count=FAKE, free_count_out=FAKE, stream=0)
@@ -122,7 +126,13 @@ def test_keep_pointers(name):
 @pytest.mark.parametrize("bad,code,text", [
     (dict(free_pages=ODD), INVALID, "free_pages"), (dict(sequences=0), INVALID, "sequences"),
     (dict(max_pages=-1), INVALID, "max_pages"), (dict(keep_stride=0), INVALID, "keep_stride"),
-    (dict(kept_lens=FAKE), INVALID, "kept_lens must not be kv_lens"),
+    (dict(kept_lens=FAKE), INVALID, "kept_lens must not overlap kv_lens"),
+    (dict(kv_lens=2 * FAKE + 4), INVALID, "kept_lens must not overlap kv_lens"),
+    (dict(cu_tokens=2 * FAKE - 8), INVALID, "kept_lens must not overlap cu_tokens"),
+    (dict(granted=2 * FAKE), INVALID, "kept_lens must not overlap granted"),
+    (dict(keep_counts=2 * FAKE), INVALID, "kept_lens must not overlap keep_counts"),
+    (dict(keep=2 * FAKE - 20), INVALID, "kept_lens must not overlap keep"),
+    (dict(block_table=2 * FAKE - 28), INVALID, "kept_lens must not overlap block_table"),
     (dict(max_pages=1 << 28), UNSUPPORTED, "31 bits"),
     (dict(sequences=1 << 29), UNSUPPORTED, "31 bits"),
     (dict(sequences=1 << 26, max_pages=1), UNSUPPORTED, "2^32 threads"),
@@ -135,10 +145,17 @@ def test_keep_refusals(bad, code, text):
 @pytest.mark.parametrize("other", [dict(num_pages=9), dict(page_size=32), dict(kv_heads=1),
                                    dict(head_dim=128), dict(kv_type="bf16")])
 def test_keep_of_unlike_caches(other):
-    got, msg = keep([cache(), cache(), cache(**other)])
+    got, msg = keep([layer(0), layer(1), layer(2, **other)])
     assert got == MISMATCH and "cache 2 differs" in msg, (got, msg)
     got, msg = keep([])
     assert got == INVALID and "layers" in msg
+
+
+def test_keep_of_a_cache_twice():
+    """Two layers of the same memory would move each other's rows."""
+    for other in (layer(0), cache(k=99 * FAKE, v=4 * FAKE), cache(k=3 * FAKE, v=99 * FAKE)):
+        got, msg = keep([layer(0), layer(1), other])
+        assert got == INVALID and "caches 0 and 2 are the same memory" in msg, (got, msg)
 
 
 @pytest.mark.parametrize("bad,code,text", [
