@@ -19,6 +19,12 @@
 // A row is cut into pieces, one workgroup each; the one that arrives last at the row's counter
 // joins their statistics in order and does the rest.  What the others wrote passes their XCD's
 // cache (device-scope stores and loads).  No result depends on the order of arrival.
+//
+// What bounds it (MI355X; 622 MB are read at 5.65 TB/s): reading the logits, for many rows.  1024
+// rows of 151936 with 20 alternatives 127 us, 4.9 TB/s, 110 for a plain read; an exponential, a
+// 64-bit addition and an fma a value take a SIMD's time beside it.  208 rows of 32000 14.6 us (5
+// for a read) and one of 151936 without alternatives 5.7 us are latencies: loads, the counter,
+// the join and the selection, one after the other.
 #include "../launch.hpp"
 #include "../paged.hpp"
 #include "../select.hpp"

@@ -5,6 +5,15 @@
 // base + i, for i < keep_counts[b]; rows increase along a path, keep[b][i] >= i, so what a later
 // entry reads no earlier one overwrites, and some entries at a time are read before they are
 // written.  A path ends before the first entry that is not above the one before it, or not a row.
+//
+// A wave has one head's path in one layer: the entries of one wave come in order, and nothing of
+// a path crosses waves.  What bounds it: a chain of latencies (lengths, entries, page table,
+// cells, stores; 1 x 8 nodes in 24 layers 6.4 us, next to 3.3 of an empty launch), and for more
+// the lines of the cache that tokens lie in beside others: a token's K is D / 8 pieces of 16
+// bytes (8 of 8 bits) 256 bytes apart, its V single elements 16 bytes apart.  32 trees of 64
+// nodes, up to 8 of them kept, in 32 layers of 8-bit pages 20 us (13 where the lines are in a
+// cache still).  With 48 kept of each 150 us, one entry at a time 232, 4 160; of f16 pages 267,
+// 340 and 194, but 4 take 24 us instead of 16 where up to 8 are kept, as most paths are.
 #include "../paged.hpp"
 
 namespace mle {

@@ -23,9 +23,10 @@
 // With weights, q and k are first normed, row by row of a head: x w / sqrt(mean x^2 + eps),
 // then rotated.  All of it in 64 bits, rounded once, so that 8-bit quants do not depend on the
 // order of the sum either; the sum is a few lane exchanges, in which the lanes of a row past its
-// head_dim take part with zeros.  That takes the 8192 tokens above 95 us, 3.8 TB/s, 11 more
-// than without norms (86 registers, with nothing kept from one head to the next 76: 101 -> 95;
-// held to 64 they spill: 215), and 37 tokens of 14 heads of 64 6.6 us.
+// head_dim take part with zeros.  That takes the 8192 tokens above 90 us, 4.0 TB/s, 6 more
+// than without norms (with nothing kept from one head to the next 101 -> 95; sums over lanes and
+// the inverse root without a call -> 90; held to 64 registers it spills: 215), and 37 tokens of
+// 14 heads of 64 6.7 us, as much as without.
 #include "../paged.hpp"
 #include "../q8_0_device.hpp"
 

@@ -60,6 +60,13 @@
 //     issued between the matrix instructions changed nothing.
 //   short calls: a chain of latencies (lengths, run, page table, keys) of 6 us for few rows
 //     and 12 for many: 129 tokens of 14 heads 8.7 us.
+//   trees: as few or many rows, by the query heads of their nodes.  8 nodes over 129 tokens, 14
+//     heads 11.5 us.  16 trees of 26 over up to 4096, 32 heads (383 MB) 89 us = 4.3 TB/s: 5 us
+//     of beginning, units of 2.4 us beside another workgroup, runs that end between 63 and 90.
+//     8 trees of 64 over up to 32768 of 8 bits, 32 heads over 8 203 us = 0.78 PFLOP/s of parts:
+//     matrix cores busy in 35% of the cycles, 1.5 waves a SIMD, since of the two workgroups of a
+//     CU the older one's waves go first and it is done at 167 us, the other alone by 210.
+//     Priorities that changed from unit to unit made their ends equal and the call no shorter.
 #pragma once
 
 #include "launch.hpp"
@@ -451,7 +458,10 @@ struct Cost {
   int tiles;
   int first, slope, cap;
   int fixed;  // of a tile's cost, what is not its units
-  int least;  // the least piece of a tile worth a workgroup of its own
+  int least;  // the least piece of a tile worth a workgroup of its own, its fixed cost in it
+
+  // The least one at a tile's end.
+  __device__ __forceinline__ int last() const { return kTrees ? least - fixed : least; }
 
   __device__ __forceinline__ int of(int t) const {
     const int64_t v = (int64_t)first + (int64_t)t * slope;
@@ -624,7 +634,7 @@ struct Cursor {
     begin = i0;
     if (at - i0 >= (uint64_t)cost.least) {
       begin = at;
-      if (i1 - at < (uint64_t)cost.least) {
+      if (i1 - at < (uint64_t)cost.last()) {
         if (i1 < total) advance(a, sch, chunk);
         else done = true;
       }
@@ -662,7 +672,7 @@ struct Cursor {
   __device__ __forceinline__ bool next(const AttentionArgs& a, const Schedule& sch, int chunk,
                                        Segment* out) {
     if (done || end <= i0 || (end < i1 && end - i0 < (uint64_t)cost.least)) return false;
-    const uint64_t stop = (int64_t)(i1 - end) < cost.least ? i1 : end;
+    const uint64_t stop = (int64_t)(i1 - end) < cost.last() ? i1 : end;
     Segment s;
     s.b = b;
     s.g = g;
@@ -681,7 +691,7 @@ struct Cursor {
     s.part = s.first = 0;
     if (begin != i0 || stop != i1) {
       // The cuts inside the tile.
-      const uint64_t lo = i0 + cost.least, hi = i1 - cost.least;
+      const uint64_t lo = i0 + cost.least, hi = i1 - cost.last();
       const int c0 = (int)quotient(lo + run - 1, run), c1 = (int)quotient(hi, run);
       s.first = c0 - 1;
       s.part = w - s.first;
