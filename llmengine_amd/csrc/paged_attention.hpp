@@ -61,12 +61,13 @@
 //   short calls: a chain of latencies (lengths, run, page table, keys) of 6 us for few rows
 //     and 12 for many: 129 tokens of 14 heads 8.7 us.
 //   trees: as few or many rows, by the query heads of their nodes.  8 nodes over 129 tokens, 14
-//     heads 11.5 us.  16 trees of 26 over up to 4096, 32 heads (383 MB) 89 us = 4.3 TB/s: 5 us
-//     of beginning, units of 2.4 us beside another workgroup, runs that end between 63 and 90.
-//     8 trees of 64 over up to 32768 of 8 bits, 32 heads over 8 203 us = 0.78 PFLOP/s of parts:
-//     matrix cores busy in 35% of the cycles, 1.5 waves a SIMD, since of the two workgroups of a
-//     CU the older one's waves go first and it is done at 167 us, the other alone by 210.
-//     Priorities that changed from unit to unit made their ends equal and the call no shorter.
+//     heads 11.4 us.  16 trees of 26 over up to 4096, 32 heads (383 MB) 90 us = 4.3 TB/s: 5 us
+//     of beginning, units of 2.4 us beside another workgroup, runs that end between 64 and 94.
+//     8 trees of 64 over up to 32768 of 8 bits, 32 heads over 8 201 us = 0.79 PFLOP/s of parts:
+//     matrix cores busy in 34% of the cycles, 1.5 waves a SIMD, since of the two workgroups of a
+//     CU the older one's waves go first and it is done at 165 us, the other by 206.  Priorities
+//     that changed from unit to unit brought their ends together, longer runs for the older ones
+//     likewise, and the call was no shorter by either.
 #pragma once
 
 #include "launch.hpp"
@@ -460,7 +461,10 @@ struct Cost {
   int fixed;  // of a tile's cost, what is not its units
   int least;  // the least piece of a tile worth a workgroup of its own, its fixed cost in it
 
-  // The least one at a tile's end.
+  // The least one at a tile's end.  A tile's fixed cost is in the account where it begins, so a
+  // run that takes up only its end, and goes on with the next, is no longer than others; one
+  // prolonged to the tile's end is, and the next is shorter (2 x 40 rows of 32 heads over 600 keys
+  // 27 us so and 22 with this, 64 of 28 over 20000 73 and 64).
   __device__ __forceinline__ int last() const { return kTrees ? least - fixed : least; }
 
   __device__ __forceinline__ int of(int t) const {
@@ -569,8 +573,8 @@ struct Schedule {
 };
 
 // A workgroup's way through its run of the work.  The whole work, `total`, is cut at
-// multiples of `run`; a cut that leaves less than cost.least of a tile before or behind it moves to
-// the tile's begin or end.
+// multiples of `run`; a cut that leaves less than cost.least of a tile before it, or cost.last()
+// behind it, moves to the tile's begin or end.
 template <KvType T, int D>
 struct Cursor {
   int b, g, t;
