@@ -353,7 +353,7 @@ def test_tree_strides_streams_and_repeats(dev, kv_type):
     b.run(out=same, q=same)
     torch.cuda.synchronize()
     assert torch.equal(same, first)
-    stream = torch.cuda.Stream()
+    stream = own_stream()
     for _ in range(3):
         other = empty_f32(first.shape, dev)
         torch.cuda.synchronize()
@@ -371,7 +371,7 @@ def test_tree_graph_replays(dev, kv_type):
     c = Trees(dev, kv_type, 8, 2, 64, 32, [(4, 1000, "any"), (40, 300, "run"), (2, 70, "tree")],
               seed=2)
     eager = [x.run() for x in (b, c)]
-    stream = torch.cuda.Stream()
+    stream = own_stream()
     capi.workspace_reserve(*capi.paged_attention_workspace_size(b.cache, 8, 3, b.T),
                            stream=stream)
     torch.cuda.synchronize()
