@@ -875,3 +875,100 @@ def test_steps_of_speculation(dev, kv_type, window):
                     slack = 0.0 if exact else 2.0 * {"f16": 2.0 ** -10, "bf16": 2.0 ** -7,
                                                      "int8": 1 / 127}[kv_type]
                     assert (np.abs(x - want) <= slack * np.abs(want).max(initial=0)).all()
+
+
+@pytest.mark.parametrize("kv_type", ["int8", "f16"])
+def test_far_pages(dev, kv_type):
+    """Pages more than 2^32 elements and bytes into a cache: the write, the attention and the
+    move do there what they do in near pages, bit for bit."""
+    import torch
+    H, G, D, page, T, pages = 16, 8, 256, 64, 100, 4
+    first = 2 ** 32 // (G * page * D) + 9
+    note(f"far pages {kv_type}")
+    rng = np.random.default_rng(3)
+    host = rng.standard_normal((T, (H + 2 * G) * D)).astype(np.float32)
+    mask, depth = tree_masks(rng, T, "tree")
+    path = np.flatnonzero(mask[T - 1])
+    w = torch.ones(D, device=dev)
+    outs = []
+    for start in (0, first):
+        cache = capi.PagedCache.allocate(kv_type, start + pages, page, G, D, dev)
+        q, k, v = to_dev(host, dev).split([H * D, G * D, G * D], dim=1)
+        order = start + np.array([2, 0, 3, 1])
+        table, kv, cu = i32(order[None], dev), i32([150], dev), i32([0, T], dev)
+        at = 50 + np.arange(T)
+        slots = i32(order[at // page] * page + at % page, dev)
+        capi.paged_kv_write_normed(cache, q, q, H, k, v, w, w, 1e-6, None, 0, D, "none", None,
+                                   slots, T)
+        out = empty_f32((T, H * D), dev)
+        capi.paged_tree_attention(cache, q, out, H, D ** -0.5, 0, table, pages, kv, cu, 1, T,
+                                  to_dev(words_of(mask, 2), dev), 2)
+        kept, count = i32([0], dev), i32([0], dev)
+        stack = i32(np.full(start + pages, -1), dev)
+        capi.paged_kv_keep(capi.PagedCaches([cache]), table, pages, kv, cu, i32([1], dev), 1,
+                           i32(path[None], dev), len(path), i32([len(path)], dev), kept, stack,
+                           count, count)
+        torch.cuda.synchronize()
+        part = [x[start * (x.numel() // (start + pages)):].clone()
+                for x in (cache.k, cache.v, cache.k_scale, cache.v_scale) if x is not None]
+        near = [x[:start * (x.numel() // (start + pages))] for x in (cache.k, cache.v)]
+        assert not any(bool(x.view(torch.uint8)[i::4096].any()) for x in near for i in (0, 2049))
+        n = int(count.item())
+        outs.append(part + [out, kept, stack[:n] - start])
+        del cache, near
+    assert len(outs[0][-1]) > 0 and outs[0][-2].item() == 50 + len(path)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_calls_at_once_and_others_between(dev):
+    """Calls on two streams at once have workspaces of their own; calls of other kinds on the
+    same stream find its counters as they leave them."""
+    import torch
+    big = Trees(dev, "f16", 2, 1, 128, 64, [(50, 11000, "tree")], seed=4)
+    few = Trees(dev, "f16", 2, 1, 128, 64, [(4, 12000, "tree"), (13, 700, "tree")], seed=5)
+    x = torch.randn(3, 40000, device=dev)
+    want = [b.run().clone() for b in (big, few)]
+    ids = torch.empty(3, dtype=torch.int32, device=dev)
+    lp, tok = empty_f32((3, 1), dev), i32([[5], [39999], [0]], dev)
+    streams = [own_stream(), own_stream()]
+    outs = [[empty_f32(w.shape, dev) for _ in range(8)] for w in want]
+    torch.cuda.synchronize()
+    note("trees on two streams, other calls between")
+    for i in range(8):
+        for b, s, o in zip((big, few), streams, outs):
+            b.run(out=o[i], stream=s)
+        capi.argmax(x, 3, 40000, ids, stream=streams[0])
+        capi.token_logprobs(x, 3, 40000, tok, 1, 0, lp, None, None, None, stream=streams[0])
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        for y in o:
+            assert torch.equal(y, w)
+    assert torch.equal(ids.long(), x.argmax(1))
+    # A term's error is (distance to the maximum + 1) 2^-22, and no two of 120000 normal values
+    # are 11 apart.
+    right = torch.log_softmax(x.double(), 1).gather(1, tok.long())
+    assert bool(((lp - right).abs() <= 2.0 ** -22 * 12 + right.abs() * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_tree_many_requests(dev, kv_type):
+    """More requests than a workgroup has threads, trees of every size, runs and none in turn."""
+    rng = np.random.default_rng(9)
+    kinds = ["tree", "run", "any", "chain", "none"]
+    for B in (257, 700):
+        lens = []
+        for b in range(B):
+            n = int(rng.choice([0, 1, 2, 5, 16, 17, 33, 70]))
+            lens.append((n, n + int(rng.choice([0, 1, 40, 100])), kinds[b % 5]))
+        note(f"tree many requests {kv_type} {B}")
+        b = Trees(dev, kv_type, 2, 1, 64, 16, lens, seed=B, window=30 if B == 700 else 0)
+        b.check(b.run())
+
+
+def test_tree_widest_masks(dev):
+    """More nodes than the widest masks name: the last ones are seen by none."""
+    n = 64 * 64 + 70
+    note("tree widest masks")
+    b = Trees(dev, "f16", 1, 1, 64, 64, [(n, n + 100, "tree"), (3, 9, "tree")], words=64)
+    b.check(b.run())
