@@ -237,8 +237,8 @@ int mle_paged_tree_attention(const mle_paged_cache* cache, const float* q, int q
  * ends before an entry that is not above the one before it or not a row of the request, and at
  * keep_stride entries.  What the cache holds past the kept tokens is left as it was.
  *   kept_lens[b] = base + the rows kept (may be the cached_lens that the plan read, not what
- *     this call reads).  Of a request that the plan refused (granted[b] == 0) it is not written; one
- *     with kv_lens[b] < n keeps kv_lens[b] and nothing moves.
+ *     this call reads).  Of a request that the plan refused (granted[b] == 0) it is not
+ *     written; one with kv_lens[b] < n keeps kv_lens[b] and nothing moves.
  *   The pages that held only rows which did not stay go on top of the free stack, in the order
  *   of the requests and of the table row, which is left as it was; free_count_out (may be
  *   free_count) = the pages then free, at most num_pages.  free_pages NULL: no pages go
