@@ -356,11 +356,13 @@ __device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int b) {
 // compute, that costs more once the requests together read some 512 MB (as if all were as long as
 // this one).  64 rows of 8 requests, 8 KV heads of 128: up to 1024 keys 21 us against 29, 4096 30
 // against 41; of 16 requests up to 8192 72 against 61.  65 rows and more: of 8 requests of 8192
-// 103 against 66.  Head size 256 leaves no registers for these tiles.
+// 103 against 66.  At head size 256, 16 x 12 rows of 16 heads over 8 (24 a tile) over 8192 of f16,
+// bf16 and 8 bits 101, 106 and 62 us against 129, 190 and 135 with the tiles of many rows, whose one
+// workgroup a CU hides less; so there f16 ones take two as well, 16 x 26 of them 129 against 135.
 template <KvType T, int D>
 __device__ __forceinline__ int most_some_rows(const AttentionArgs& a, const Seq& s) {
-  if (!kTrees || D > 128) return 0;
-  if (T != KvType::kF16) return 2 * kSomeRows;
+  if (!kTrees) return 0;
+  if (T != KvType::kF16 || D > 128) return 2 * kSomeRows;
   const int64_t keys = (int64_t)s.pos0 + s.n;
   return keys * a.sequences * a.cache.kv_heads < (int64_t(1) << 29) / (4 * D) ? 2 * kSomeRows
                                                                              : kSomeRows;
@@ -1160,6 +1162,16 @@ struct FewRows {
       }
     };
     begin();
+    // The sums of 32 rows of 256 lie where only matrix instructions reach them, as far as it
+    // goes: beside 16-bit loads in flight they would take all the others, and those loads were
+    // spilled as they came (16 x 26 rows of 16 heads over 8192: 278 us, so 134).
+    auto set_aside = [&] {
+      if constexpr (R == 2 && D > 128 && !kBytes<T>)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) asm("" : "+a"(acc[r][db]));
+    };
     // Twice in the code, so that the first pass has nothing of what only the second does.
     auto pass = [&](auto second) __attribute__((always_inline)) {
       constexpr bool careful = decltype(second)::value;
@@ -1168,6 +1180,7 @@ struct FewRows {
         const uint32_t bad_now = (uint32_t)(bad >> (at * kTiles)) & ((1u << kTiles) - 1);
         const bool whole = base >= s.span.lo_all && base + kStep <= s.span.hi_all && bad_now == 0;
 
+        set_aside();
         float sc[R][kTiles][4];
         if constexpr (R == 1) {
 #pragma unroll
@@ -1336,6 +1349,7 @@ struct FewRows {
           }
         }
 
+        set_aside();
         // P as the right operand: tokens 4 h' .. of a pair of tiles, by one exchange of the
         // wave's halves.
 #pragma unroll
@@ -2175,8 +2189,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
     const int kind = kind_of(s);
     if (kind == 0) {
       if (!go(FewRows<T, D, 1>{}, 0, s)) return;
-    } else if (kTrees && D <= 128 && kind == 1) {
-      if constexpr (kTrees && D <= 128)
+    } else if (kTrees && kind == 1) {
+      if constexpr (kTrees)
         if (!go(FewRows<T, D, 2>{}, 1, s)) return;
     } else {
       ManyRows<T, D>::run(s, sh, smem);

@@ -253,11 +253,11 @@ def test_tree_bad_pages_and_short_lengths(dev, kv_type):
 
 
 @pytest.mark.parametrize("kv_type", ("f16", "bf16"))
-@pytest.mark.parametrize("n", [5, 60, 140])
-def test_tree_non_finite_values(dev, kv_type, n):
+@pytest.mark.parametrize("n,D", [(5, 64), (60, 64), (140, 64), (14, 128), (14, 256), (30, 256)])
+def test_tree_non_finite_values(dev, kv_type, n, D):
     """A node's NaN or infinite K or V reaches the nodes that see it and no other."""
     import torch
-    G, H, D, page, total = 2, 4, 64, 16, n + 45
+    G, H, page, total = 2, 4, 16, n + 45
     for what, value in (("k", float("nan")), ("v", float("nan")), ("v", float("inf")),
                         ("k", float("inf"))):
         note(f"tree non-finite {kv_type} {what}={value} n={n}")
