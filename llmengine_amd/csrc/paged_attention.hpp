@@ -766,6 +766,12 @@ __device__ __forceinline__ bool join_parts(const Shared& sh, const Segment& s, i
   if (count > 1) {
     if (!last_to_arrive(tile + first * kCounterStride + 1, count, shared)) return false;
     join(first, 1, count);
+    // Every wave has read the part `first` before it is written over: all of them read the maxima
+    // and sums of few rows, and one writes them.
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
     keep(first);
   }
   const int groups = (s.parts + size - 1) / size;

@@ -972,3 +972,19 @@ def test_tree_widest_masks(dev):
     note("tree widest masks")
     b = Trees(dev, "f16", 1, 1, 64, 64, [(n, n + 100, "tree"), (3, 9, "tree")], words=64)
     b.check(b.run())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+def test_tree_joined_groups_weigh_parts_by_their_own_maxima(dev, kv_type, D):
+    """Tiles of 9 to 32 rows in more than 12 parts, a group of which is joined into the place of
+    its first one while other waves may still read that one's maxima and sums.  Logits of a
+    standard deviation of 8: the parts' maxima are apart by more than the tolerance, so that
+    sums weighed by another part's show; the same bits on every run."""
+    for n, total in ((9, 12000), (13, 9000), (16, 14001), (17, 11000), (26, 8000), (32, 15000)):
+        note(f"tree joined groups {kv_type} D={D} {n} over {total}")
+        b = Trees(dev, kv_type, 1, 1, D, 64, [(n, total, "tree")], seed=n, scale=4 * D ** -0.5)
+        out = b.run().clone()
+        b.check(out)
+        for _ in range(12):
+            assert bool((b.run() == out).all())
