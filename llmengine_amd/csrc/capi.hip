@@ -1575,18 +1575,57 @@ int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* 
   if (mle::paged_keep_blocks(most, sequences, caches->kv_heads) >= mle::kMostBlocks)
     return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx +
                                      ": layers * sequences * kv_heads take more than 2^32 threads");
-  // Other workgroups read these while the lengths are written.
-  const struct { const int32_t* p; const char* name; int64_t n; } read[] = {
-      {kv_lens, "kv_lens", sequences},
-      {cu_tokens, "cu_tokens", (int64_t)sequences + 1},
-      {granted, "granted", sequences},
-      {keep_counts, "keep_counts", sequences},
-      {keep, "keep", (int64_t)sequences * keep_stride},
-      {block_table, "block_table", (int64_t)sequences * max_pages}};
-  for (const auto& r : read)
-    if (kept_lens < r.p + r.n && r.p < kept_lens + sequences)
-      return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": kept_lens must not overlap " +
-                                            r.name + ", which the move reads");
+  // What is written is nothing else's: workgroups read the arrays while one writes these three, and
+  // all write the caches.  The count may take its own place.
+  struct Range {
+    const void* p;
+    size_t bytes;
+    const char* name;
+  };
+  const size_t rows = (size_t)sequences, word = sizeof(int32_t);
+  const bool stack = free_pages != nullptr;
+  const Range written[] = {{kept_lens, rows * word, "kept_lens"},
+                           {free_pages, stack ? caches->num_pages * word : 0, "free_pages"},
+                           {free_count_out, stack ? word : 0, "free_count_out"}};
+  const Range read[] = {{kv_lens, rows * word, "kv_lens"},
+                        {cu_tokens, (rows + 1) * word, "cu_tokens"},
+                        {granted, rows * word, "granted"},
+                        {keep_counts, rows * word, "keep_counts"},
+                        {keep, rows * keep_stride * word, "keep"},
+                        {block_table, rows * max_pages * word, "block_table"},
+                        {free_count, stack ? word : 0, "free_count"}};
+  auto overlap = [](const Range& x, const Range& y) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+    return x.bytes != 0 && y.bytes != 0 && (a < b ? b - a < x.bytes : a - b < y.bytes);
+  };
+  auto refused = [&](const Range& x, const std::string& other) {
+    return fail(MLE_INVALID_ARGUMENT,
+                std::string("hip ") + ctx + ": " + x.name + " must not overlap " + other);
+  };
+  for (const Range& w : written) {
+    for (const Range& r : read) {
+      const bool in_place = &w == written + 2 && &r == read + 6 && w.p == r.p;  // the count
+      if (overlap(w, r) && !in_place)
+        return refused(w, std::string(r.name) + ", which the call reads");
+    }
+    for (const Range* o = &w + 1; o != std::end(written); ++o)
+      if (overlap(w, *o)) return refused(w, std::string(o->name) + ", which the call writes too");
+  }
+  const size_t cells = (size_t)caches->num_pages * caches->page_size * caches->kv_heads;
+  const bool bytes = caches->type == MLE_KV_INT8;
+  const size_t held = cells * caches->head_dim * (bytes ? 1 : 2);
+  const size_t scales = bytes ? cells * sizeof(float) : 0;
+  for (int i = 0; i < layers; ++i) {
+    const mle_paged_cache& c = caches[i];
+    const Range parts[] = {{c.k, held, ""}, {c.v, held, ""}, {c.k_scale, scales, ""},
+                           {c.v_scale, scales, ""}};
+    for (const Range& part : parts) {
+      for (const Range& w : written)
+        if (overlap(w, part)) return refused(w, "cache " + std::to_string(i));
+      for (const Range& r : read)
+        if (overlap(r, part)) return refused(r, "cache " + std::to_string(i));
+    }
+  }
   mle::KeepArgs a{};
   a.num_pages = caches->num_pages;
   a.page_size = caches->page_size;

@@ -142,6 +142,54 @@ def test_keep_refusals(bad, code, text):
     assert got == code and text in msg, (got, msg)
 
 
+# What keep reads and writes, each in a place of its own.
+APART = {n: 0x100000 + 0x1000 * i for i, n in enumerate(
+    ("kv_lens", "cu_tokens", "granted", "keep_counts", "keep", "block_table", "free_count",
+     "kept_lens", "free_pages", "free_count_out"))}
+
+
+@pytest.mark.parametrize("written,size", [("kept_lens", 8), ("free_pages", 32),
+                                          ("free_count_out", 4)])
+@pytest.mark.parametrize("other", list(APART))
+def test_keep_writes_over_nothing(written, size, other):
+    """No array that the call writes may lie over another, in any part of either."""
+    if other == written:
+        return
+    sizes = dict(kv_lens=8, cu_tokens=12, granted=8, keep_counts=8, keep=24, block_table=32,
+                 free_count=4, kept_lens=8, free_pages=32, free_count_out=4)
+    for off in {0, 4 - size, sizes[other] - 4}:
+        if (written, other, off) == ("free_count_out", "free_count", 0):
+            continue
+        got, msg = keep(**{**APART, written: APART[other] + off})
+        assert got == INVALID and written in msg and other in msg, (off, got, msg)
+        assert "must not overlap" in msg
+
+
+def test_keep_count_in_place():
+    """The count may take its own place (what is refused then comes later), not another's."""
+    same = {**APART, "free_count_out": APART["free_count"]}
+    got, msg = keep([layer(0), layer(500)], **{**same, "kept_lens": 3 * FAKE + 8})
+    assert got == INVALID and "kept_lens must not overlap cache 0" in msg, (got, msg)
+    for other in ("kv_lens", "kept_lens", "free_pages"):
+        got, msg = keep(**{**same, other: APART["free_count"]})
+        assert got == INVALID and "must not overlap" in msg and "cache" not in msg, (got, msg)
+
+
+@pytest.mark.parametrize("name", list(APART))
+@pytest.mark.parametrize("kv_type", ["f16", "int8"])
+def test_keep_arrays_outside_the_caches(name, kv_type):
+    """Nor may the caches, which the moves write, lie over an array: their last bytes here."""
+    size = dict(f16=2, int8=1)[kv_type] * 8 * 16 * 2 * 64
+    at = dict(k=0x400000, v=0x500000)
+    if kv_type == "int8":
+        at.update(k_scale=0x600000, v_scale=0x700000)
+    for part, base in at.items():
+        last = base + (8 * 16 * 2 * 4 if "scale" in part else size) - 4
+        got, msg = keep([layer(500, kv_type=kv_type, **{n: 0x800000 for n in at if "s" in n}),
+                         cache(kv_type=kv_type, **at)], **{**APART, name: last})
+        assert got == INVALID and name + " must not overlap cache 1" in msg, (part, got, msg)
+
+
 @pytest.mark.parametrize("other", [dict(num_pages=9), dict(page_size=32), dict(kv_heads=1),
                                    dict(head_dim=128), dict(kv_type="bf16")])
 def test_keep_of_unlike_caches(other):
