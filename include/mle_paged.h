@@ -245,9 +245,9 @@ int mle_paged_tree_attention(const mle_paged_cache* cache, const float* q, int q
  *   back, the counts may be NULL (a second group of layers).
  * A token in a page outside [0, num_pages) neither moves nor is written over.  One launch for
  * up to 64 layers; no workspace.  Deterministic.
- * Errors: NULL or misaligned pointers, sizes <= 0, the same cache twice, kept_lens,
- * free_pages [num_pages] or free_count_out over another array's memory (but for free_count in
- * its own place), any array over a cache's -> InvalidArgument;
+ * Errors: NULL or misaligned pointers, sizes <= 0, one memory as two of the caches' k and v (or
+ * scales), kept_lens, free_pages [num_pages] or free_count_out over another array's memory (but
+ * for free_count in its own place), any array over a cache's -> InvalidArgument;
  * caches of different type or sizes -> ShapeMismatch; more than 31 bits of max_pages *
  * page_size or sequences * max_pages, or as many threads as a launch does not hold (64 for
  * each layer, request and KV head) -> Unsupported.

@@ -1546,11 +1546,17 @@ int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* 
       return fail(MLE_SHAPE_MISMATCH, std::string("hip ") + ctx + ": cache " +
                                           std::to_string(i) +
                                           " differs from cache 0 in type or sizes");
-    for (int j = 0; j < i; ++j)
-      if (caches[i].k == caches[j].k || caches[i].v == caches[j].v)
+    for (int j = 0; j <= i; ++j) {
+      const mle_paged_cache &x = caches[i], &y = caches[j];
+      auto twice = [&](const void* xk, const void* xv, const void* yk, const void* yv) {
+        return (j < i && (xk == yk || xv == yv)) || xk == yv || xv == yk;
+      };
+      if (twice(x.k, x.v, y.k, y.v) ||
+          (x.type == MLE_KV_INT8 && twice(x.k_scale, x.v_scale, y.k_scale, y.v_scale)))
         return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": caches " +
                                               std::to_string(j) + " and " + std::to_string(i) +
                                               " are the same memory");
+    }
   }
   const struct { const void* p; const char* name; bool need; } bufs[] = {
       {block_table, "block_table", true}, {kv_lens, "kv_lens", true},

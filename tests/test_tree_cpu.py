@@ -185,8 +185,9 @@ def test_keep_arrays_outside_the_caches(name, kv_type):
         at.update(k_scale=0x600000, v_scale=0x700000)
     for part, base in at.items():
         last = base + (8 * 16 * 2 * 4 if "scale" in part else size) - 4
-        got, msg = keep([layer(500, kv_type=kv_type, **{n: 0x800000 for n in at if "s" in n}),
-                         cache(kv_type=kv_type, **at)], **{**APART, name: last})
+        scales = dict(k_scale=0x800000, v_scale=0x900000) if kv_type == "int8" else {}
+        got, msg = keep([layer(500, kv_type=kv_type, **scales), cache(kv_type=kv_type, **at)],
+                        **{**APART, name: last})
         assert got == INVALID and name + " must not overlap cache 1" in msg, (part, got, msg)
 
 
@@ -204,6 +205,22 @@ def test_keep_of_a_cache_twice():
     for other in (layer(0), cache(k=99 * FAKE, v=4 * FAKE), cache(k=3 * FAKE, v=99 * FAKE)):
         got, msg = keep([layer(0), layer(1), other])
         assert got == INVALID and "caches 0 and 2 are the same memory" in msg, (got, msg)
+
+
+def test_keep_of_k_that_is_v():
+    """One layer's K that is another's V, or its own, would be moved as both."""
+    for caches, which in (
+            ([layer(0), layer(1), cache(k=99 * FAKE, v=3 * FAKE)], "0 and 2"),
+            ([layer(0), layer(1), cache(k=6 * FAKE, v=99 * FAKE)], "1 and 2"),
+            ([layer(0), cache(k=98 * FAKE, v=98 * FAKE)], "1 and 1")):
+        got, msg = keep(caches)
+        assert got == INVALID and f"caches {which} are the same memory" in msg, (got, msg)
+    for scales, which in (((50, 51), "0 and 1"), ((52, 50), "0 and 1"), ((51, 53), "0 and 1"),
+                          ((54, 54), "1 and 1")):
+        got, msg = keep([layer(0, kv_type="int8", k_scale=50 * FAKE, v_scale=51 * FAKE),
+                         layer(1, kv_type="int8", k_scale=scales[0] * FAKE,
+                               v_scale=scales[1] * FAKE)])
+        assert got == INVALID and f"caches {which} are the same memory" in msg, (got, msg)
 
 
 @pytest.mark.parametrize("bad,code,text", [
