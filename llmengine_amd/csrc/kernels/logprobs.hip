@@ -253,7 +253,6 @@ __device__ void select_of(int count, F key, int k, uint64_t* out, SelectLds& sm)
   for (int shift = 56; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += kThreads) sm.hist[i] = 0;
     __syncthreads();
-#pragma unroll 4
     for (int i = tid; i < past; i += kThreads) {
       const uint64_t v = i < count ? key(i) : 0;
       count_bin(sm.hist, (uint32_t)(v >> shift) & 255u, v != 0 && (v & mask) == prefix);
@@ -441,7 +440,7 @@ __device__ __forceinline__ void select_tokens(const Args& a, int64_t r, const Ma
           for (int e = 0; e < 4; ++e)
             if (at + e < n) most = fmaxf(most, scaled(a, v[e]));
         },
-        [](auto&, auto&) {});
+        [](const uint32_t (&)[kAtOnce], const f4 (&)[kAtOnce]) {});
   } else {
     maxima.each([&](int, float v) { most = fmaxf(most, v); });
   }

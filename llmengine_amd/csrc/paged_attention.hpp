@@ -346,7 +346,10 @@ __device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int b) {
   int c0 = a.cu[b], c1 = a.cu[b + 1], len = a.kv_lens[b];
   c0 = c0 < 0 ? 0 : c0 < a.tokens ? c0 : a.tokens;
   c1 = c1 < c0 ? c0 : c1 < a.tokens ? c1 : a.tokens;
-  Seq s{c0, c1 - c0, (len < 0 ? 0 : len) - (c1 - c0)};
+  Seq s{};
+  s.row0 = c0;
+  s.n = c1 - c0;
+  s.pos0 = (len < 0 ? 0 : len) - s.n;
   read_kind(a, b, s);
   return s;
 }
@@ -1044,7 +1047,7 @@ struct FewRows {
 #pragma unroll
       for (int i = 0; i < NJ; ++i)
         if (Part::has(at, i, bits))
-          *reinterpret_cast<f32x4*>(o + (at + i * kThreads >> bits) * 4) =
+          *reinterpret_cast<f32x4*>(o + ((at + i * kThreads) >> bits) * 4) =
               L != 0.0f ? out[i] * inv : f32x4{};
     }
   }
@@ -1238,7 +1241,7 @@ struct FewRows {
         } else if (careful) {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            if (!__any(any_nan(sc[r]) & finite(r))) continue;
+            if (!__any((int)any_nan(sc[r]) & (int)finite(r))) continue;
             const AttentionArgs a = fresh_args();
             const int me = fresh(lane), place = r * 16 + (me & 15);
             const int in = (R > 1 ? s.r0 : 0) + (place < s.rows ? place : s.rows - 1);
@@ -1426,7 +1429,7 @@ struct FewRows {
 #pragma unroll
           for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[r][db][i], 0.0f, zero);
         // A row of q that is not finite is NaN either way.
-        if (__any(zero != zero) && __any((zero != zero) & finite(r))) again = true;
+        if (__any(zero != zero) && __any((int)(zero != zero) & (int)finite(r))) again = true;
       }
       if (again) {
         begin();
@@ -1869,7 +1872,7 @@ struct ManyRows {
                 sc[b4 * 4 + i] = __builtin_fmaf(sc[b4 * 4 + i] * c, k4[i], l4[i]);
             }
           }
-          if (!kBytes<T> && kSecond && __any(any_nan(sc) & finite_q(qp))) {
+          if (!kBytes<T> && kSecond && __any((int)any_nan(sc) & (int)finite_q(qp))) {
             const AttentionArgs a = fresh_args();
             const int me = fresh_tid(), in = (me >> 6) * 32 + (me & 31);
             const int row = s.r0 + (in < s.rows ? in : s.rows - 1);
@@ -2097,7 +2100,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attention_kernel(A
   int tiles = 0;
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
-    Seq s{0, 0, 0};
+    Seq s{};
     if (b < a.sequences) s = seq_of(a, b);
     sch.seq[tid] = s;
     const Cost c = cost_of<T, D>(a, s);
