@@ -1283,7 +1283,9 @@ int mle_token_logprobs_workspace_size(int rows, int n, int top_n, size_t* bytes,
   MLE_TRY(check_ptrs(ctx, bytes, "bytes", counters, "counters", counters, "counters"));
   MLE_TRY(check_positive(ctx, rows, "rows"));
   MLE_TRY(check_positive(ctx, n, "n"));
-  if (top_n < 0 || top_n > mle::kTopTokensMax || rows > 65535)
+  if (top_n < 0)
+    return fail(MLE_INVALID_ARGUMENT, std::string("hip ") + ctx + ": top_n must not be negative");
+  if (top_n > mle::kTopTokensMax || rows > 65535)
     return fail(MLE_UNSUPPORTED, std::string("hip ") + ctx + ": at most 65535 rows, top_n 0 to " +
                                      std::to_string(mle::kTopTokensMax));
   const mle::SplitKNeed need = mle::token_logprobs_workspace(rows, n, top_n);

@@ -261,3 +261,13 @@ def test_logprobs_workspace_size():
     assert lib.mle_token_logprobs_workspace_size(1, 5, 129, ctypes.byref(n),
                                                  ctypes.byref(n)) == UNSUPPORTED
     assert lib.mle_token_logprobs_workspace_size(1, 5, 1, None, ctypes.byref(n)) == INVALID
+
+
+def test_logprobs_workspace_refusals():
+    """As the call's own: a negative top_n is no argument, one too large is not supported."""
+    n = ctypes.c_size_t()
+    size = capi.load().mle_token_logprobs_workspace_size
+    for args, code in (((1, 5, -1), INVALID), ((1, 0, 1), INVALID), ((-1, 5, 1), INVALID),
+                       ((65536, 5, 1), UNSUPPORTED), ((1, 5, 129), UNSUPPORTED)):
+        assert size(*args, ctypes.byref(n), ctypes.byref(n)) == code, args
+        assert "token_logprobs_workspace_size" in capi.last_error()
