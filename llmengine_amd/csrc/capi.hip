@@ -1623,11 +1623,22 @@ int mle_paged_kv_keep(const mle_paged_cache* caches, int layers, const int32_t* 
   const bool bytes = caches->type == MLE_KV_INT8;
   const size_t held = cells * caches->head_dim * (bytes ? 1 : 2);
   const size_t scales = bytes ? cells * sizeof(float) : 0;
+  // Seldom is any array near a cache: where they lie together first.
+  uintptr_t lo = UINTPTR_MAX, hi = 0;
+  auto widen = [&](const Range& r) {
+    if (r.bytes == 0) return;
+    lo = std::min(lo, reinterpret_cast<uintptr_t>(r.p));
+    hi = std::max(hi, reinterpret_cast<uintptr_t>(r.p) + r.bytes);
+  };
+  for (const Range& w : written) widen(w);
+  for (const Range& r : read) widen(r);
+  const Range all{reinterpret_cast<const void*>(lo), hi - lo, ""};
   for (int i = 0; i < layers; ++i) {
     const mle_paged_cache& c = caches[i];
     const Range parts[] = {{c.k, held, ""}, {c.v, held, ""}, {c.k_scale, scales, ""},
                            {c.v_scale, scales, ""}};
     for (const Range& part : parts) {
+      if (!overlap(all, part)) continue;
       for (const Range& w : written)
         if (overlap(w, part)) return refused(w, "cache " + std::to_string(i));
       for (const Range& r : read)
