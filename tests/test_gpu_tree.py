@@ -988,3 +988,42 @@ def test_tree_joined_groups_weigh_parts_by_their_own_maxima(dev, kv_type, D):
         b.check(out)
         for _ in range(12):
             assert bool((b.run() == out).all())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("D", [96, 128, 256])
+def test_tree_several_tiles_a_workgroup(dev, kv_type, D):
+    """More tiles than workgroups, several one after the other in each: trees of 17 to 64 rows
+    only, whose next loads go out before a tile is joined, and all heights in turn with runs
+    between; the same bits again."""
+    rng = np.random.default_rng(D)
+    some = [(n, n + int(rng.choice([0, 3, 60, 200])), "tree")
+            for n in rng.integers(17, 65, 300).tolist()]
+    kinds = ["tree", "any", "run", "chain", "tree", "none", "tree"]
+    mixed = []
+    for b in range(300):
+        n = int(rng.choice([0, 1, 7, 8, 9, 15, 16, 17, 24, 31, 32, 33, 40, 70]))
+        mixed.append((n, n + int(rng.choice([0, 1, 40, 150])), kinds[b % 7]))
+    for lens, H, G, window in ((some, 2, 2, 50), (mixed, 6, 3, 0)):
+        note(f"tree several tiles {kv_type} D={D} H={H} G={G} window={window}")
+        b = Trees(dev, kv_type, H, G, D, 16, lens, seed=D + H, window=window)
+        out = b.run().clone()
+        b.check(out)
+        for _ in range(3):
+            assert bool((b.run() == out).all())
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_tree_chain_is_near_the_run(dev, kv_type):
+    """A tree without branches is a run of tokens.  The tiles, cuts and joins of the two calls
+    differ, so their sums do, each by the tolerance at most."""
+    import torch
+    for lens, D in (([(1, 700), (9, 3000), (2, 2)], 64), ([(100, 700), (33, 60)], 128),
+                    ([(40, 900), (17, 5000)], 256)):
+        note(f"tree chain and run {kv_type} {lens}")
+        b = Trees(dev, kv_type, 4, 2, D, 32, [(n, t, "chain") for n, t in lens], seed=D)
+        trees, runs = b.run(), empty_f32((b.T, 4 * D), dev)
+        capi.paged_attention(b.cache, b.q, runs, 4, b.scale, 0, b.table, b.max_pages, b.kv_lens,
+                             b.cu, len(lens), b.T)
+        torch.cuda.synchronize()
+        assert (trees - runs).abs().max().item() <= 2 * b.tol
