@@ -249,8 +249,10 @@ int mle_top_tokens_f32(const float* logits, int rows, int n, int top_n, float te
  *   top_ids, top_logprobs[r][j], j < min(top_n, n): the tokens of largest probability and
  *     their log probabilities, largest first, ties to the lower id.
  * A row whose maximum is not finite or that holds a NaN is the uniform distribution 1 / n,
- * as mle_top_tokens_f32 has it.  Sums are of 64 bits: log p is good to fp32 rounding also
- * where it is near 0.  tokens_per_row 0, entropy NULL and top_n 0 leave a part out.
+ * as mle_top_tokens_f32 has it.  A term e^(x - max) is good to 2^-22 (|x - max| + 1) of itself,
+ * sums are of 64 bits: so is log p where it is near 0, where it is what the other terms add up
+ * to, and with fp32's rounding elsewhere.  tokens_per_row 0, entropy NULL and top_n 0 leave a
+ * part out.
  * Takes the per-stream workspace; mle_token_logprobs_workspace_size says how much any call of
  * up to these sizes takes (mle_workspace_reserve, before a graph is captured).
  * Errors: NULL pointers of a part asked for, rows or n <= 0, tokens_per_row or top_n < 0

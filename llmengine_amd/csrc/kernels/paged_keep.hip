@@ -14,6 +14,8 @@
 // nodes, up to 8 of them kept, in 32 layers of 8-bit pages 20 us (13 where the lines are in a
 // cache still).  With 48 kept of each 150 us, one entry at a time 232, 4 160; of f16 pages 267,
 // 340 and 194, but 4 take 24 us instead of 16 where up to 8 are kept, as most paths are.
+// (All with the pieces of 16 bits' K in scratch memory, 144 bytes a lane, where the compiler puts
+// an array of class type that is filled under a condition; of 8 bits there is none.)
 #include "../paged.hpp"
 
 namespace mle {

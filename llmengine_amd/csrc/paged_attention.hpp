@@ -63,8 +63,8 @@
 //   trees: as few or many rows, by the query heads of their nodes.  8 nodes over 129 tokens, 14
 //     heads 11.4 us.  16 trees of 26 over up to 4096, 32 heads (383 MB) 90 us = 4.3 TB/s: 5 us
 //     of beginning, units of 2.4 us beside another workgroup, runs that end between 64 and 94.
-//     8 trees of 64 over up to 32768 of 8 bits, 32 heads over 8 201 us = 0.79 PFLOP/s of parts:
-//     matrix cores busy in 34% of the cycles, 1.5 waves a SIMD, since of the two workgroups of a
+//     8 trees of 64 over up to 32768 of 8 bits, 32 heads over 8 198-200 us = 0.79 PFLOP/s of parts:
+//     matrix cores busy in 35% of the cycles, 1.5 waves a SIMD, since of the two workgroups of a
 //     CU the older one's waves go first and it is done at 165 us, the other by 206.  Priorities
 //     that changed from unit to unit brought their ends together, longer runs for the older ones
 //     likewise, and the call was no shorter by either.
@@ -469,7 +469,8 @@ struct Cost {
   // The least one at a tile's end.  A tile's fixed cost is in the account where it begins, so a
   // run that takes up only its end, and goes on with the next, is no longer than others; one
   // prolonged to the tile's end is, and the next is shorter (2 x 40 rows of 32 heads over 600 keys
-  // 27 us so and 22 with this, 64 of 28 over 20000 73 and 64).
+  // 27 us so and 22 with this, 64 of 28 over 20000 73 and 64; but 32 x 8 of 14 over
+  // up to 8192 29 and 31).
   __device__ __forceinline__ int last() const { return kTrees ? least - fixed : least; }
 
   __device__ __forceinline__ int of(int t) const {
